@@ -17,6 +17,7 @@
 #include <cstdlib>
 #include "dpipe_common.h"
 #include "lds_dma_tiles.h"
+#include "attention_tiles.h"
 #include "../../include/dpipe_hip.h"
 
 using namespace dpipe;
@@ -43,32 +44,6 @@ struct AttnParams {
 // behind a LayerNorm usually do) both are ~ dO . c and the difference is what matters: the 2^-9 rounding of a bf16 O then lands on dS, dQ and dK amplified by
 // |c| / |v_j| (measured on the full-size SDXL step: 8 % of sum|g| on the to_q / to_k weights of the deepest self-attentions; a host simulation with |c| = 3 |v_j|:
 // dQ 25 % off with the bf16 O, 1.4 % with the fp32 one).  The forward therefore stores O a second time in fp32 for the backward (optional: NULL = bf16 O).
-
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
-
-__device__ __forceinline__ f32x16 mfma16(bf16x8_t a, bf16x8_t b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_mfma, a), __builtin_bit_cast(bf16x8_mfma, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 zero16() {
-    f32x16 z;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) z[e] = 0.f;
-    return z;
-}
-__device__ __forceinline__ bf16x8_t zero_frag() {
-    bf16x8_t z;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = 0;
-    return z;
-}
-// 8 consecutive accumulator entries (e0 .. e0+7) -> bf16 MFMA operand
-__device__ __forceinline__ bf16x8_t pack_frag(const f32x16& s, int e0) {
-    uint4 u;
-    u.x = pack_bf16x2(s[e0 + 0], s[e0 + 1]); u.y = pack_bf16x2(s[e0 + 2], s[e0 + 3]);
-    u.z = pack_bf16x2(s[e0 + 4], s[e0 + 5]); u.w = pack_bf16x2(s[e0 + 6], s[e0 + 7]);
-    return __builtin_bit_cast(bf16x8_t, u);
-}
 
 // ---- LDS tiles: `ROWS` rows of D bf16, row stride RS bytes ------------------------------------------------------
 // A/B fragment with the K index along the row (contiguous): lane (i, h) reads 8 bf16 at (row0 + i, col + 8h).

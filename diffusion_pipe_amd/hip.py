@@ -16,7 +16,7 @@ import os
 LIB_PATH = Path(os.environ.get('DPIPE_HIP_LIB') or Path(__file__).resolve().parent / 'libdpipe_hip.so')
 
 BF16, F32 = 0, 1
-ABI_VERSION = 10                     # DPIPE_ABI_VERSION of include/dpipe_hip.h this binding was written against
+ABI_VERSION = 11                     # DPIPE_ABI_VERSION of include/dpipe_hip.h this binding was written against
 CONV_OUT_F32, CONV_ACCUMULATE, CONV_BIAS_PER_SAMPLE, CONV_BIAS_HILO = 1, 2, 4, 8  # dpipe_conv2d_fwd / _dgrad `flags`
 OPT_ATTN_FWD_DMA, OPT_ATTN_BWD_DMA, OPT_ATTN_DQ8, OPT_ATTN_DKV_SPLIT, OPT_GEMM_SHALLOW, OPT_GEMM_BIG_TILES = 0, 1, 2, 3, 4, 5     # dpipe_set_option ids (include/dpipe_hip.h)
 ACT = {None: 0, 'none': 0, 'gelu_tanh': 1, 'gelu': 2, 'gelu_erf': 2, 'silu': 3, 'quick_gelu': 4}
@@ -104,6 +104,13 @@ _SIGNATURES = {
     'dpipe_attn_fwd': (I, [P, P, P, P, P, P, I, I, I, I, I] + [L] * 12 + [F, I, P, P]),
     'dpipe_attn_bwd_partial_floats': (L, [I, I, I, I, I]),
     'dpipe_attn_bwd': (I, [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I] + [L] * 24 + [F, I, P, L, P, P]),
+    'dpipe_attn_varlen_fwd_workspace_floats': (L, [L, L, I, I, I, I]),
+    'dpipe_attn_varlen_fwd': (I, [P] * 9 + [L, L, L, I, I, I, I] + [L] * 6 + [F, I, P]),
+    'dpipe_attn_varlen_bwd_workspace_floats': (L, [L, L, I, I, I, I]),
+    'dpipe_attn_varlen_bwd': (I, [P] * 13 + [L, L, L, I, I, I, I] + [L] * 8 + [F, I, P]),
+    'dpipe_rope_axes_fwd': (I, [P, P, P, I, P, P, P, P, P, P, L, L, I, I, I, I, I] + [L] * 4 + [F, I, I, I, I, P]),
+    'dpipe_rope_axes_workspace_floats': (L, [I]),
+    'dpipe_rope_axes_bwd': (I, [P, P, P, P, P, I] + [P] * 9 + [L, L, I, I, I, I, I] + [L] * 8 + [F] + [I] * 6 + [P]),
 }
 
 _lib = None

@@ -3,6 +3,8 @@
 Every function here launches gfx950 kernels from libdpipe_hip.so on the current HIP stream; there is no PyTorch /
 CPU fallback (a CPU tensor or a missing library raises `DpipeHipError`).  Reference semantics are cited per op.
 """
+import ctypes
+import functools
 import math
 import os as _os_mod
 
@@ -1397,6 +1399,142 @@ def rms_norm_rope(x, weight, cos, sin, eps=1e-6, per_head=True, token_offset=0, 
     return _RMSNormRopeFn.apply(x, weight, cos, sin, eps, per_head, token_offset, rope_tokens)
 
 
+# Rotary positions from the positions themselves: several axes, any position per token, query and key heads in one launch
+def _head_rows(x):
+    """x [..., H, D] as rows the kernels walk by (token stride, head stride): (tensor, tokens, H, D, token stride, head stride).  A view with one uniform token stride (a column block
+    of a fused projection) is taken as it is; anything else, or an address that is not 16-byte aligned, is copied once."""
+    H, D = x.shape[-2:]
+    tokens = x.numel() // (H * D) if H * D else 0
+    ok = x.stride(-1) == 1 and x.stride(-2) % 8 == 0 and x.data_ptr() % 16 == 0
+    ss, span = None, 1
+    for size, st in reversed(list(zip(x.shape[:-2], x.stride()[:-2]))):
+        if size == 1:
+            continue
+        if ss is None:
+            ss = st
+        elif st != ss * span:
+            ok = False
+        span *= size
+    ss = H * D if ss is None else ss
+    if not ok or ss % 8 or not D <= ss < 2 ** 23:
+        x, ss = x.clone(memory_format=torch.contiguous_format), H * D
+    return x, tokens, H, D, ss, x.stride(-2)
+
+
+@functools.lru_cache(maxsize=64)
+def _rope_axes_tables(axes_dim, theta, shared):
+    """host tables of the kernel: (turns per unit of position, axis) of every channel pair, in fp64"""
+    total, freq, axis = sum(axes_dim), [], []
+    for a, dim in enumerate(axes_dim):
+        for j in range(dim // 2):
+            e = -2.0 * len(freq) / total if shared else -2.0 * j / dim
+            freq.append(theta[a] ** e / (2.0 * math.pi))
+            axis.append(a)
+    return (ctypes.c_double * len(freq))(*freq), (ctypes.c_int * len(axis))(*axis), len(freq)
+
+
+_POSITION_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
+
+
+class _RopeAxesFn(Function):
+    """q', k' = R(positions) [rms_norm](q, k); see rope_axes.  The backward re-derives the norm's statistics from q / k: nothing but the inputs is kept."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, q_weight, k_weight, tables, eps, half):
+        q, tokens, hq, D, q_ss, q_sh = _head_rows(q)
+        yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        hk = k_ss = k_sh = 0
+        yk = None
+        if k is not None:
+            k, _, hk, _, k_ss, k_sh = _head_rows(k)
+            yk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        freq, axis, pairs = tables
+        period, axes = positions.numel() // positions.shape[-1], positions.shape[-1]
+        meta = (tokens, period, axes, pairs, hq, hk, D)
+        wd = [dtype_code(w.dtype) if w is not None else dtype_code(q.dtype) for w in (q_weight, k_weight)]
+        wq, wk = _al(q_weight), _al(k_weight)
+        if tokens:
+            check(lib().dpipe_rope_axes_fwd(ptr(q), ptr(k), ptr(positions), _POSITION_TYPES[positions.dtype], freq, axis, ptr(wq), ptr(wk), ptr(yq), ptr(yk), *meta,
+                                            q_ss, q_sh, k_ss, k_sh, float(eps), int(half), dtype_code(q.dtype), *wd, stream()), 'rope_axes_fwd')
+        ctx.save_for_backward(q if wq is not None or wk is not None else None, k if wq is not None or wk is not None else None, positions, q_weight, k_weight)
+        ctx.meta = (meta, tables, (q_ss, q_sh, k_ss, k_sh), wd, eps, half, q.shape, k.shape if k is not None else None, q.dtype)
+        return yq, yk
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        q, k, positions, q_weight, k_weight = ctx.saved_tensors
+        meta, (freq, axis, _), strides, wd, eps, half, q_shape, k_shape, dtype = ctx.meta
+        tokens, D = meta[0], meta[-1]
+        with torch.cuda.device(gq.device):
+            gq, _, _, _, gq_ss, gq_sh = _head_rows(gq)
+            dq = torch.empty(q_shape, device=gq.device, dtype=dtype)
+            dk, gk_ss, gk_sh = None, 0, 0
+            if k_shape is not None:
+                gk, _, _, _, gk_ss, gk_sh = _head_rows(gk)
+                dk = torch.empty(k_shape, device=gq.device, dtype=dtype)
+            normed = q_weight is not None or k_weight is not None
+            if not normed:
+                q, k, strides = gq, (gk if k_shape is not None else None), (gq_ss, gq_sh, gk_ss, gk_sh)
+            dw, fused = [None, None], [False, False]
+            for i, w in enumerate((q_weight, k_weight)):
+                if w is not None and ctx.needs_input_grad[3 + i]:
+                    dw[i] = _accum_target(w)
+                    fused[i] = dw[i] is not None
+                    if dw[i] is None:
+                        dw[i] = torch.empty_like(w) if tokens else torch.zeros_like(w)
+            if tokens:
+                ws = torch.empty(lib().dpipe_rope_axes_workspace_floats(D), device=gq.device, dtype=torch.float32) if normed else None
+                check(lib().dpipe_rope_axes_bwd(ptr(q), ptr(k), ptr(gq), ptr(gk) if k_shape is not None else None, ptr(positions), _POSITION_TYPES[positions.dtype], freq, axis,
+                                                ptr(_al(q_weight)), ptr(_al(k_weight)), ptr(dq), ptr(dk), ptr(dw[0]), ptr(dw[1]), ptr(ws), *meta, *strides,
+                                                gq_ss, gq_sh, gk_ss, gk_sh, float(eps), int(half), dtype_code(dtype), *wd,
+                                                _acc_all(fused[0], dw[0]), _acc_all(fused[1], dw[1]), stream()), 'rope_axes_bwd')
+        return dq, dk, None, (None if fused[0] else dw[0]), (None if fused[1] else dw[1]), None, None, None
+
+
+def rope_axes(q, k, positions, axes_dim, theta=10000.0, q_weight=None, k_weight=None, eps=1e-6, interleaved=True, shared=False):
+    """Rotary positions with several axes on query and key heads, optionally behind their per-head RMS norms, in one launch; differentiable in q, k and the weights.
+
+    q [..., H, D], k [..., Hk, D] or None (bf16 or fp32, the same leading sizes; D a multiple of 8 up to 256; column blocks of a fused projection are read in place).
+    positions [..., axes] (fp32, int32 or int64): one row per token, or one row per token of the innermost leading sizes, repeated over the outer ones ([S, axes] for q [B, S, H, D]).
+    axes_dim: channels of every axis (even, together at most D; the channels behind them are not rotated), e.g. (16, 56, 56) for (time, height, width).
+    theta: base of the frequencies theta ** (-2 j / dim), one number or one per axis; shared=True: one run of frequencies over all axes' channels together instead.
+    q_weight, k_weight [D]: x * rsqrt(mean(x ** 2) + eps) * weight before the rotation (None: no norm).
+    interleaved: pairs are neighbouring channels (2 p, 2 p + 1); False: the halves (p, p + sum(axes_dim) / 2) of the rotated channels, whose count is a multiple of 8.
+    Angles are formed in fp64 from the positions: far positions keep their precision.  (models/wan/model.py:40-67; diffusers FluxPosEmbed; models/hunyuan_video.py:35-81)
+    -> (q', k'), contiguous; k' is None without k."""
+    axes_dim = tuple(int(a) for a in axes_dim)
+    theta = (float(theta),) * len(axes_dim) if not isinstance(theta, (tuple, list)) else tuple(float(t) for t in theta)
+    if q.dim() < 3 or (k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype)):
+        raise DpipeHipError(f'rope_axes: q [..., H, D] and k [..., Hk, D] of one dtype; got {tuple(q.shape)} {q.dtype} and {(tuple(k.shape), k.dtype) if k is not None else None}')
+    dtype_code(q.dtype)
+    D = q.shape[-1]
+    if D % 8 or not 0 < D <= 256 or q.shape[-2] == 0 or (k is not None and k.shape[-2] == 0):
+        raise DpipeHipError(f'rope_axes: the head dim must be a multiple of 8 up to 256, with at least one head; got {tuple(q.shape)}')
+    if not axes_dim or any(a <= 0 or a % 2 for a in axes_dim) or sum(axes_dim) > D or (not interleaved and sum(axes_dim) % 8) or len(theta) != len(axes_dim) \
+            or any(not (t > 0.0 and math.isfinite(t)) for t in theta) or (shared and len(set(theta)) > 1):
+        raise DpipeHipError(f'rope_axes: even axis sizes that fit the head dim {D} (halves pairing: together a multiple of 8) and a positive theta (shared: one); got {axes_dim}, {theta}')
+    if positions.dtype not in _POSITION_TYPES or positions.requires_grad:
+        raise DpipeHipError(f'rope_axes: positions are fp32, int32 or int64 and have no gradient; got {positions.dtype}')
+    lead = tuple(q.shape[:-2])
+    if positions.dim() < 2 or positions.shape[-1] != len(axes_dim) or tuple(positions.shape[:-1]) != lead[len(lead) - positions.dim() + 1:]:
+        raise DpipeHipError(f'rope_axes: positions {tuple(positions.shape)} do not fit tokens {lead} and {len(axes_dim)} axes')
+    for w in (q_weight, k_weight):
+        if w is not None and tuple(w.shape) != (D,):
+            raise DpipeHipError(f'rope_axes: norm weights have shape [{D}]; got {tuple(w.shape)}')
+    if k is None and k_weight is not None:
+        raise DpipeHipError('rope_axes: a key weight needs k')
+    require_cuda(q, k, positions, q_weight, k_weight)
+    _same_device(q, k, positions, q_weight, k_weight)
+    with torch.cuda.device(q.device):
+        return _RopeAxesFn.apply(q, k, _contig(positions), q_weight, k_weight, _rope_axes_tables(axes_dim, theta, bool(shared)), eps, not interleaved)
+
+
+def _same_device(*tensors):
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise DpipeHipError(f'operands on different devices: {sorted(map(str, devices))}')
+
+
 # -------------------------------------------------------------------------------------------- attention (K4)
 def _bshd_strides(t):
     if t.stride(3) != 1:
@@ -1586,6 +1724,80 @@ def attention(q, k, v, kv_len=None, scale=None, impl='auto', causal=False):
             kv_len = kv_len.to(torch.int32)
         return _FlashAttnFn.apply(q, k, v, kv_len, scale, causal)
     return _UnfusedAttnFn.apply(q, k, v, scale, causal, kv_len)
+
+
+class _AttnVarlenFn(Function):
+    """see attention_varlen; keeps the unrounded output for the backward's delta, as _FlashAttnFn does"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, scale, causal):
+        (q, tq, hq, D, *qs), (k, tk, hk, _, *ks), (v, _, _, _, *vs) = _head_rows(q), _head_rows(k), _head_rows(v)
+        n = cu_q.numel() - 1
+        if tq == 0 or tk == 0:                    # nothing to read: every row is empty
+            ctx.meta = None
+            ctx.shapes = (q.shape, k.shape, v.shape, q.dtype)
+            return torch.zeros(q.shape, device=q.device, dtype=q.dtype)
+        sizes = (tq, tk, n, hq, hk, D)
+        keep = any(ctx.needs_input_grad[:3])
+        o = torch.empty((tq, hq, D), device=q.device, dtype=q.dtype)
+        lse = torch.empty((hq, tq), device=q.device, dtype=torch.float32)
+        o32 = torch.empty((tq, hq, D), device=q.device, dtype=torch.float32) if keep else None
+        need = lib().dpipe_attn_varlen_fwd_workspace_floats(*sizes)
+        ws = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
+        check(lib().dpipe_attn_varlen_fwd(ptr(q), ptr(k), ptr(v), ptr(cu_q), ptr(cu_k), ptr(o), ptr(lse), ptr(o32), ptr(ws), need, *sizes, *qs, *ks, *vs,
+                                          float(scale), int(causal), stream()), 'attn_varlen_fwd')
+        if keep:
+            ctx.save_for_backward(q, k, v, cu_q, cu_k, o32, lse)
+        ctx.meta = (sizes, (*qs, *ks, *vs), scale, causal)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        if ctx.meta is None:
+            *shapes, dtype = ctx.shapes
+            return (*(torch.zeros(sh, device=do.device, dtype=dtype) for sh in shapes), None, None, None, None)
+        q, k, v, cu_q, cu_k, o32, lse = ctx.saved_tensors
+        sizes, strides, scale, causal = ctx.meta
+        tq, tk, _, hq, hk, D = sizes
+        with torch.cuda.device(q.device):
+            do, _, _, _, *ds = _head_rows(do)
+            dq = torch.empty((tq, hq, D), device=q.device, dtype=q.dtype)
+            dk, dv = (torch.empty((tk, hk, D), device=q.device, dtype=q.dtype) for _ in range(2))
+            delta = torch.empty((hq, tq), device=q.device, dtype=torch.float32)
+            need = lib().dpipe_attn_varlen_bwd_workspace_floats(*sizes)
+            ws = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
+            check(lib().dpipe_attn_varlen_bwd(ptr(q), ptr(k), ptr(v), ptr(cu_q), ptr(cu_k), ptr(o32), ptr(do), ptr(lse), ptr(delta), ptr(dq), ptr(dk), ptr(dv), ptr(ws), need,
+                                              *sizes, *strides, *ds, float(scale), int(causal), stream()), 'attn_varlen_bwd')
+        return dq, dk, dv, None, None, None, None
+
+
+def attention_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=False):
+    """softmax(scale q k^T) v over sequences of different lengths packed back to back; bf16, head dim 64 or 128, differentiable in q, k, v.
+
+    q [Tq, H, D], k / v [Tk, Hk, D] with H a multiple of Hk: query head h reads key head h // (H // Hk).  Column blocks of a fused projection are read in place.
+    cu_q, cu_k: int32 offsets [N + 1] on the device, ascending from 0; sequence b holds query tokens cu_q[b] .. cu_q[b + 1] - 1 and key tokens cu_k[b] .. cu_k[b + 1] - 1, either
+    of which may be empty.  cu_k None: the queries' offsets (Tk = Tq).  The lengths are never read on the host: the call can be captured and replayed with other offsets.
+    causal: query i sees key j of its sequence when j - len_k <= i - len_q (the last query sees every key; with equal lengths j <= i).
+    A query that sees no key, and the rows behind the last sequence, give zeros and take and give no gradient, whatever those rows hold (values INSIDE a sequence are expected to be
+    finite: a masked infinity or NaN reaches its sequence's other rows).  The same inputs give the same bits (no atomics).  (models/wan/attention.py:91-122)
+    -> [Tq, H, D]"""
+    cu_k = cu_q if cu_k is None else cu_k
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2] or k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise DpipeHipError(f'attention_varlen: q [Tq, H, D], k and v [Tk, Hk, D] with H a multiple of Hk; got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
+    if not flash_eligible(q.dtype, q.shape[2]) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise DpipeHipError(f'attention_varlen computes in bf16 at head dim 64 or 128; got {q.dtype}, {k.dtype}, {v.dtype}, head dim {q.shape[2]}')
+    for cu in (cu_q, cu_k):
+        if cu.dtype not in (torch.int32, torch.int64) or cu.dim() != 1 or cu.numel() < 2 or cu.numel() != cu_q.numel():
+            raise DpipeHipError(f'attention_varlen: offsets are int32 [N + 1], N >= 1, for queries and keys alike; got {cu.dtype} {tuple(cu.shape)}, {tuple(cu_q.shape)}')
+    if cu_k is cu_q and k.shape[0] != q.shape[0]:
+        raise DpipeHipError(f'attention_varlen: shared offsets need as many keys as queries; got {q.shape[0]} and {k.shape[0]}')
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise DpipeHipError(f'attention_varlen: scale must be positive and finite, got {scale}')
+    require_cuda(q, k, v, cu_q, cu_k)
+    _same_device(q, k, v, cu_q, cu_k)
+    with torch.cuda.device(q.device):
+        return _AttnVarlenFn.apply(q, k, v, _contig(cu_q.to(torch.int32)), _contig(cu_k.to(torch.int32)), scale, bool(causal))
 
 
 # ------------------------------------------------------------------------------------------------- loss (K9)

@@ -37,7 +37,7 @@ extern "C" {
 #define DPIPE_LOSS_SMOOTH_L1 2
 
 /* ABI version: bumped whenever a signature of this header changes; the host binding refuses a library of another version. */
-#define DPIPE_ABI_VERSION 10
+#define DPIPE_ABI_VERSION 11
 int dpipe_version(void);
 const char* dpipe_last_error(void);
 /* Kernel-selection options (process-wide; for A/B timing and for testing the fallback kernels -- every default is the measured-faster choice).
@@ -375,6 +375,38 @@ int dpipe_attn_bwd(const void* q, const void* k, const void* v, const void* o, c
                    long o_sb, long o_ss, long o_sh, long do_sb, long do_ss, long do_sh, long dq_sb, long dq_ss,
                    long dq_sh, long dk_sb, long dk_ss, long dk_sh, long dv_sb, long dv_ss, long dv_sh, float scale,
                    int causal, float* dkv_partial, long dkv_partial_floats, const float* o_f32, void* stream);
+
+/* ---- (ABI 11) attention over sequences of different lengths packed back to back (models/wan/attention.py:91-122 flash_attn_varlen_func; the joint attention over
+ * [image ; text] of HunyuanVideo, models/hunyuan_video.py, hands it cu_seqlens), with grouped heads, causal or not
+ * q [tq, hq, D], k / v [tk, hk, D] bf16, hq a multiple of hk (query head h reads key head h / (hq / hk)), token / head strides in elements, head dim contiguous, D in {64, 128}.
+ * cu_q, cu_k: device int32 [n + 1], ascending from 0: sequence b = query tokens cu_q[b] .. cu_q[b + 1] - 1 and key tokens cu_k[b] .. cu_k[b + 1] - 1; either may be empty.
+ * causal: query i sees key j of its sequence when j - len_k <= i - len_q (the last query sees every key).  A query that sees nothing and the rows behind cu_q[n] get o = 0.
+ * o [tq, hq, D] bf16 contiguous; lse [hq, tq] fp32 in log2 units (+inf: nothing seen); o_f32: the output before its rounding (NULL: not kept; the backward needs it).
+ * ws: ..._workspace_floats() fp32, 16-byte aligned, contents irrelevant (0 floats: may be NULL).  Wrong offsets (not ascending, past the end) are clamped to the tensors. */
+long dpipe_attn_varlen_fwd_workspace_floats(long tq, long tk, int n, int hq, int hk, int D);
+int dpipe_attn_varlen_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, float* lse, float* o_f32, float* ws, long ws_floats, long tq,
+                          long tk, int n, int hq, int hk, int D, long q_ss, long q_sh, long k_ss, long k_sh, long v_ss, long v_sh, float scale, int causal, void* stream);
+/* dq [tq, hq, D], dk / dv [tk, hk, D] bf16 contiguous, every row written; delta [hq, tq] fp32 scratch.  No atomics: the same inputs give the same bits. */
+long dpipe_attn_varlen_bwd_workspace_floats(long tq, long tk, int n, int hq, int hk, int D);
+int dpipe_attn_varlen_bwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, const float* o_f32, const void* dout, const float* lse, float* delta,
+                          void* dq, void* dk, void* dv, float* ws, long ws_floats, long tq, long tk, int n, int hq, int hk, int D, long q_ss, long q_sh, long k_ss, long k_sh,
+                          long v_ss, long v_sh, long do_ss, long do_sh, float scale, int causal, void* stream);
+
+/* ---- (ABI 11) rotary positions with several axes on query and key heads in one launch, with their per-head RMS norms (models/wan/model.py:40-67 rope_apply over (frame, height,
+ * width); diffusers FluxPosEmbed + apply_rotary_emb behind models/flux.py; hyvideo get_nd_rotary_pos_embed behind models/hunyuan_video.py:35-81)
+ * q [tokens, heads_q, D], k [tokens, heads_k, D] (heads_k = 0: none), token / head strides in elements, head dim contiguous; yq, yk contiguous.  dtype bf16 or fp32, D % 8 == 0, <= 256.
+ * positions [period, axes], pos_type 0 fp32, 1 int32, 2 int64; token t uses row t % period.  freq, axis: HOST arrays of `pairs` entries, copied into the launch: channel pair p turns
+ * by positions[.][axis[p]] * freq[p] TURNS (one turn = 2 pi).  half = 0: pair p = channels (2 p, 2 p + 1); 1: (p, p + pairs), pairs % 4 == 0.  Channels from 2 * pairs on are not rotated.
+ * wq, wk (NULL: no norm): weight [D] of x * rsqrt(mean(x^2) + eps) * w, applied before the rotation. */
+int dpipe_rope_axes_fwd(const void* q, const void* k, const void* positions, int pos_type, const double* freq, const int* axis, const void* wq, const void* wk, void* yq,
+                        void* yk, long tokens, long period, int axes, int pairs, int heads_q, int heads_k, int D, long q_ss, long q_sh, long k_ss, long k_sh, float eps,
+                        int half, int dtype, int wq_dtype, int wk_dtype, void* stream);
+/* dq, dk contiguous; dwq, dwk (NULL: not wanted) [D] in the weights' dtypes, stored or (accumulate_*) added to what is there; ws: ..._workspace_floats(D) fp32 when a norm is present. */
+long dpipe_rope_axes_workspace_floats(int D);
+int dpipe_rope_axes_bwd(const void* q, const void* k, const void* gq, const void* gk, const void* positions, int pos_type, const double* freq, const int* axis, const void* wq,
+                        const void* wk, void* dq, void* dk, void* dwq, void* dwk, float* ws, long tokens, long period, int axes, int pairs, int heads_q, int heads_k, int D,
+                        long q_ss, long q_sh, long k_ss, long k_sh, long gq_ss, long gq_sh, long gk_ss, long gk_sh, float eps, int half, int dtype, int wq_dtype, int wk_dtype,
+                        int accumulate_wq, int accumulate_wk, void* stream);
 
 #ifdef __cplusplus
 }
