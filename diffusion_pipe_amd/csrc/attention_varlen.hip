@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(NW * 64, (NW == 8 || D == 64) && QB == 1 ? 2 :
         const long tok = orow[qb] / p.hq, hd = orow[qb] - tok * p.hq;
         const float lse = lsum == 0.f ? (SPLIT ? -INFINITY : INFINITY) : m[qb] + __builtin_amdgcn_logf(lsum);      // v_log_f32 = log2
         float* f32 = SPLIT ? p.part + ((long)split * p.tq * p.hq + orow[qb]) * D : p.o32 ? p.o32 + orow[qb] * D : nullptr;
-        if (h == 0) (SPLIT ? p.part_lse + (long)split * p.tq * p.hq : p.lse)[hd * p.tq + tok] = lse;
+        if (h == 0 && (SPLIT || p.lse)) (SPLIT ? p.part_lse + (long)split * p.tq * p.hq : p.lse)[hd * p.tq + tok] = lse;
         if (SPLIT && lsum == 0.f) continue;                    // the join does not read this row
         bf16_t* O = p.o + orow[qb] * D;
 #pragma unroll
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(256) varlen_join_kernel(const VarlenParams p) 
     a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
     *reinterpret_cast<uint2*>(p.o + row * D + d) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
     if (p.o32) *reinterpret_cast<float4*>(p.o32 + row * D + d) = a;
-    if (d == 0) p.lse[at] = sum == 0.f ? INFINITY : base + __builtin_amdgcn_logf(sum);
+    if (d == 0 && p.lse) p.lse[at] = sum == 0.f ? INFINITY : base + __builtin_amdgcn_logf(sum);
 }
 
 // ================================================================================================ backward: dQ (and delta)
@@ -688,7 +688,7 @@ int dpipe_attn_varlen_fwd(const void* q, const void* k, const void* v, const int
     const int rc = fill(p, "dpipe_attn_varlen_fwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal);
     if (rc) return rc;
     const long need = dpipe_attn_varlen_fwd_workspace_floats(tq, tk, n, hq, hk, D);
-    if (!o || !lse || !aligned16(o) || !aligned16(o_f32) || (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) {
+    if (!o || !aligned16(o) || !aligned16(o_f32) || (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) {
         set_last_error("dpipe_attn_varlen_fwd: bad output or workspace"); return DPIPE_ERR_ARG; }
     if (ablated(ABL_ATTN)) return DPIPE_OK;
     p.o = (bf16_t*)o; p.lse = lse; p.o32 = o_f32;

@@ -3,6 +3,7 @@
 Every function here launches gfx950 kernels from libdpipe_hip.so on the current HIP stream; there is no PyTorch /
 CPU fallback (a CPU tensor or a missing library raises `DpipeHipError`).  Reference semantics are cited per op.
 """
+import contextlib
 import ctypes
 import functools
 import math
@@ -1399,26 +1400,61 @@ def rms_norm_rope(x, weight, cos, sin, eps=1e-6, per_head=True, token_offset=0, 
     return _RMSNormRopeFn.apply(x, weight, cos, sin, eps, per_head, token_offset, rope_tokens)
 
 
-# Rotary positions from the positions themselves: several axes, any position per token, query and key heads in one launch
+# Rotary positions from the positions themselves: several axes, any position per token, query and key heads in one launch.
+# (These operators and attention_varlen are also called where a call costs more than its kernels -- a prompt, one image's tokens: their host path passes plain
+#  integers to the C entry, takes the raw stream handle, and enters autograd only when a gradient is wanted.)
 def _head_rows(x):
     """x [..., H, D] as rows the kernels walk by (token stride, head stride): (tensor, tokens, H, D, token stride, head stride).  A view with one uniform token stride (a column block
     of a fused projection) is taken as it is; anything else, or an address that is not 16-byte aligned, is copied once."""
-    H, D = x.shape[-2:]
-    tokens = x.numel() // (H * D) if H * D else 0
-    ok = x.stride(-1) == 1 and x.stride(-2) % 8 == 0 and x.data_ptr() % 16 == 0
-    ss, span = None, 1
-    for size, st in reversed(list(zip(x.shape[:-2], x.stride()[:-2]))):
-        if size == 1:
-            continue
-        if ss is None:
-            ss = st
-        elif st != ss * span:
-            ok = False
-        span *= size
-    ss = H * D if ss is None else ss
+    shape, st = x.shape, x.stride()
+    H, D = shape[-2:]
+    ss = H * D
+    ok = st[-1] == 1 and st[-2] % 8 == 0 and x.data_ptr() % 16 == 0
+    if len(shape) == 3:
+        tokens = shape[0]
+        if tokens > 1:
+            ss = st[0]
+    else:
+        tokens, first = 1, True
+        for size, s in zip(shape[-3::-1], st[-3::-1]):
+            if size != 1:
+                if first:
+                    ss, first = s, False
+                elif s != ss * tokens:
+                    ok = False
+            tokens *= size
     if not ok or ss % 8 or not D <= ss < 2 ** 23:
-        x, ss = x.clone(memory_format=torch.contiguous_format), H * D
-    return x, tokens, H, D, ss, x.stride(-2)
+        x = x.clone(memory_format=torch.contiguous_format)
+        return x, tokens, H, D, H * D, D
+    return x, tokens, H, D, ss, st[-2]
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _one_device(*tensors):
+    """the operands' device; DpipeHipError for a CPU tensor or operands on different devices"""
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise DpipeHipError(f'operands on different devices: {device} and {t.device}')
+    require_cuda(tensors[0])
+    return device
+
+
+@contextlib.contextmanager
+def _launching_on(device):
+    """kernels are launched on the current device: make it the operands'"""
+    with torch.cuda.device(device):
+        yield
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    return _HERE if device.index == torch.cuda.current_device() else _launching_on(device)
 
 
 @functools.lru_cache(maxsize=64)
@@ -1436,45 +1472,58 @@ def _rope_axes_tables(axes_dim, theta, shared):
 _POSITION_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 
 
+def _rope_axes_forward(q, k, positions, q_weight, k_weight, tables, eps, half):
+    """-> (yq, yk, (q, k as read), what the backward's call repeats)"""
+    device = q.device
+    q, tokens, hq, D, q_ss, q_sh = _head_rows(q)
+    yq = torch.empty(q.shape, device=device, dtype=q.dtype)
+    hk = k_ss = k_sh = 0
+    yk = None
+    if k is not None:
+        k, _, hk, _, k_ss, k_sh = _head_rows(k)
+        yk = torch.empty(k.shape, device=device, dtype=k.dtype)
+    freq, axis, pairs = tables
+    axes = positions.shape[-1]
+    meta = (tokens, positions.numel() // axes, axes, pairs, hq, hk, D)
+    dt = dtype_code(q.dtype)
+    tail = (eps, half, dt, dt if q_weight is None else dtype_code(q_weight.dtype), dt if k_weight is None else dtype_code(k_weight.dtype))
+    strides = (q_ss, q_sh, k_ss, k_sh)
+    if tokens:
+        wq, wk = _al(q_weight), _al(k_weight)
+        check(lib().dpipe_rope_axes_fwd(q.data_ptr(), _addr(k), positions.data_ptr(), _POSITION_TYPES[positions.dtype], freq, axis, _addr(wq), _addr(wk), yq.data_ptr(), _addr(yk),
+                                        *meta, *strides, *tail, hip.raw_stream(device)), 'rope_axes_fwd')
+    return yq, yk, q, k, (meta, strides, tail, tables)
+
+
 class _RopeAxesFn(Function):
     """q', k' = R(positions) [rms_norm](q, k); see rope_axes.  The backward re-derives the norm's statistics from q / k: nothing but the inputs is kept."""
 
     @staticmethod
     def forward(ctx, q, k, positions, q_weight, k_weight, tables, eps, half):
-        q, tokens, hq, D, q_ss, q_sh = _head_rows(q)
-        yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        hk = k_ss = k_sh = 0
-        yk = None
-        if k is not None:
-            k, _, hk, _, k_ss, k_sh = _head_rows(k)
-            yk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-        freq, axis, pairs = tables
-        period, axes = positions.numel() // positions.shape[-1], positions.shape[-1]
-        meta = (tokens, period, axes, pairs, hq, hk, D)
-        wd = [dtype_code(w.dtype) if w is not None else dtype_code(q.dtype) for w in (q_weight, k_weight)]
-        wq, wk = _al(q_weight), _al(k_weight)
-        if tokens:
-            check(lib().dpipe_rope_axes_fwd(ptr(q), ptr(k), ptr(positions), _POSITION_TYPES[positions.dtype], freq, axis, ptr(wq), ptr(wk), ptr(yq), ptr(yk), *meta,
-                                            q_ss, q_sh, k_ss, k_sh, float(eps), int(half), dtype_code(q.dtype), *wd, stream()), 'rope_axes_fwd')
-        ctx.save_for_backward(q if wq is not None or wk is not None else None, k if wq is not None or wk is not None else None, positions, q_weight, k_weight)
-        ctx.meta = (meta, tables, (q_ss, q_sh, k_ss, k_sh), wd, eps, half, q.shape, k.shape if k is not None else None, q.dtype)
+        ctx.shapes = (q.shape, None if k is None else k.shape, q.dtype)
+        yq, yk, q, k, ctx.call = _rope_axes_forward(q, k, positions, q_weight, k_weight, tables, eps, half)
+        normed = q_weight is not None or k_weight is not None
+        ctx.save_for_backward(q if normed else None, k if normed else None, positions, q_weight, k_weight)
         return yq, yk
 
     @staticmethod
     def backward(ctx, gq, gk):
         q, k, positions, q_weight, k_weight = ctx.saved_tensors
-        meta, (freq, axis, _), strides, wd, eps, half, q_shape, k_shape, dtype = ctx.meta
-        tokens, D = meta[0], meta[-1]
-        with torch.cuda.device(gq.device):
+        meta, strides, tail, (freq, axis, _) = ctx.call
+        q_shape, k_shape, dtype = ctx.shapes
+        tokens, D, device = meta[0], meta[-1], gq.device
+        with _on(device):
             gq, _, _, _, gq_ss, gq_sh = _head_rows(gq)
-            dq = torch.empty(q_shape, device=gq.device, dtype=dtype)
+            dq = torch.empty(q_shape, device=device, dtype=dtype)
             dk, gk_ss, gk_sh = None, 0, 0
             if k_shape is not None:
                 gk, _, _, _, gk_ss, gk_sh = _head_rows(gk)
-                dk = torch.empty(k_shape, device=gq.device, dtype=dtype)
-            normed = q_weight is not None or k_weight is not None
+                dk = torch.empty(k_shape, device=device, dtype=dtype)
+            else:
+                gk = None
+            normed = q is not None
             if not normed:
-                q, k, strides = gq, (gk if k_shape is not None else None), (gq_ss, gq_sh, gk_ss, gk_sh)
+                q, k, strides = gq, gk, (gq_ss, gq_sh, gk_ss, gk_sh)
             dw, fused = [None, None], [False, False]
             for i, w in enumerate((q_weight, k_weight)):
                 if w is not None and ctx.needs_input_grad[3 + i]:
@@ -1483,11 +1532,11 @@ class _RopeAxesFn(Function):
                     if dw[i] is None:
                         dw[i] = torch.empty_like(w) if tokens else torch.zeros_like(w)
             if tokens:
-                ws = torch.empty(lib().dpipe_rope_axes_workspace_floats(D), device=gq.device, dtype=torch.float32) if normed else None
-                check(lib().dpipe_rope_axes_bwd(ptr(q), ptr(k), ptr(gq), ptr(gk) if k_shape is not None else None, ptr(positions), _POSITION_TYPES[positions.dtype], freq, axis,
-                                                ptr(_al(q_weight)), ptr(_al(k_weight)), ptr(dq), ptr(dk), ptr(dw[0]), ptr(dw[1]), ptr(ws), *meta, *strides,
-                                                gq_ss, gq_sh, gk_ss, gk_sh, float(eps), int(half), dtype_code(dtype), *wd,
-                                                _acc_all(fused[0], dw[0]), _acc_all(fused[1], dw[1]), stream()), 'rope_axes_bwd')
+                ws = torch.empty(lib().dpipe_rope_axes_workspace_floats(D), device=device, dtype=torch.float32) if normed else None
+                wq, wk = _al(q_weight), _al(k_weight)
+                check(lib().dpipe_rope_axes_bwd(q.data_ptr(), _addr(k), gq.data_ptr(), _addr(gk), positions.data_ptr(), _POSITION_TYPES[positions.dtype], freq, axis, _addr(wq), _addr(wk),
+                                                dq.data_ptr(), _addr(dk), _addr(dw[0]), _addr(dw[1]), _addr(ws), *meta, *strides, gq_ss, gq_sh, gk_ss, gk_sh, *tail,
+                                                _acc_all(fused[0], dw[0]), _acc_all(fused[1], dw[1]), hip.raw_stream(device)), 'rope_axes_bwd')
         return dq, dk, None, (None if fused[0] else dw[0]), (None if fused[1] else dw[1]), None, None, None
 
 
@@ -1523,16 +1572,11 @@ def rope_axes(q, k, positions, axes_dim, theta=10000.0, q_weight=None, k_weight=
             raise DpipeHipError(f'rope_axes: norm weights have shape [{D}]; got {tuple(w.shape)}')
     if k is None and k_weight is not None:
         raise DpipeHipError('rope_axes: a key weight needs k')
-    require_cuda(q, k, positions, q_weight, k_weight)
-    _same_device(q, k, positions, q_weight, k_weight)
-    with torch.cuda.device(q.device):
-        return _RopeAxesFn.apply(q, k, _contig(positions), q_weight, k_weight, _rope_axes_tables(axes_dim, theta, bool(shared)), eps, not interleaved)
-
-
-def _same_device(*tensors):
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise DpipeHipError(f'operands on different devices: {sorted(map(str, devices))}')
+    args = (q, k, _contig(positions), q_weight, k_weight, _rope_axes_tables(axes_dim, theta, bool(shared)), float(eps), int(not interleaved))
+    with _on(_one_device(q, k, positions, q_weight, k_weight)):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+            return _RopeAxesFn.apply(*args)
+        return _rope_axes_forward(*args)[:2]
 
 
 # -------------------------------------------------------------------------------------------- attention (K4)
@@ -1726,48 +1770,50 @@ def attention(q, k, v, kv_len=None, scale=None, impl='auto', causal=False):
     return _UnfusedAttnFn.apply(q, k, v, scale, causal, kv_len)
 
 
+def _varlen_forward(q, k, v, cu_q, cu_k, scale, causal, keep):
+    """-> (o, what the backward reads, what its call repeats); keep: the unrounded output and the row statistics are stored for the backward's delta and P"""
+    device = q.device
+    (q, tq, hq, D, *qs), (k, tk, hk, _, *ks), (v, _, _, _, *vs) = _head_rows(q), _head_rows(k), _head_rows(v)
+    if tq == 0 or tk == 0:                        # nothing to read: every row is empty
+        return torch.zeros(q.shape, device=device, dtype=q.dtype), (), None
+    sizes, strides = (tq, tk, cu_q.shape[0] - 1, hq, hk, D), (*qs, *ks, *vs)
+    o = torch.empty((tq, hq, D), device=device, dtype=q.dtype)
+    lse = torch.empty((hq, tq), device=device, dtype=torch.float32) if keep else None
+    o32 = torch.empty((tq, hq, D), device=device, dtype=torch.float32) if keep else None
+    need = lib().dpipe_attn_varlen_fwd_workspace_floats(*sizes)
+    ws = torch.empty(need, device=device, dtype=torch.float32) if need else None
+    check(lib().dpipe_attn_varlen_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _addr(lse), _addr(o32), _addr(ws), need, *sizes,
+                                      *strides, scale, causal, hip.raw_stream(device)), 'attn_varlen_fwd')
+    return o, (q, k, v, cu_q, cu_k, o32, lse), (sizes, strides, scale, causal)
+
+
 class _AttnVarlenFn(Function):
     """see attention_varlen; keeps the unrounded output for the backward's delta, as _FlashAttnFn does"""
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale, causal):
-        (q, tq, hq, D, *qs), (k, tk, hk, _, *ks), (v, _, _, _, *vs) = _head_rows(q), _head_rows(k), _head_rows(v)
-        n = cu_q.numel() - 1
-        if tq == 0 or tk == 0:                    # nothing to read: every row is empty
-            ctx.meta = None
-            ctx.shapes = (q.shape, k.shape, v.shape, q.dtype)
-            return torch.zeros(q.shape, device=q.device, dtype=q.dtype)
-        sizes = (tq, tk, n, hq, hk, D)
-        keep = any(ctx.needs_input_grad[:3])
-        o = torch.empty((tq, hq, D), device=q.device, dtype=q.dtype)
-        lse = torch.empty((hq, tq), device=q.device, dtype=torch.float32)
-        o32 = torch.empty((tq, hq, D), device=q.device, dtype=torch.float32) if keep else None
-        need = lib().dpipe_attn_varlen_fwd_workspace_floats(*sizes)
-        ws = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
-        check(lib().dpipe_attn_varlen_fwd(ptr(q), ptr(k), ptr(v), ptr(cu_q), ptr(cu_k), ptr(o), ptr(lse), ptr(o32), ptr(ws), need, *sizes, *qs, *ks, *vs,
-                                          float(scale), int(causal), stream()), 'attn_varlen_fwd')
-        if keep:
-            ctx.save_for_backward(q, k, v, cu_q, cu_k, o32, lse)
-        ctx.meta = (sizes, (*qs, *ks, *vs), scale, causal)
+        ctx.shapes = (q.shape, k.shape, v.shape, q.dtype)
+        o, saved, ctx.call = _varlen_forward(q, k, v, cu_q, cu_k, scale, causal, True)
+        ctx.save_for_backward(*saved)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        if ctx.meta is None:
+        device = do.device
+        if ctx.call is None:
             *shapes, dtype = ctx.shapes
-            return (*(torch.zeros(sh, device=do.device, dtype=dtype) for sh in shapes), None, None, None, None)
+            return (*(torch.zeros(sh, device=device, dtype=dtype) for sh in shapes), None, None, None, None)
         q, k, v, cu_q, cu_k, o32, lse = ctx.saved_tensors
-        sizes, strides, scale, causal = ctx.meta
-        tq, tk, _, hq, hk, D = sizes
-        with torch.cuda.device(q.device):
+        sizes, strides, scale, causal = ctx.call
+        with _on(device):
             do, _, _, _, *ds = _head_rows(do)
-            dq = torch.empty((tq, hq, D), device=q.device, dtype=q.dtype)
-            dk, dv = (torch.empty((tk, hk, D), device=q.device, dtype=q.dtype) for _ in range(2))
-            delta = torch.empty((hq, tq), device=q.device, dtype=torch.float32)
+            dq, dk, dv = (torch.empty(sh, device=device, dtype=q.dtype) for sh in ctx.shapes[:3])
+            delta = torch.empty_like(lse)
             need = lib().dpipe_attn_varlen_bwd_workspace_floats(*sizes)
-            ws = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
-            check(lib().dpipe_attn_varlen_bwd(ptr(q), ptr(k), ptr(v), ptr(cu_q), ptr(cu_k), ptr(o32), ptr(do), ptr(lse), ptr(delta), ptr(dq), ptr(dk), ptr(dv), ptr(ws), need,
-                                              *sizes, *strides, *ds, float(scale), int(causal), stream()), 'attn_varlen_bwd')
+            ws = torch.empty(need, device=device, dtype=torch.float32) if need else None
+            check(lib().dpipe_attn_varlen_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o32.data_ptr(), do.data_ptr(), lse.data_ptr(),
+                                              delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _addr(ws), need, *sizes, *strides, *ds, scale, causal,
+                                              hip.raw_stream(device)), 'attn_varlen_bwd')
         return dq, dk, dv, None, None, None, None
 
 
@@ -1782,22 +1828,25 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=False):
     finite: a masked infinity or NaN reaches its sequence's other rows).  The same inputs give the same bits (no atomics).  (models/wan/attention.py:91-122)
     -> [Tq, H, D]"""
     cu_k = cu_q if cu_k is None else cu_k
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2] or k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
-        raise DpipeHipError(f'attention_varlen: q [Tq, H, D], k and v [Tk, Hk, D] with H a multiple of Hk; got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
-    if not flash_eligible(q.dtype, q.shape[2]) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise DpipeHipError(f'attention_varlen computes in bf16 at head dim 64 or 128; got {q.dtype}, {k.dtype}, {v.dtype}, head dim {q.shape[2]}')
+    qs, ks, dtype = q.shape, k.shape, q.dtype
+    if len(qs) != 3 or len(ks) != 3 or ks != v.shape or ks[2] != qs[2] or ks[1] == 0 or qs[1] == 0 or qs[1] % ks[1]:
+        raise DpipeHipError(f'attention_varlen: q [Tq, H, D], k and v [Tk, Hk, D] with H a multiple of Hk; got {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}')
+    if not flash_eligible(dtype, qs[2]) or k.dtype != dtype or v.dtype != dtype:
+        raise DpipeHipError(f'attention_varlen computes in bf16 at head dim 64 or 128; got {dtype}, {k.dtype}, {v.dtype}, head dim {qs[2]}')
     for cu in (cu_q, cu_k):
-        if cu.dtype not in (torch.int32, torch.int64) or cu.dim() != 1 or cu.numel() < 2 or cu.numel() != cu_q.numel():
+        if cu.dtype not in (torch.int32, torch.int64) or cu.dim() != 1 or cu.shape[0] < 2 or cu.shape[0] != cu_q.shape[0]:
             raise DpipeHipError(f'attention_varlen: offsets are int32 [N + 1], N >= 1, for queries and keys alike; got {cu.dtype} {tuple(cu.shape)}, {tuple(cu_q.shape)}')
-    if cu_k is cu_q and k.shape[0] != q.shape[0]:
-        raise DpipeHipError(f'attention_varlen: shared offsets need as many keys as queries; got {q.shape[0]} and {k.shape[0]}')
-    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    if cu_k is cu_q and ks[0] != qs[0]:
+        raise DpipeHipError(f'attention_varlen: shared offsets need as many keys as queries; got {qs[0]} and {ks[0]}')
+    scale = 1.0 / math.sqrt(qs[2]) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise DpipeHipError(f'attention_varlen: scale must be positive and finite, got {scale}')
-    require_cuda(q, k, v, cu_q, cu_k)
-    _same_device(q, k, v, cu_q, cu_k)
-    with torch.cuda.device(q.device):
-        return _AttnVarlenFn.apply(q, k, v, _contig(cu_q.to(torch.int32)), _contig(cu_k.to(torch.int32)), scale, bool(causal))
+    device = _one_device(q, k, v, cu_q, cu_k)
+    cu_q, cu_k = (cu if cu.dtype == torch.int32 and cu.is_contiguous() else cu.to(torch.int32).contiguous() for cu in (cu_q, cu_k))
+    with _on(device):
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return _AttnVarlenFn.apply(q, k, v, cu_q, cu_k, scale, int(causal))
+        return _varlen_forward(q, k, v, cu_q, cu_k, scale, int(causal), False)[0]
 
 
 # ------------------------------------------------------------------------------------------------- loss (K9)

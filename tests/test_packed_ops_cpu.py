@@ -117,7 +117,7 @@ def _varlen_c(name='fwd', **kw):
 
 
 @pytest.mark.parametrize('name', ['fwd', 'bwd'])
-@pytest.mark.parametrize('kw', [{'q': None}, {'cu_k': None}, {'lse': None}, {'tq': 0}, {'tk': -1}, {'n': 0}, {'hq': 3, 'hk': 2}, {'D': 96}, {'D': 256}, {'scale': 0.0}, {'scale': math.nan},
+@pytest.mark.parametrize('kw', [{'q': None}, {'cu_k': None}, {'tq': 0}, {'tk': -1}, {'n': 0}, {'hq': 3, 'hk': 2}, {'D': 96}, {'D': 256}, {'scale': 0.0}, {'scale': math.nan},
                                 {'scale': math.inf}, {'q': 264}, {'q_ss': 132}, {'k_ss': 32}, {'v_ss': 2 ** 23}, {'k_sh': -64}, {'tq': 2 ** 31}, {'n': 2 ** 23}, {'tk': 2 ** 18}])
 def test_attention_varlen_c_entries_refuse(name, kw):
     """(the last: few rows and long keys -- or few keys' gradients -- need the workspace, which is missing)"""
