@@ -13,7 +13,7 @@
 // Few rows against long keys: the key range of every sequence is cut into `nsplit` parts (own workgroups, fp32 partial rows) that a second kernel joins.
 //
 // As in attention.hip everything is v_mfma_f32_32x32x16_bf16 on the transposed score tile S^T = K . Q^T (a lane owns one query column: softmax statistics are
-// lane-local), tiles stream global -> LDS by buffer_load ... lds into a two-deep ring of lds_dma_tiles.h images; rows past a sequence's end come back as zeros from the
+// lane-local), tiles stream global -> LDS by buffer_load ... lds into a two-deep ring; rows past a sequence's end come back as zeros from the
 // buffer bounds check, whatever the neighbouring sequence holds.  Each tile has a buffer descriptor of its own, so a sequence may span more than 4 GiB.
 #include <cstdio>
 #include "dpipe_common.h"
@@ -33,11 +33,12 @@ struct VarlenParams {
     const int *cu_q, *cu_k;
     float *part, *part_lse;              // split forms: forward rows [split][Tq][Hq][D] and their lse [split][Hq][Tq]; dK / dV [split][2][Tk][Hk][D]
     long tq, tk;
-    int n, hq, hk, g, slots, nsplit, causal;
+    int n, hq, hk, g, nsplit, causal;
     long q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, do_ss, do_sh;    // o, dq, dk, dv are contiguous
     float scale;
 };
 
+constexpr int NT = 256, ROWS = 128;       // threads, query rows (dK / dV: keys) of a workgroup: 4 waves of 32
 constexpr int KT = 64;                   // keys (dK / dV: queries) per LDS tile
 constexpr float M_INIT = -3.0e38f;       // running maximum before the first key: finite, so that exp2(-inf - m) is 0 and never NaN
 constexpr float RESCALE_AT = 8.f;        // the accumulator is rescaled when the maximum grew by more than 2^8: P stays below 256, its relative rounding is the same
@@ -85,10 +86,39 @@ __device__ __forceinline__ Tile find_tile(const VarlenParams& p, int slot, bool 
     return t;
 }
 
-// consecutive workgroup ids go round the 8 XCDs: each XCD gets a contiguous run of (head, slot), so tiles that stream the same K / V share an L2
-__device__ __forceinline__ int xcd_order(int id, int total) {
-    const int per = total / 8, rest = total % 8, x = id % 8;
-    return (x < rest ? x * (per + 1) : rest * (per + 1) + (x - rest) * per) + id / 8;
+// The lane's query row: token (in the buffer) and query head; `last`: the last key of its sequence it sees (-1: none)
+struct Row { long token, head; int last; bool live; };
+__device__ __forceinline__ Row find_row(const VarlenParams& p, const Tile& t, int kh, int wid, int i) {
+    const long at = t.row0 + 32 * wid + i;
+    Row r;
+    r.live = at < t.rows;
+    const unsigned row = r.live ? (unsigned)at : 0u, tok = row / (unsigned)p.g;
+    r.token = t.q0 + tok; r.head = (long)kh * p.g + (row - tok * p.g);
+    r.last = p.causal ? (int)min((long)tok + t.lk - t.lq, (long)t.lk - 1) : t.lk - 1;
+    return r;
+}
+// How many keys (from the first on) some row of the workgroup sees, some row of the wave, every live row of the wave
+struct Seen { int group, wave, all; };
+__device__ __forceinline__ Seen keys_seen(const VarlenParams& p, const Tile& t, int wid) {
+    const long r0 = t.row0 + 32 * wid, last = min(t.row0 + ROWS, t.rows) - 1, wlast = min(r0 + 32, t.rows) - 1;
+    if (!p.causal) return {t.lk, wlast < r0 ? 0 : t.lk, t.lk};
+    auto upto = [&](long row) { return (int)max(0l, min((long)t.lk, row / p.g + t.lk - t.lq + 1)); };
+    return {upto(last), wlast < r0 ? 0 : upto(wlast), wlast < r0 ? 0 : upto(r0)};
+}
+
+// Workgroup id -> (key head, slot, part).  Consecutive ids go round the 8 XCDs, each with an L2 of its own: an XCD gets whole key heads, or every c-th slot of one when the heads
+// are not a multiple of 8 -- the tiles that stream one head's rows share an L2, and long and short sequences (causal: early and late tiles) are spread evenly over the XCDs.
+struct Work { int head, slot, part; };
+__host__ __device__ __forceinline__ int xcd_classes(int heads) { return heads % 8 == 0 ? 1 : heads % 4 == 0 ? 2 : heads % 2 == 0 ? 4 : 8; }
+__host__ __device__ __forceinline__ long work_groups(long slots, int heads, int parts) { const int c = xcd_classes(heads); return (slots + c - 1) / c * c * heads * parts; }
+__device__ __forceinline__ Work find_work(int id, int heads, int parts) {
+    const int c = xcd_classes(heads), units = heads * c / 8;  // (head, slot class) pairs per XCD
+    int j = id / 8;
+    Work w;
+    w.part = j % parts; j /= parts;
+    const int unit = id % 8 * units + j % units;
+    w.head = unit / c; w.slot = j / units * c + unit % c;
+    return w;
 }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, long bytes) {
@@ -103,14 +133,20 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const bf16_t* base, 
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, char* dst, unsigned off) { __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)dst, 16, off, 0, 0, 0); }
 __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, char* dst, unsigned off) { __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)dst, 4, off, 0, 0, 0); }
 
-template <int D, int NW> struct Offsets {                     // per-lane source offsets of this wave's DMA pieces of one tile
+// LDS image of a 64-row tile, read both by rows and transposed: slices of 64 columns, [64 rows][128 B] each, 16-byte chunk c of row r at chunk c ^ f(r) with
+// f(r) = (r1 r3 r2) in bits of r.  Rows 0 .. 15 of one chunk (ds_read_b128) then cover the 256 B of all banks once, and so do the 4 rows x 64 B of one transposed read's half wave
+// (rows r .. r + 3 differ in r0 -- the 128-byte half -- and r1 -- the 64-byte granule).  One image where a tile is needed both ways (K in dQ; Q and dO in dK / dV) halves its DMA
+// traffic and its LDS.
+__device__ __forceinline__ int swizzle(int r) { return ((r >> 1) & 1) << 2 | ((r >> 2) & 3); }
+
+template <int D, int NW> struct Offsets {                     // per-lane source offsets of this wave's 1 KiB DMA pieces (8 rows of a slice) of one tile
     static constexpr int PP = KT * D * 2 / 1024 / NW;
     unsigned o[PP];
-    template <bool MN> __device__ __forceinline__ void init(int wid, int lane, long ss) {
+    __device__ __forceinline__ void init(int wid, int lane, long ss) {
 #pragma unroll
         for (int j = 0; j < PP; ++j) {
-            const int P = j * NW + wid;
-            o[j] = MN ? dma_voffset<true, D>(P, lane, 0, ss) : dma_voffset<false, KT>(P % 8, lane, 0, ss) + (unsigned)(P / 8) * 128u;
+            const int P = j * NW + wid, row = 8 * (P % 8) + (lane >> 3);
+            o[j] = (unsigned)(row * ss * 2) + (unsigned)(P / 8) * 128u + (unsigned)(((lane & 7) ^ swizzle(row)) << 4);
         }
     }
     __device__ __forceinline__ void issue(__amdgpu_buffer_rsrc_t rs, char* img, int wid) const {
@@ -118,6 +154,25 @@ template <int D, int NW> struct Offsets {                     // per-lane source
         for (int j = 0; j < PP; ++j) dma16(rs, img + (j * NW + wid) * 1024, o[j]);
     }
 };
+
+// MFMA operand with k along the row: lane (i, h) gets columns 16 ks + 8 h .. + 8 of row `row + i` (row a multiple of 32)
+__device__ __forceinline__ bf16x8_t by_rows(const char* img, int row, int ks, int lane) {
+    const int i = lane & 31;
+    return *reinterpret_cast<const bf16x8_t*>(img + (ks / 4) * (KT * 128) + row * 128 + i * 128 + ((((lane >> 5) ^ swizzle(i)) ^ (2 * (ks & 3))) << 4));
+}
+// MFMA operand of the transposed tile: m = column `col + i` (col a multiple of 32), k = the rows of the 16-row block r0 in the order a lane holds them in a score accumulator
+// ({4 h + 0 .. 3, 8 + 4 h + 0 .. 3}), so P / dS go from their accumulators straight into the product
+__device__ __forceinline__ bf16x8_t by_cols(const char* img, int col, int r0, int lane) {
+    const int t = lane & 15, g = lane >> 4, r = 4 * (g >> 1) + (t >> 2);
+    const char* p = img + (col / 64) * (KT * 128) + r0 * 128 + r * 128 + (t & 1) * 8;
+    const int c = (((col / 32) & 1) << 2 | (g & 1) << 1 | ((t & 3) >> 1)) ^ swizzle(r);
+    const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4_t*)(p + (c << 4)));
+    const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4_t*)(p + 8 * 128 + ((c ^ 2) << 4)));
+    bf16x8_t out;
+    out[0] = lo[0]; out[1] = lo[1]; out[2] = lo[2]; out[3] = lo[3];
+    out[4] = hi[0]; out[5] = hi[1]; out[6] = hi[2]; out[7] = hi[3];
+    return out;
+}
 
 __device__ __forceinline__ float max_halves(float x) {        // max over lane and lane ^ 32, in both
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -129,460 +184,344 @@ __device__ __forceinline__ float sum_halves(float x) {
 }
 
 // ================================================================================================ forward
-template <int D, int QB, int NW, bool SPLIT>
-__global__ void __launch_bounds__(NW * 64, (NW == 8 || D == 64) && QB == 1 ? 2 : 1) varlen_fwd_kernel(const VarlenParams p) {
-    constexpr int QW = 32 * QB, QWG = QW * NW, NKS = D / 16, NDB = D / 32, IMG = KT * D * 2, STAGE = 2 * IMG;
+// 128 rows per workgroup of 4 waves, two workgroups per CU: one's softmax runs under the other's products without a barrier between them.
+template <int D, bool SPLIT>
+__global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const VarlenParams p) {
+    constexpr int NKS = D / 16, NDB = D / 32, IMG = KT * D * 2, STAGE = 2 * IMG;
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-    int L = xcd_order(blockIdx.x, gridDim.x);
-    const int split = SPLIT ? L % p.nsplit : 0;
-    if (SPLIT) L /= p.nsplit;
-    const int kh = L / p.slots;
-    const Tile t = find_tile<QWG>(p, L % p.slots, false, p.causal);
+    const Work w = find_work(blockIdx.x, p.hk, SPLIT ? p.nsplit : 1);
+    const Tile t = find_tile<ROWS>(p, w.slot, false, p.causal);
     if (!t.live) return;
 
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
-    const long r0 = t.row0 + wid * QW;                         // first row of this wave
-    const int seen = t.lk - t.lq;                              // causal: token x sees keys 0 .. x + seen
-    const bf16_t* K = p.k + t.k0 * p.k_ss + kh * p.k_sh;
-    const bf16_t* V = p.v + t.k0 * p.v_ss + kh * p.v_sh;
+    const Row r = find_row(p, t, w.head, wid, i);
+    const Seen seen = keys_seen(p, t, wid);
+    const bf16_t* K = p.k + t.k0 * p.k_ss + w.head * p.k_sh;
+    const bf16_t* V = p.v + t.k0 * p.v_ss + w.head * p.v_sh;
+    const bf16_t* Q = p.q + r.token * p.q_ss + r.head * p.q_sh;
     const float sl2 = p.scale * LOG2E;
 
-    bf16x8_t qf[QB][NKS];
-    long orow[QB];                                             // (token * Hq + head) of the lane's rows, -1: none
-    int lim[QB];                                               // last key the row sees
+    bf16x8_t qf[NKS];
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-        const long r = r0 + 32 * qb + i;
-        const bool live = r < t.rows;
-        const unsigned tok = live ? (unsigned)r / (unsigned)p.g : 0u, hd = live ? (unsigned)r - tok * (unsigned)p.g : 0u;
-        orow[qb] = live ? (t.q0 + tok) * p.hq + kh * p.g + hd : -1;
-        lim[qb] = p.causal ? (int)min((long)tok + seen, (long)t.lk - 1) : t.lk - 1;
-        const bf16_t* Q = p.q + (t.q0 + tok) * p.q_ss + (long)(kh * p.g + hd) * p.q_sh;
+    for (int ks = 0; ks < NKS; ++ks) qf[ks] = r.live ? *reinterpret_cast<const bf16x8_t*>(Q + 16 * ks + 8 * h) : zero_frag();
+    f32x16 oacc[NDB];
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) qf[qb][ks] = live ? *reinterpret_cast<const bf16x8_t*>(Q + 16 * ks + 8 * h) : zero_frag();
-    }
-    f32x16 oacc[QB][NDB];
-    float m[QB], l[QB];                                        // m: running maximum in log2 units; l: this lane's part of the sum
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) oacc[qb][db] = zero16();
-        m[qb] = M_INIT; l[qb] = 0.f;
-    }
+    for (int db = 0; db < NDB; ++db) oacc[db] = zero16();
+    float m = M_INIT, l = 0.f;                                 // running maximum in log2 units; this lane's part of the sum
 
-    // keys that any row of the workgroup / every row of the wave sees (wave-uniform)
-    const long last = min(t.row0 + QWG, t.rows) - 1, wlast = min(r0 + QW, t.rows) - 1;
-    const int wg_keys = p.causal ? (int)max(0l, min((long)t.lk, last / p.g + seen + 1)) : t.lk;
-    const int w_keys = wlast < r0 ? 0 : p.causal ? (int)max(0l, min((long)t.lk, wlast / p.g + seen + 1)) : t.lk;
-    const int w_full = wlast < r0 ? 0 : p.causal ? (int)max(0l, min((long)t.lk, r0 / p.g + seen + 1)) : t.lk;
-    const int nkt = (wg_keys + KT - 1) / KT;
-    int kt0 = 0, kt1 = nkt;
+    int kt0 = 0, kt1 = (seen.group + KT - 1) / KT;
     if (SPLIT) {                                               // every part of the sequence's key tiles, cut by its full length
         const int all = (t.lk + KT - 1) / KT, per = (all + p.nsplit - 1) / p.nsplit;
-        kt0 = min(nkt, split * per); kt1 = min(nkt, kt0 + per);
+        kt0 = min(kt1, w.part * per); kt1 = min(kt1, kt0 + per);
     }
-    Offsets<D, NW> oK, oV;
-    oK.template init<false>(wid, lane, p.k_ss); oV.template init<true>(wid, lane, p.v_ss);
-    auto issue = [&](int kt, int buf) {
-        char* base = lds + buf * STAGE;
+    Offsets<D, 4> oK, oV;
+    oK.init(wid, lane, p.k_ss); oV.init(wid, lane, p.v_ss);
+    auto issue = [&](int kt) {
+        char* base = lds + (kt & 1) * STAGE;
         oK.issue(rows_rsrc<D>(K, p.k_ss, kt * KT, t.lk), base, wid);
         oV.issue(rows_rsrc<D>(V, p.v_ss, kt * KT, t.lk), base + IMG, wid);
     };
-    if (kt0 < kt1) issue(kt0, kt0 & 1);
+    if (kt0 < kt1) issue(kt0);
     for (int kt = kt0; kt < kt1; ++kt) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's pieces of tile kt
         __builtin_amdgcn_s_barrier();                          // everyone's pieces landed; everyone is done with the other buffer
-        if (kt + 1 < kt1) issue(kt + 1, (kt + 1) & 1);
+        if (kt + 1 < kt1) issue(kt + 1);
         const char* Kl = lds + (kt & 1) * STAGE;
         const char* Vl = Kl + IMG;
         const int key0 = kt * KT;
-        if (key0 >= w_keys) continue;                          // wave-uniform: no row of this wave sees the tile
-        f32x16 s[QB][2];
+        if (key0 >= seen.wave) continue;                       // wave-uniform: no row of this wave sees the tile
+        f32x16 s[2] = {zero16(), zero16()};
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) { s[qb][0] = zero16(); s[qb][1] = zero16(); }
+        for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) {
-            const bf16x8_t k0f = read_frag<false, KT>(Kl + (ks / 4) * (KT * 128), 0, ks & 3, lane), k1f = read_frag<false, KT>(Kl + (ks / 4) * (KT * 128), 32, ks & 3, lane);
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) { s[qb][0] = mfma16(k0f, qf[qb][ks], s[qb][0]); s[qb][1] = mfma16(k1f, qf[qb][ks], s[qb][1]); }
-        }
-        bf16x8_t pf[QB][4];
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-            if (key0 + KT > w_full) {                          // some row of the wave does not see the whole tile
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int key = key0 + 32 * kb + (e & 3) + 8 * (e >> 2) + 4 * h;
-                        s[qb][kb][e] = key <= lim[qb] ? s[qb][kb][e] : -INFINITY;
-                    }
-            }
-            float mx = s[qb][0][0];
+            for (int kb = 0; kb < 2; ++kb) s[kb] = mfma16(by_rows(Kl, 32 * kb, ks, lane), qf[ks], s[kb]);
+        if (key0 + KT > seen.all) {                            // some row of the wave does not see the whole tile
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[qb][kb][e]);
-            mx = max_halves(mx) * sl2;
-            if (!__all(mx <= m[qb] + RESCALE_AT)) {
-                const float m_new = fmaxf(m[qb], mx), alpha = __builtin_amdgcn_exp2f(m[qb] - m_new);
-                l[qb] *= alpha; m[qb] = m_new;
-#pragma unroll
-                for (int db = 0; db < NDB; ++db)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) oacc[qb][db][e] *= alpha;
-            }
-            const float mm = m[qb];
-            float rs = 0.f;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) { const float pe = __builtin_amdgcn_exp2f(s[qb][kb][e] * sl2 - mm); s[qb][kb][e] = pe; rs += pe; }
-            l[qb] += rs;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) pf[qb][u] = pack_frag(s[qb][u >> 1], 8 * (u & 1));
+                for (int e = 0; e < 16; ++e) s[kb][e] = key0 + 32 * kb + (e & 3) + 8 * (e >> 2) + 4 * h <= r.last ? s[kb][e] : -INFINITY;
         }
+        float mx = s[0][0];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)                            // O^T += V^T . P^T
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int db = 0; db < NDB; ++db) {
-                const bf16x8_t vf = read_frag_tr_acc<D>(Vl, 32 * db, 16 * u, lane);
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
+        mx = max_halves(mx) * sl2;
+        if (!__all(mx <= m + RESCALE_AT)) {
+            const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
+            l *= alpha; m = m_new;
 #pragma unroll
-                for (int qb = 0; qb < QB; ++qb) oacc[qb][db] = mfma16(vf, pf[qb][u], oacc[qb][db]);
-            }
+            for (int db = 0; db < NDB; ++db)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) oacc[db][e] *= alpha;
+        }
+        float rs = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) { const float pe = __builtin_amdgcn_exp2f(s[kb][e] * sl2 - m); s[kb][e] = pe; rs += pe; }
+        l += rs;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {                          // O^T += V^T . P^T, P rounded to the products' bf16
+            const bf16x8_t pf = pack_frag(s[u >> 1], 8 * (u & 1));
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) oacc[db] = mfma16(by_cols(Vl, 32 * db, 16 * u, lane), pf, oacc[db]);
+        }
     }
 
+    const float sum = sum_halves(l);
+    if (!r.live) return;
+    const float inv = sum > 0.f ? 1.f / sum : sum;             // nothing seen: 0;  NaN stays NaN
+    const float lse = sum == 0.f ? (SPLIT ? -INFINITY : INFINITY) : m + __builtin_amdgcn_logf(sum);      // v_log_f32 = log2
+    const long row = r.token * p.hq + r.head, at = r.head * p.tq + r.token, part = SPLIT ? w.part * p.tq * p.hq : 0;
+    if (h == 0 && (SPLIT || p.lse)) (SPLIT ? p.part_lse + part : p.lse)[at] = lse;
+    if (SPLIT && sum == 0.f) return;                           // the join does not read this row
+    float* f32 = SPLIT ? p.part + (part + row) * D : p.o32 ? p.o32 + row * D : nullptr;
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-        const float lsum = sum_halves(l[qb]);
-        if (orow[qb] < 0) continue;
-        const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);          // nothing seen: 0;  NaN stays NaN
-        const long tok = orow[qb] / p.hq, hd = orow[qb] - tok * p.hq;
-        const float lse = lsum == 0.f ? (SPLIT ? -INFINITY : INFINITY) : m[qb] + __builtin_amdgcn_logf(lsum);      // v_log_f32 = log2
-        float* f32 = SPLIT ? p.part + ((long)split * p.tq * p.hq + orow[qb]) * D : p.o32 ? p.o32 + orow[qb] * D : nullptr;
-        if (h == 0 && (SPLIT || p.lse)) (SPLIT ? p.part_lse + (long)split * p.tq * p.hq : p.lse)[hd * p.tq + tok] = lse;
-        if (SPLIT && lsum == 0.f) continue;                    // the join does not read this row
-        bf16_t* O = p.o + orow[qb] * D;
+    for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int eg = 0; eg < 4; ++eg) {
-                const float4 v = make_float4(oacc[qb][db][4 * eg] * inv, oacc[qb][db][4 * eg + 1] * inv, oacc[qb][db][4 * eg + 2] * inv, oacc[qb][db][4 * eg + 3] * inv);
-                const int d = 32 * db + 8 * eg + 4 * h;
-                if (!SPLIT) *reinterpret_cast<uint2*>(O + d) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-                if (f32) *reinterpret_cast<float4*>(f32 + d) = v;
-            }
-    }
+        for (int eg = 0; eg < 4; ++eg) {
+            const float4 v = make_float4(oacc[db][4 * eg] * inv, oacc[db][4 * eg + 1] * inv, oacc[db][4 * eg + 2] * inv, oacc[db][4 * eg + 3] * inv);
+            const int d = 32 * db + 8 * eg + 4 * h;
+            if (!SPLIT) *reinterpret_cast<uint2*>(p.o + row * D + d) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+            if (f32) *reinterpret_cast<float4*>(f32 + d) = v;
+        }
 }
 
-// joins the parts of a row: o = sum_s 2^(lse_s - top) o_s / sum_s 2^(lse_s - top); one thread per 4 channels
+// joins the parts of a row: o = sum_s 2^(lse_s - top) o_s / sum_s 2^(lse_s - top); one wave per row, its lanes hold the parts' weights (nsplit <= 64), then D / 64 channels each
 template <int D>
-__global__ void __launch_bounds__(256) varlen_join_kernel(const VarlenParams p) {
-    const long idx = (long)blockIdx.x * 256 + threadIdx.x, rows = p.tq * p.hq, row = idx / (D / 4);
+__global__ void __launch_bounds__(NT) varlen_join_kernel(const VarlenParams p) {
+    constexpr int C = D / 64;
+    const long rows = p.tq * p.hq, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= rows) return;
-    const int d = 4 * (int)(idx % (D / 4));
-    const long tok = row / p.hq, hd = row - tok * p.hq, at = hd * p.tq + tok;
-    float top = -INFINITY;
-    for (int s = 0; s < p.nsplit; ++s) top = fmaxf(top, p.part_lse[s * rows + at]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll 4
+    const int lane = threadIdx.x & 63;
+    const long tok = row / p.hq, at = (row - tok * p.hq) * p.tq + tok;
+    const float ls = lane < p.nsplit ? p.part_lse[lane * rows + at] : -INFINITY;
+    const float top = wave_max(ls), base = top == -INFINITY ? 0.f : top;
+    const float w = __builtin_amdgcn_exp2f(ls - base), sum = wave_sum(w);
+    float a[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) a[c] = 0.f;
+#pragma unroll 8
     for (int s = 0; s < p.nsplit; ++s) {
-        const float ls = p.part_lse[s * rows + at];
-        if (ls == -INFINITY) continue;
-        const float w = __builtin_amdgcn_exp2f(ls - base);
-        const float4 v = *reinterpret_cast<const float4*>(p.part + (s * rows + row) * D + d);
-        a.x += w * v.x; a.y += w * v.y; a.z += w * v.z; a.w += w * v.w; sum += w;
+        const float ws = __shfl(w, s, 64);
+        const bool stored = __shfl(ls, s, 64) != -INFINITY;    // a part that saw nothing stored nothing: what is read there does not count
+        const float* src = p.part + (s * rows + row) * D + lane * C;
+#pragma unroll
+        for (int c = 0; c < C; ++c) { const float v = src[c]; a[c] += stored ? ws * v : 0.f; }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
-    *reinterpret_cast<uint2*>(p.o + row * D + d) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
-    if (p.o32) *reinterpret_cast<float4*>(p.o32 + row * D + d) = a;
-    if (d == 0 && p.lse) p.lse[at] = sum == 0.f ? INFINITY : base + __builtin_amdgcn_logf(sum);
+    const float inv = sum > 0.f ? 1.f / sum : sum;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        a[c] *= inv;
+        p.o[row * D + lane * C + c] = f32_to_bf16(a[c]);
+        if (p.o32) p.o32[row * D + lane * C + c] = a[c];
+    }
+    if (lane == 0 && p.lse) p.lse[at] = sum == 0.f ? INFINITY : base + __builtin_amdgcn_logf(sum);
 }
 
 // ================================================================================================ backward: dQ (and delta)
-// Per 64-key tile three images: K by rows (S^T = K . Q^T), K transposed (dQ^T += K^T . dS^T), V by rows (dP^T = V . dO^T).
-template <int D, int QB, int NW>
-__global__ void __launch_bounds__(NW * 64, (NW == 8 || D == 64) && QB == 1 ? 2 : 1) varlen_dq_kernel(const VarlenParams p) {
-    constexpr int QW = 32 * QB, QWG = QW * NW, NKS = D / 16, NDB = D / 32, IMG = KT * D * 2, STAGE = 3 * IMG;
+// Per 64-key tile: K, read by rows (S^T = K . Q^T) and transposed (dQ^T += K^T . dS^T), and V by rows (dP^T = V . dO^T).
+template <int D>
+__global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const VarlenParams p) {
+    constexpr int NKS = D / 16, NDB = D / 32, IMG = KT * D * 2, STAGE = 2 * IMG;
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-    const int L = xcd_order(blockIdx.x, gridDim.x);
-    const int kh = L / p.slots;
-    const Tile t = find_tile<QWG>(p, L % p.slots, false, p.causal);
+    const Work w = find_work(blockIdx.x, p.hk, 1);
+    const Tile t = find_tile<ROWS>(p, w.slot, false, p.causal);
     if (!t.live) return;
 
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
-    const long r0 = t.row0 + wid * QW;
-    const int seen = t.lk - t.lq;
-    const bf16_t* K = p.k + t.k0 * p.k_ss + kh * p.k_sh;
-    const bf16_t* V = p.v + t.k0 * p.v_ss + kh * p.v_sh;
+    const Row r = find_row(p, t, w.head, wid, i);
+    const Seen seen = keys_seen(p, t, wid);
+    const bf16_t* K = p.k + t.k0 * p.k_ss + w.head * p.k_sh;
+    const bf16_t* V = p.v + t.k0 * p.v_ss + w.head * p.v_sh;
+    const bf16_t* Q = p.q + r.token * p.q_ss + r.head * p.q_sh;
+    const bf16_t* DO = p.dout + r.token * p.do_ss + r.head * p.do_sh;
+    const long row = r.token * p.hq + r.head, at = r.head * p.tq + r.token;
     const float sl2 = p.scale * LOG2E;
 
-    bf16x8_t qf[QB][NKS], dof[QB][NKS];
-    long orow[QB];
-    int lim[QB];
-    float lse[QB], dl[QB];
+    bf16x8_t qf[NKS], dof[NKS];
+    float dl = 0.f;
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-        const long r = r0 + 32 * qb + i;
-        const bool live = r < t.rows;
-        const unsigned tok = live ? (unsigned)r / (unsigned)p.g : 0u, hd = live ? (unsigned)r - tok * (unsigned)p.g : 0u;
-        const long head = kh * p.g + hd;
-        orow[qb] = live ? (t.q0 + tok) * p.hq + head : -1;
-        lim[qb] = p.causal ? (int)min((long)tok + seen, (long)t.lk - 1) : t.lk - 1;
-        const bf16_t* Q = p.q + (t.q0 + tok) * p.q_ss + head * p.q_sh;
-        const bf16_t* DO = p.dout + (t.q0 + tok) * p.do_ss + head * p.do_sh;
-        float d = 0.f;
+    for (int ks = 0; ks < NKS; ++ks) {
+        qf[ks] = r.live ? *reinterpret_cast<const bf16x8_t*>(Q + 16 * ks + 8 * h) : zero_frag();
+        dof[ks] = r.live ? *reinterpret_cast<const bf16x8_t*>(DO + 16 * ks + 8 * h) : zero_frag();
+        if (r.live) {
+            const float4 a = *reinterpret_cast<const float4*>(p.o32 + row * D + 16 * ks + 8 * h), c = *reinterpret_cast<const float4*>(p.o32 + row * D + 16 * ks + 8 * h + 4);
+            const float of[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) {
-            qf[qb][ks] = live ? *reinterpret_cast<const bf16x8_t*>(Q + 16 * ks + 8 * h) : zero_frag();
-            dof[qb][ks] = live ? *reinterpret_cast<const bf16x8_t*>(DO + 16 * ks + 8 * h) : zero_frag();
-            if (live) {
-                const float4 a = *reinterpret_cast<const float4*>(p.o32 + orow[qb] * D + 16 * ks + 8 * h), c = *reinterpret_cast<const float4*>(p.o32 + orow[qb] * D + 16 * ks + 8 * h + 4);
-                const float of[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) d += of[e] * bf16_to_f32((bf16_t)dof[qb][ks][e]);
-            }
+            for (int e = 0; e < 8; ++e) dl += of[e] * bf16_to_f32((bf16_t)dof[ks][e]);
         }
-        dl[qb] = sum_halves(d);
-        const long at = head * p.tq + t.q0 + tok;
-        lse[qb] = live ? p.lse[at] : INFINITY;
-        if (live && h == 0) p.delta[at] = dl[qb];
     }
-    f32x16 dq[QB][NDB];
+    dl = sum_halves(dl);
+    const float lse = r.live ? p.lse[at] : INFINITY;
+    if (r.live && h == 0) p.delta[at] = dl;
+    f32x16 dq[NDB];
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) dq[qb][db] = zero16();
+    for (int db = 0; db < NDB; ++db) dq[db] = zero16();
 
-    const long last = min(t.row0 + QWG, t.rows) - 1, wlast = min(r0 + QW, t.rows) - 1;
-    const int wg_keys = p.causal ? (int)max(0l, min((long)t.lk, last / p.g + seen + 1)) : t.lk;
-    const int w_keys = wlast < r0 ? 0 : p.causal ? (int)max(0l, min((long)t.lk, wlast / p.g + seen + 1)) : t.lk;
-    const int w_full = wlast < r0 ? 0 : p.causal ? (int)max(0l, min((long)t.lk, r0 / p.g + seen + 1)) : t.lk;
-    const int nkt = (wg_keys + KT - 1) / KT;
-
-    Offsets<D, NW> oKc, oKm, oVc;
-    oKc.template init<false>(wid, lane, p.k_ss); oKm.template init<true>(wid, lane, p.k_ss); oVc.template init<false>(wid, lane, p.v_ss);
+    const int nkt = (seen.group + KT - 1) / KT;
+    Offsets<D, 4> oK, oV;
+    oK.init(wid, lane, p.k_ss); oV.init(wid, lane, p.v_ss);
     auto issue = [&](int kt) {
         char* base = lds + (kt & 1) * STAGE;
-        const auto rk = rows_rsrc<D>(K, p.k_ss, kt * KT, t.lk);
-        oKc.issue(rk, base, wid); oKm.issue(rk, base + IMG, wid);
-        oVc.issue(rows_rsrc<D>(V, p.v_ss, kt * KT, t.lk), base + 2 * IMG, wid);
+        oK.issue(rows_rsrc<D>(K, p.k_ss, kt * KT, t.lk), base, wid);
+        oV.issue(rows_rsrc<D>(V, p.v_ss, kt * KT, t.lk), base + IMG, wid);
     };
     if (nkt > 0) issue(0);
     for (int kt = 0; kt < nkt; ++kt) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         if (kt + 1 < nkt) issue(kt + 1);
-        const char* Kc = lds + (kt & 1) * STAGE;
-        const char* Km = Kc + IMG;
-        const char* Vc = Kc + 2 * IMG;
+        const char* Kl = lds + (kt & 1) * STAGE;
+        const char* Vl = Kl + IMG;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             const int key0 = kt * KT + 32 * kb;
-            if (key0 >= w_keys) break;
-            f32x16 s[QB], dp[QB];
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) { s[qb] = zero16(); dp[qb] = zero16(); }
+            if (key0 >= seen.wave) break;
+            f32x16 s = zero16(), dp = zero16();
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) {
-                const bf16x8_t kf = read_frag<false, KT>(Kc + (ks / 4) * (KT * 128), 32 * kb, ks & 3, lane), vf = read_frag<false, KT>(Vc + (ks / 4) * (KT * 128), 32 * kb, ks & 3, lane);
-#pragma unroll
-                for (int qb = 0; qb < QB; ++qb) { s[qb] = mfma16(kf, qf[qb][ks], s[qb]); dp[qb] = mfma16(vf, dof[qb][ks], dp[qb]); }
+                s = mfma16(by_rows(Kl, 32 * kb, ks, lane), qf[ks], s);
+                dp = mfma16(by_rows(Vl, 32 * kb, ks, lane), dof[ks], dp);
             }
-            bf16x8_t ds[QB][2];
+            if (key0 + 32 > seen.all) {
 #pragma unroll
-            for (int qb = 0; qb < QB; ++qb) {
-                if (key0 + 32 > w_full) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s[qb][e] = key0 + (e & 3) + 8 * (e >> 2) + 4 * h <= lim[qb] ? s[qb][e] : -INFINITY;
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[qb][e] = __builtin_amdgcn_exp2f(s[qb][e] * sl2 - lse[qb]) * (dp[qb][e] - dl[qb]);
-                ds[qb][0] = pack_frag(s[qb], 0); ds[qb][1] = pack_frag(s[qb], 8);
+                for (int e = 0; e < 16; ++e) s[e] = key0 + (e & 3) + 8 * (e >> 2) + 4 * h <= r.last ? s[e] : -INFINITY;
             }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * sl2 - lse) * (dp[e] - dl);
+            const bf16x8_t ds[2] = {pack_frag(s, 0), pack_frag(s, 8)};
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int db = 0; db < NDB; ++db) {
-                    const bf16x8_t kf = read_frag_tr_acc<D>(Km, 32 * db, 32 * kb + 16 * u, lane);
-#pragma unroll
-                    for (int qb = 0; qb < QB; ++qb) dq[qb][db] = mfma16(kf, ds[qb][u], dq[qb][db]);
-                }
+                for (int db = 0; db < NDB; ++db) dq[db] = mfma16(by_cols(Kl, 32 * db, 32 * kb + 16 * u, lane), ds[u], dq[db]);
         }
     }
+    if (!r.live) return;
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-        if (orow[qb] < 0) continue;
-        bf16_t* DQ = p.dq + orow[qb] * D;
+    for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int eg = 0; eg < 4; ++eg)
-                *reinterpret_cast<uint2*>(DQ + 32 * db + 8 * eg + 4 * h) =
-                    make_uint2(pack_bf16x2(dq[qb][db][4 * eg] * p.scale, dq[qb][db][4 * eg + 1] * p.scale), pack_bf16x2(dq[qb][db][4 * eg + 2] * p.scale, dq[qb][db][4 * eg + 3] * p.scale));
-    }
+        for (int eg = 0; eg < 4; ++eg)
+            *reinterpret_cast<uint2*>(p.dq + row * D + 32 * db + 8 * eg + 4 * h) =
+                make_uint2(pack_bf16x2(dq[db][4 * eg] * p.scale, dq[db][4 * eg + 1] * p.scale), pack_bf16x2(dq[db][4 * eg + 2] * p.scale, dq[db][4 * eg + 3] * p.scale));
 }
 
 // ================================================================================================ backward: dK, dV
-// Key-outer; a lane owns one key column per block:  S = Q . K^T, dP = dO . V^T, dV^T += dO^T . P, dK^T += Q^T . dS.  Per 64-query tile four images (Q and dO, by rows and
-// transposed) and the tile's lse / delta.  Query rows past the sequence arrive as zeros (Q, dO, lse, delta): P = 1 there, but dO = 0 and dS = 0.  MODE 0: both; 1: dV; 2: dK.
-template <int D, int KB, int NW, int MODE>
-__global__ void __launch_bounds__(NW * 64, (NW == 8 || D == 64) && KB == 1 ? 2 : 1) varlen_dkv_kernel(const VarlenParams p) {
-    constexpr bool DO_K = MODE != 1, DO_V = MODE != 2;
-    constexpr int KW = 32 * KB, KWG = KW * NW, QT = 64, NKS = D / 16, NDB = D / 32, IMG = QT * D * 2, NIMG = 1 + (DO_V ? 1 : 0) + (DO_K ? 2 : 0), STAGE = NIMG * IMG + 1024;
-    constexpr int O_DOM = IMG, O_DOC = (1 + (DO_V ? 1 : 0)) * IMG, O_QM = O_DOC + IMG, O_STAT = NIMG * IMG;
+// Key-outer; a lane owns one key column:  S = Q . K^T, dP = dO . V^T, dV^T += dO^T . P, dK^T += Q^T . dS.  Per 64-query tile Q and dO, both read by rows and transposed, and the
+// tile's lse / delta.  Query rows past the sequence arrive as zeros (Q, dO, lse, delta): P = 1 there, but dO = 0 and dS = 0.
+template <int D>
+__global__ void __launch_bounds__(NT, 2) varlen_dkv_kernel(const VarlenParams p) {
+    constexpr int QT = KT, NKS = D / 16, NDB = D / 32, IMG = QT * D * 2, O_STAT = 2 * IMG, STAGE = O_STAT + 1024;
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-    int L = xcd_order(blockIdx.x, gridDim.x);
-    const int split = L % p.nsplit;
-    L /= p.nsplit;
-    const int kh = L / p.slots;
-    const Tile t = find_tile<KWG>(p, L % p.slots, true, false);
+    const Work w = find_work(blockIdx.x, p.hk, p.nsplit);
+    const Tile t = find_tile<ROWS>(p, w.slot, true, false);
     if (!t.live) return;
 
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
-    const int k0w = (int)t.row0 + wid * KW;                    // first key of this wave
-    const int seen = t.lk - t.lq;
+    const int k0w = (int)t.row0 + wid * 32, key = k0w + i;     // first key of this wave, this lane's key
+    const bool live = key < t.lk;
+    const int ahead = t.lk - t.lq;                             // causal: query x sees keys 0 .. x + ahead
     const float sl2 = p.scale * LOG2E;
-    bf16x8_t kf[KB][NKS], vf[KB][NKS];
+    const bf16_t* K = p.k + (t.k0 + (live ? key : 0)) * p.k_ss + w.head * p.k_sh;
+    const bf16_t* V = p.v + (t.k0 + (live ? key : 0)) * p.v_ss + w.head * p.v_sh;
+    bf16x8_t kf[NKS], vf[NKS];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-        const int key = k0w + 32 * kb + i;
-        const bool live = key < t.lk;
-        const bf16_t* K = p.k + (t.k0 + (live ? key : 0)) * p.k_ss + kh * p.k_sh;
-        const bf16_t* V = p.v + (t.k0 + (live ? key : 0)) * p.v_ss + kh * p.v_sh;
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) {
-            kf[kb][ks] = live ? *reinterpret_cast<const bf16x8_t*>(K + 16 * ks + 8 * h) : zero_frag();
-            if constexpr (DO_K) vf[kb][ks] = live ? *reinterpret_cast<const bf16x8_t*>(V + 16 * ks + 8 * h) : zero_frag();
-        }
+    for (int ks = 0; ks < NKS; ++ks) {
+        kf[ks] = live ? *reinterpret_cast<const bf16x8_t*>(K + 16 * ks + 8 * h) : zero_frag();
+        vf[ks] = live ? *reinterpret_cast<const bf16x8_t*>(V + 16 * ks + 8 * h) : zero_frag();
     }
-    f32x16 dk[KB][NDB], dv[KB][NDB];
+    f32x16 dk[NDB], dv[NDB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) { dk[kb][db] = zero16(); dv[kb][db] = zero16(); }
+    for (int db = 0; db < NDB; ++db) { dk[db] = zero16(); dv[db] = zero16(); }
 
-    // query tiles: from the first one that sees a key of this workgroup, for each of the g heads
-    const int qt0 = p.causal ? max(0, (int)t.row0 - seen) / QT : 0;
-    const int per_head = max(0, (t.lq + QT - 1) / QT - qt0);
+    // query tiles: from the first one that sees a key of this workgroup, for each of the g heads; this part's share of them
+    const int first = p.causal ? max(0, (int)t.row0 - ahead) / QT * QT : 0;
+    const int per_head = max(0, (t.lq - first + QT - 1) / QT);
     const long all = (long)per_head * p.g, per = (all + p.nsplit - 1) / p.nsplit;
-    const int it0 = (int)min(all, split * per), it1 = (int)min(all, it0 + per);
+    const int it0 = (int)min(all, w.part * per), count = (int)min(all, it0 + per) - it0;
+    int hd = per_head > 0 ? it0 / per_head : 0, q = first + (it0 - hd * per_head) * QT;      // of the tile to fetch next
+    const bf16_t* Q = p.q + t.q0 * p.q_ss + w.head * p.g * p.q_sh;
+    const bf16_t* DO = p.dout + t.q0 * p.do_ss + w.head * p.g * p.do_sh;
+    const long stat = (long)w.head * p.g * p.tq + t.q0;
 
-    Offsets<D, NW> oQc, oQm, oDc, oDm;
-    oQc.template init<false>(wid, lane, p.q_ss); oQm.template init<true>(wid, lane, p.q_ss);
-    oDc.template init<false>(wid, lane, p.do_ss); oDm.template init<true>(wid, lane, p.do_ss);
-    auto issue = [&](int it, int buf) {
-        const int hd = it / per_head, q = (qt0 + it - hd * per_head) * QT;
-        const long head = kh * p.g + hd;
+    Offsets<D, 4> oQ, oD;
+    oQ.init(wid, lane, p.q_ss); oD.init(wid, lane, p.do_ss);
+    auto issue = [&](int buf) {
         char* base = lds + buf * STAGE;
-        const auto rq = rows_rsrc<D>(p.q + t.q0 * p.q_ss + head * p.q_sh, p.q_ss, q, t.lq), rd = rows_rsrc<D>(p.dout + t.q0 * p.do_ss + head * p.do_sh, p.do_ss, q, t.lq);
-        oQc.issue(rq, base, wid);
-        if constexpr (DO_V) oDm.issue(rd, base + O_DOM, wid);
-        if constexpr (DO_K) { oDc.issue(rd, base + O_DOC, wid); oQm.issue(rq, base + O_QM, wid); }
-        const int rows = min(QT, t.lq - q);
-        if (wid == 0) dma4(tile_rsrc(p.lse + head * p.tq + t.q0 + q, rows * 4), base + O_STAT, lane * 4);
-        if (DO_K && wid == 1) dma4(tile_rsrc(p.delta + head * p.tq + t.q0 + q, rows * 4), base + O_STAT + 256, lane * 4);
+        oQ.issue(rows_rsrc<D>(Q + hd * p.q_sh, p.q_ss, q, t.lq), base, wid);
+        oD.issue(rows_rsrc<D>(DO + hd * p.do_sh, p.do_ss, q, t.lq), base + IMG, wid);
+        const int bytes = min(QT, t.lq - q) * 4;
+        if (wid == 0) dma4(tile_rsrc(p.lse + stat + hd * p.tq + q, bytes), base + O_STAT, lane * 4);
+        if (wid == 1) dma4(tile_rsrc(p.delta + stat + hd * p.tq + q, bytes), base + O_STAT + 256, lane * 4);
     };
-    if (it0 < it1) issue(it0, 0);
-    for (int it = it0; it < it1; ++it) {
-        const int buf = (it - it0) & 1;
+    if (count > 0) issue(0);
+    for (int it = 0; it < count; ++it) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        if (it + 1 < it1) issue(it + 1, buf ^ 1);
-        const int q00 = (qt0 + it % per_head) * QT;
-        const char* Qc = lds + buf * STAGE;
-        const char* DOm = Qc + O_DOM;
-        const char* DOc = Qc + O_DOC;
-        const char* Qm = Qc + O_QM;
-        const float* lse_l = reinterpret_cast<const float*>(Qc + O_STAT);
-        const float* dl_l = lse_l + 64;
+        const int qt = q;                                      // the tile at hand
+        q += QT;
+        if (q >= t.lq) { q = first; ++hd; }
+        if (it + 1 < count) issue((it + 1) & 1);
+        const char* Ql = lds + (it & 1) * STAGE;
+        const char* DOl = Ql + IMG;
+        const float* lse_l = reinterpret_cast<const float*>(Ql + O_STAT);
+        const float* dl_l = lse_l + QT;
         if (k0w >= t.lk) continue;                             // wave-uniform: no live key
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
-            const int q0 = q00 + 32 * qb;
+            const int q0 = qt + 32 * qb;
             if (q0 >= t.lq) break;
-            if (p.causal && q0 + 31 + seen < k0w) continue;    // no query of the block sees a key of this wave
-            f32x16 s[KB], dp[KB];
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) { s[kb] = zero16(); dp[kb] = zero16(); }
+            if (p.causal && q0 + 31 + ahead < k0w) continue;   // no query of the block sees a key of this wave
+            f32x16 s = zero16(), dp = zero16();
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) {
-                const bf16x8_t qf = read_frag<false, QT>(Qc + (ks / 4) * (QT * 128), 32 * qb, ks & 3, lane);
+                s = mfma16(by_rows(Ql, 32 * qb, ks, lane), kf[ks], s);
+                dp = mfma16(by_rows(DOl, 32 * qb, ks, lane), vf[ks], dp);
+            }
+            if (p.causal && q0 + ahead < k0w + 31) {           // some query of the block does not see every key of this wave
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) s[kb] = mfma16(qf, kf[kb][ks], s[kb]);
-                if constexpr (DO_K) {
-                    const bf16x8_t df = read_frag<false, QT>(DOc + (ks / 4) * (QT * 128), 32 * qb, ks & 3, lane);
+                for (int e = 0; e < 16; ++e) s[e] = key <= q0 + 8 * (e >> 2) + 4 * h + (e & 3) + ahead ? s[e] : -INFINITY;
+            }
+            f32x16 pr;
 #pragma unroll
-                    for (int kb = 0; kb < KB; ++kb) dp[kb] = mfma16(df, vf[kb][ks], dp[kb]);
+            for (int eg = 0; eg < 4; ++eg) {
+                const float4 l4 = *reinterpret_cast<const float4*>(&lse_l[32 * qb + 8 * eg + 4 * h]), d4 = *reinterpret_cast<const float4*>(&dl_l[32 * qb + 8 * eg + 4 * h]);
+                const float ll[4] = {l4.x, l4.y, l4.z, l4.w}, dd[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = 4 * eg + j;
+                    pr[e] = __builtin_amdgcn_exp2f(s[e] * sl2 - ll[j]);
+                    s[e] = pr[e] * (dp[e] - dd[j]);
                 }
             }
-            const bool masked = p.causal && q0 + seen < k0w + KW - 1;      // some query of the block does not see every key of this wave
-            bf16x8_t pf[KB][2], ds[KB][2];
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                const int key = k0w + 32 * kb + i;
-                if (masked) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s[kb][e] = key <= q0 + 8 * (e >> 2) + 4 * h + (e & 3) + seen ? s[kb][e] : -INFINITY;
-                }
-                f32x16 pr;
-#pragma unroll
-                for (int eg = 0; eg < 4; ++eg) {
-                    const float4 l4 = *reinterpret_cast<const float4*>(&lse_l[32 * qb + 8 * eg + 4 * h]);
-                    float4 d4 = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if constexpr (DO_K) d4 = *reinterpret_cast<const float4*>(&dl_l[32 * qb + 8 * eg + 4 * h]);
-                    const float ll[4] = {l4.x, l4.y, l4.z, l4.w}, dd[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int e = 4 * eg + j;
-                        pr[e] = __builtin_amdgcn_exp2f(s[kb][e] * sl2 - ll[j]);
-                        s[kb][e] = pr[e] * (dp[kb][e] - dd[j]);
-                    }
-                }
-                pf[kb][0] = pack_frag(pr, 0); pf[kb][1] = pack_frag(pr, 8);
-                ds[kb][0] = pack_frag(s[kb], 0); ds[kb][1] = pack_frag(s[kb], 8);
-            }
+            const bf16x8_t pf[2] = {pack_frag(pr, 0), pack_frag(pr, 8)}, ds[2] = {pack_frag(s, 0), pack_frag(s, 8)};
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int db = 0; db < NDB; ++db) {
-                    if constexpr (DO_V) {
-                        const bf16x8_t df = read_frag_tr_acc<D>(DOm, 32 * db, 32 * qb + 16 * u, lane);
-#pragma unroll
-                        for (int kb = 0; kb < KB; ++kb) dv[kb][db] = mfma16(df, pf[kb][u], dv[kb][db]);
-                    }
-                    if constexpr (DO_K) {
-                        const bf16x8_t qf = read_frag_tr_acc<D>(Qm, 32 * db, 32 * qb + 16 * u, lane);
-#pragma unroll
-                        for (int kb = 0; kb < KB; ++kb) dk[kb][db] = mfma16(qf, ds[kb][u], dk[kb][db]);
-                    }
+                    dv[db] = mfma16(by_cols(DOl, 32 * db, 32 * qb + 16 * u, lane), pf[u], dv[db]);
+                    dk[db] = mfma16(by_cols(Ql, 32 * db, 32 * qb + 16 * u, lane), ds[u], dk[db]);
                 }
         }
     }
+    if (!live) return;
+    const long row = ((t.k0 + key) * p.hk + w.head) * D, slice = p.tk * p.hk * D;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-        const int key = k0w + 32 * kb + i;
-        if (key >= t.lk) continue;
-        const long row = ((t.k0 + key) * p.hk + kh) * D, slice = p.tk * p.hk * D;
+    for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int eg = 0; eg < 4; ++eg) {
-                const long at = row + 32 * db + 8 * eg + 4 * h;
-                const float4 a = make_float4(dk[kb][db][4 * eg] * p.scale, dk[kb][db][4 * eg + 1] * p.scale, dk[kb][db][4 * eg + 2] * p.scale, dk[kb][db][4 * eg + 3] * p.scale);
-                const float4 c = make_float4(dv[kb][db][4 * eg], dv[kb][db][4 * eg + 1], dv[kb][db][4 * eg + 2], dv[kb][db][4 * eg + 3]);
-                if (p.nsplit > 1) {
-                    if constexpr (DO_K) *reinterpret_cast<float4*>(p.part + 2 * split * slice + at) = a;
-                    if constexpr (DO_V) *reinterpret_cast<float4*>(p.part + (2 * split + 1) * slice + at) = c;
-                } else {
-                    if constexpr (DO_K) *reinterpret_cast<uint2*>(p.dk + at) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
-                    if constexpr (DO_V) *reinterpret_cast<uint2*>(p.dv + at) = make_uint2(pack_bf16x2(c.x, c.y), pack_bf16x2(c.z, c.w));
-                }
+        for (int eg = 0; eg < 4; ++eg) {
+            const long at = row + 32 * db + 8 * eg + 4 * h;
+            const float4 a = make_float4(dk[db][4 * eg] * p.scale, dk[db][4 * eg + 1] * p.scale, dk[db][4 * eg + 2] * p.scale, dk[db][4 * eg + 3] * p.scale);
+            const float4 c = make_float4(dv[db][4 * eg], dv[db][4 * eg + 1], dv[db][4 * eg + 2], dv[db][4 * eg + 3]);
+            if (p.nsplit > 1) {
+                *reinterpret_cast<float4*>(p.part + 2 * w.part * slice + at) = a;
+                *reinterpret_cast<float4*>(p.part + (2 * w.part + 1) * slice + at) = c;
+            } else {
+                *reinterpret_cast<uint2*>(p.dk + at) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+                *reinterpret_cast<uint2*>(p.dv + at) = make_uint2(pack_bf16x2(c.x, c.y), pack_bf16x2(c.z, c.w));
             }
-    }
+        }
 }
 
 // dK / dV = sum of the parts in order, one thread per 4 channels
@@ -602,20 +541,21 @@ __global__ void __launch_bounds__(256) varlen_dkv_sum_kernel(const VarlenParams 
 // ------------------------------------------------------------------------------------------------ host side
 int row_slots(long tokens, int g, int n, int per) { return (int)(tokens * g / per + n + 1); }
 
+
 // parts of the key range: when the row tiles alone leave CUs idle, enough parts for two workgroups per CU, of at least 4 key tiles of an average sequence each
 int fwd_splits(long tq, long tk, int n, int hq, int hk) {
-    const long wgs = cdiv(tq * (hq / hk), 128) * hk, tiles = tk / n / KT;
+    const long wgs = cdiv(tq * (hq / hk), ROWS) * hk, tiles = tk / n / KT;
     if (wgs >= 256 || tiles < 8) return 1;
     long s = cdiv(512, wgs);
     if (s > tiles / 4) s = tiles / 4;
-    return (int)(s > 128 ? 128 : s);
+    return (int)(s > 64 ? 64 : s);
 }
-// parts of the query range for dK / dV, likewise
+// parts of the query tiles (of all g heads) for dK / dV, likewise; with grouped heads up to g parts also where the key tiles alone are fewer than 4 a CU
 int dkv_splits(long tq, long tk, int n, int hq, int hk) {
-    const long wgs = cdiv(tk, 128) * hk, tiles = tq / n / 64 * (hq / hk);
-    if (wgs >= 256 || tiles < 8) return 1;
-    long s = cdiv(512, wgs);
-    if (s > tiles / 4) s = tiles / 4;
+    const long wgs = cdiv(tk, ROWS) * hk, g = hq / hk, tiles = tq / n / KT * g;
+    long s = 1;
+    if (wgs < 256 && tiles >= 8) { s = cdiv(512, wgs); if (s > tiles / 4) s = tiles / 4; }
+    if (wgs < 1024 && g > 1 && tiles >= 8 * g) { long m = cdiv(1024, wgs); if (m > g) m = g; if (m > s) s = m; }
     return (int)(s > 64 ? 64 : s);
 }
 
@@ -629,42 +569,26 @@ int fill(VarlenParams& p, const char* what, const void* q, const void* k, const 
     if (!q || !k || !v || !cu_q || !cu_k || tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk) return bad("bad argument");
     if (D != 64 && D != 128) return bad("head dim must be 64 or 128", DPIPE_ERR_UNSUPPORTED);
     if (!(scale > 0.f) || scale > 1e30f) return bad("scale must be positive and finite");
-    if (tq * (hq / hk) >= (1l << 31) || tk >= (1l << 31) || ((tq * hq + tk * hk) / 128 + (n + 1l) * hk) * fwd_splits(tq, tk, n, hq, hk) >= (1l << 23) ||
-        (tk * hk / 128 + (n + 1l) * hk) * dkv_splits(tq, tk, n, hq, hk) >= (1l << 23)) return bad("too many rows or sequences", DPIPE_ERR_UNSUPPORTED);
+    const int fs = fwd_splits(tq, tk, n, hq, hk), bs = dkv_splits(tq, tk, n, hq, hk);
+    if (tq * (hq / hk) >= (1l << 31) || tk >= (1l << 31) || work_groups(tq * (hq / hk) / ROWS + n + 1, hk, fs) >= (1l << 23) || work_groups(tk / ROWS + n + 1, hk, bs) >= (1l << 23))
+        return bad("too many rows or sequences", DPIPE_ERR_UNSUPPORTED);
     if (!rows_ok(q, q_ss, q_sh, D) || !rows_ok(k, k_ss, k_sh, D) || !rows_ok(v, v_ss, v_sh, D)) return bad("tensors must be 16-byte aligned with strides multiple of 8 elements");
     p.q = (const bf16_t*)q; p.k = (const bf16_t*)k; p.v = (const bf16_t*)v; p.cu_q = cu_q; p.cu_k = cu_k; p.tq = tq; p.tk = tk; p.n = n; p.hq = hq; p.hk = hk; p.g = hq / hk;
     p.q_ss = q_ss; p.q_sh = q_sh; p.k_ss = k_ss; p.k_sh = k_sh; p.v_ss = v_ss; p.v_sh = v_sh; p.scale = scale; p.causal = causal != 0; p.nsplit = 1;
     return DPIPE_OK;
 }
 
-template <int D, int QB, int NW, bool SPLIT> void launch_fwd(VarlenParams& p, hipStream_t s) {
-    p.slots = row_slots(p.tq, p.g, p.n, 32 * QB * NW);
-    varlen_fwd_kernel<D, QB, NW, SPLIT><<<(unsigned)((long)p.slots * p.hk * p.nsplit), NW * 64, 0, s>>>(p);
+template <int D> void forward(const VarlenParams& p, hipStream_t s) {
+    const unsigned grid = (unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, p.nsplit);
+    if (p.nsplit == 1) { varlen_fwd_kernel<D, false><<<grid, NT, 0, s>>>(p); return; }
+    varlen_fwd_kernel<D, true><<<grid, NT, 0, s>>>(p);
+    varlen_join_kernel<D><<<(unsigned)cdiv(p.tq * p.hq, 4), NT, 0, s>>>(p);
 }
-template <int D> void forward(VarlenParams& p, hipStream_t s) {
-    if (p.nsplit > 1) {
-        launch_fwd<D, 1, 4, true>(p, s);
-        varlen_join_kernel<D><<<(unsigned)cdiv(p.tq * p.hq * (D / 4), 256), 256, 0, s>>>(p);
-    } else if (cdiv(p.tq * p.g, 256) * p.hk >= 192) {
-        launch_fwd<D, 1, 8, false>(p, s);
-    } else {
-        launch_fwd<D, 1, 4, false>(p, s);
-    }
-}
-template <int D, int QB, int NW> void launch_dq(VarlenParams& p, hipStream_t s) {
-    p.slots = row_slots(p.tq, p.g, p.n, 32 * QB * NW);
-    varlen_dq_kernel<D, QB, NW><<<(unsigned)((long)p.slots * p.hk), NW * 64, 0, s>>>(p);
-}
-template <int D, int KB, int NW, int MODE> void launch_dkv(VarlenParams& p, hipStream_t s) {
-    p.slots = row_slots(p.tk, 1, p.n, 32 * KB * NW);
-    varlen_dkv_kernel<D, KB, NW, MODE><<<(unsigned)((long)p.slots * p.hk * p.nsplit), NW * 64, 0, s>>>(p);
-}
-template <int D> void backward(VarlenParams& p, int splits, hipStream_t s) {
-    if (cdiv(p.tq * p.g, 256) * p.hk >= 192) launch_dq<D, 1, 8>(p, s); else launch_dq<D, 1, 4>(p, s);
-    p.nsplit = splits;
-    if (D == 128 && splits == 1 && cdiv(p.tk, 256) * p.hk >= 192) { launch_dkv<D, 1, 8, 1>(p, s); launch_dkv<D, 1, 8, 2>(p, s); }
-    else launch_dkv<D, 1, 4, 0>(p, s);
-    if (splits > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
+template <int D> void backward(VarlenParams& p, int parts, hipStream_t s) {
+    varlen_dq_kernel<D><<<(unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, 1), NT, 0, s>>>(p);
+    p.nsplit = parts;
+    varlen_dkv_kernel<D><<<(unsigned)work_groups(row_slots(p.tk, 1, p.n, ROWS), p.hk, parts), NT, 0, s>>>(p);
+    if (parts > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
 }
 
 }  // namespace
@@ -672,12 +596,12 @@ template <int D> void backward(VarlenParams& p, int splits, hipStream_t s) {
 extern "C" {
 
 long dpipe_attn_varlen_fwd_workspace_floats(long tq, long tk, int n, int hq, int hk, int D) {
-    if (tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk) return 0;
+    if (tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk || (D != 64 && D != 128)) return 0;
     const int s = fwd_splits(tq, tk, n, hq, hk);
     return s > 1 ? (long)s * tq * hq * (D + 1) : 0;
 }
 long dpipe_attn_varlen_bwd_workspace_floats(long tq, long tk, int n, int hq, int hk, int D) {
-    if (tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk) return 0;
+    if (tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk || (D != 64 && D != 128)) return 0;
     const int s = dkv_splits(tq, tk, n, hq, hk);
     return s > 1 ? 2l * s * tk * hk * D : 0;
 }
