@@ -8,8 +8,8 @@
 //
 // Rows: the g query heads that share a key head are one list of len_q * g rows (row r = token r / g, head r % g), so a single token already fills g rows of a tile and the
 // shared K / V are staged once for all of them; the dK / dV kernel walks the g heads and sums in registers (no atomics, one fixed order).
-// Tiles: sequence b owns the tile slots from  cu[b] * g / TILE + b  on -- at least ceil(rows / TILE) of them for any lengths, at most N + 1 unused ones in all --
-// so the grid follows from Tq, N and g alone; a workgroup finds its sequence with one wave-wide comparison, and neither the host nor a planning kernel has to know a length.
+// Tiles: there are at most rows / TILE + N + 1 tile slots for any lengths, so the grid follows from Tq, N and g alone; a workgroup finds its sequence in the offsets by itself
+// (find_tile), and neither the host nor a planning kernel has to know a length.
 // Few rows against long keys: the key range of every sequence is cut into `nsplit` parts (own workgroups, fp32 partial rows) that a second kernel joins.
 //
 // As in attention.hip everything is v_mfma_f32_32x32x16_bf16 on the transposed score tile S^T = K . Q^T (a lane owns one query column: softmax statistics are
@@ -28,8 +28,8 @@ namespace {
 
 struct VarlenParams {
     const bf16_t *q, *k, *v, *dout;
-    bf16_t *o, *dq, *dk, *dv;
-    float *lse, *delta, *o32;            // lse / delta [Hq][Tq]; o32 [Tq][Hq][D]: the unrounded output, kept for the backward's delta (may be null in the forward)
+    bf16_t *o, *o_lo, *dq, *dk, *dv;     // o_lo: what the rounding of o left, rounded: o + o_lo is the output to 2^-17, which the backward's delta is formed from (forward: may be null)
+    float *lse, *delta;                  // [Hq][Tq]
     const int *cu_q, *cu_k;
     float *part, *part_lse;              // split forms: forward rows [split][Tq][Hq][D] and their lse [split][Hq][Tq]; dK / dV [split][2][Tk][Hk][D]
     long tq, tk;
@@ -40,49 +40,64 @@ struct VarlenParams {
 
 constexpr int NT = 256, ROWS = 128;       // threads, query rows (dK / dV: keys) of a workgroup: 4 waves of 32
 constexpr int KT = 64;                   // keys (dK / dV: queries) per LDS tile
+constexpr int AQ = 4, AK = 1;            // steps of LDS operands read ahead of their products in the dQ and the dK / dV kernels
 constexpr float M_INIT = -3.0e38f;       // running maximum before the first key: finite, so that exp2(-inf - m) is 0 and never NaN
 constexpr float RESCALE_AT = 8.f;        // the accumulator is rescaled when the maximum grew by more than 2^8: P stays below 256, its relative rounding is the same
 
 // ------------------------------------------------------------------------------------------------ which sequence, which rows
-struct Tile { int b; long row0, rows; long q0, k0; int lq, lk; bool live; };
+struct Tile { long row0, rows, q0, k0; int lq, lk; bool live; };
 
-__device__ __forceinline__ long bound(const int* cu, int i, int n, long total) {
+// offset i of the ascending sums, kept inside the tensor (i > n: its end)
+__device__ __forceinline__ int bound(const int* cu, int i, int n, int total) {
     if (i == 0) return 0;
     if (i > n) return total;
-    const long c = cu[i];
+    const int c = cu[i];
     return c < 0 ? 0 : c > total ? total : c;
 }
-// slot -> sequence (n: the rows behind the last one) and its first row; PER = rows per tile, gg = rows per token on the tiled side
+// slot -> sequence and first row; PER = rows per tile, gg = rows per token on the tiled side.  Up to 64 sequences (a lane each): the tiles of the sequences with the longest other
+// side first -- the workgroups with the most work start first -- each sequence's tiles from its ascending sum on, the rows behind the last sequence (n) after them.  More sequences:
+// the slots from  start / PER + b  on, in order.  `reversed`: the last tile of a sequence (causal: the one that sees most) first.
 template <int PER>
 __device__ __forceinline__ Tile find_tile(const VarlenParams& p, int slot, bool keys, bool reversed) {
-    const int* cu = keys ? p.cu_k : p.cu_q;
-    const long total = keys ? p.tk : p.tq;
+    const int *cu = keys ? p.cu_k : p.cu_q, *cu2 = keys ? p.cu_q : p.cu_k;
+    const int total = (int)(keys ? p.tk : p.tq), total2 = (int)(keys ? p.tq : p.tk), n = p.n;
     const int gg = keys ? 1 : p.g, lane = threadIdx.x & 63;
-    int count = 0;
-    for (int base = 0; base <= p.n; base += 64) {
-        const int i = base + lane;
-        const bool at = i <= p.n && bound(cu, i, p.n, total) * gg / PER + i <= slot;
-        const int c = __popcll(__ballot(at));
-        count += c;
-        if (c < 64) break;
+    int b, at, s0, s1, o0 = 0, o1 = 0;   // sequence, tile of it, its range on the tiled side and on the other (the rows behind the last sequence have no other side)
+    if (n <= 64) {
+        const int i0 = min(lane, n - 1);
+        const int my_s0 = bound(cu, i0, n, total), my_s1 = max(my_s0, bound(cu, i0 + 1, n, total)), my_o0 = bound(cu2, i0, n, total2), my_o1 = max(my_o0, bound(cu2, i0 + 1, n, total2));
+        const int nt = ((my_s1 - my_s0) * gg + PER - 1) / PER, work = my_o1 - my_o0;
+        int start = 0, all = 0;
+        for (int i = 0; i < n; ++i) {
+            const int nt_i = __builtin_amdgcn_readlane(nt, i), work_i = __builtin_amdgcn_readlane(work, i);
+            start += work_i > work || (work_i == work && i < lane) ? nt_i : 0;
+            all += nt_i;
+        }
+        const unsigned long long here = __ballot(lane < n && slot >= start && slot < start + nt);
+        b = here ? __builtin_amdgcn_readfirstlane(__builtin_ctzll(here)) : n - 1;
+        s0 = __builtin_amdgcn_readlane(my_s0, b); s1 = __builtin_amdgcn_readlane(my_s1, b);
+        if (here) { at = slot - __builtin_amdgcn_readlane(start, b); o0 = __builtin_amdgcn_readlane(my_o0, b); o1 = __builtin_amdgcn_readlane(my_o1, b); }
+        else { at = slot - all; b = n; s0 = s1; s1 = max(s0, total); }
+    } else {
+        int count = 0;
+        for (int base = 0; base <= n; base += 64) {
+            const int i = base + lane;
+            const int c = __popcll(__ballot(i <= n && (long)bound(cu, i, n, total) * gg / PER + i <= slot));
+            count += c;
+            if (c < 64) break;
+        }
+        b = __builtin_amdgcn_readfirstlane(count - 1);
+        s0 = bound(cu, b, n, total); s1 = max(s0, bound(cu, b + 1, n, total));
+        at = slot - (int)((long)s0 * gg / PER + b);
+        if (b < n) { o0 = bound(cu2, b, n, total2); o1 = max(o0, bound(cu2, b + 1, n, total2)); }
     }
     Tile t;
-    t.b = __builtin_amdgcn_readfirstlane(count - 1);
-    const bool tail = t.b >= p.n;
-    const long s0 = bound(cu, t.b, p.n, total), s1 = max(s0, bound(cu, t.b + 1, p.n, total));
-    const long rows = (s1 - s0) * gg;
-    const int at = slot - (int)(s0 * gg / PER + t.b), nt = (int)((rows + PER - 1) / PER);
+    t.rows = (long)(s1 - s0) * gg;
+    const int nt = (int)((t.rows + PER - 1) / PER);
     t.live = at >= 0 && at < nt;         // (offsets that do not ascend reach no row outside their tensor)
     t.row0 = (long)(reversed ? nt - 1 - at : at) * PER;
-    t.rows = rows;
-    long o0 = 0, o1 = 0;                 // the other side of the sequence; the rows behind the last sequence have none
-    if (!tail) {
-        const int* cu2 = keys ? p.cu_q : p.cu_k;
-        const long total2 = keys ? p.tq : p.tk;
-        o0 = bound(cu2, t.b, p.n, total2); o1 = max(o0, t.b + 1 > p.n ? o0 : bound(cu2, t.b + 1, p.n, total2));
-    }
     t.q0 = keys ? o0 : s0; t.k0 = keys ? s0 : o0;
-    t.lq = (int)(keys ? o1 - o0 : s1 - s0); t.lk = (int)(keys ? s1 - s0 : o1 - o0);
+    t.lq = keys ? o1 - o0 : s1 - s0; t.lk = keys ? s1 - s0 : o1 - o0;
     return t;
 }
 
@@ -174,6 +189,24 @@ __device__ __forceinline__ bf16x8_t by_cols(const char* img, int col, int r0, in
     return out;
 }
 
+// N steps of products whose LDS operands are read AHEAD steps before their use: step j's products, then the reads of step j + AHEAD, in exactly this order.  (Left to itself the
+// compiler reads every operand right before its product and waits the LDS latency out each time: 56 % of all wave cycles of the dK / dV kernel.)
+template <int AHEAD, typename Frag, typename Load>
+__device__ __forceinline__ void ahead_start(Frag (&f)[AHEAD], Load load) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) f[j] = load(j);
+    __builtin_amdgcn_sched_barrier(0);
+}
+template <int N, int AHEAD, typename Frag, typename Load, typename Use>
+__device__ __forceinline__ void ahead_run(Frag (&f)[AHEAD], Load load, Use use) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        use(j, f[j % AHEAD]);
+        if (j + AHEAD < N) f[j % AHEAD] = load(j + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 __device__ __forceinline__ float max_halves(float x) {        // max over lane and lane ^ 32, in both
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -181,6 +214,27 @@ __device__ __forceinline__ float max_halves(float x) {        // max over lane a
 __device__ __forceinline__ float sum_halves(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// 32 channels of a lane's row from a transposed accumulator (the lane holds channels 8 e + 4 h + 0 .. 3): halves exchanged with lane ^ 32, two 16-byte stores a lane.
+// `lo`: where the rounding's remainders go (null: nowhere)
+__device__ __forceinline__ void store_row(bf16_t* dst, bf16_t* lo, const f32x16& a, float scale, int h) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        uint32_t w[4], r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = a[8 * j + 2 * i] * scale, y = a[8 * j + 2 * i + 1] * scale;
+            w[i] = pack_bf16x2(x, y);
+            r[i] = pack_bf16x2(x - __uint_as_float(w[i] << 16), y - __uint_as_float(w[i] & 0xffff0000u));
+        }
+        auto p0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), p1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+        *reinterpret_cast<uint4*>(dst + 16 * j + 8 * h) = make_uint4(p0[0], p1[0], p0[1], p1[1]);
+        if (lo) {
+            p0 = __builtin_amdgcn_permlane32_swap(r[0], r[2], false, false); p1 = __builtin_amdgcn_permlane32_swap(r[1], r[3], false, false);
+            *reinterpret_cast<uint4*>(lo + 16 * j + 8 * h) = make_uint4(p0[0], p1[0], p0[1], p1[1]);
+        }
+    }
 }
 
 // ================================================================================================ forward
@@ -276,16 +330,14 @@ __global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const VarlenParams p)
     const long row = r.token * p.hq + r.head, at = r.head * p.tq + r.token, part = SPLIT ? w.part * p.tq * p.hq : 0;
     if (h == 0 && (SPLIT || p.lse)) (SPLIT ? p.part_lse + part : p.lse)[at] = lse;
     if (SPLIT && sum == 0.f) return;                           // the join does not read this row
-    float* f32 = SPLIT ? p.part + (part + row) * D : p.o32 ? p.o32 + row * D : nullptr;
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
+    for (int db = 0; db < NDB; ++db) {
+        if (!SPLIT) { store_row(p.o + row * D + 32 * db, p.o_lo ? p.o_lo + row * D + 32 * db : nullptr, oacc[db], inv, h); continue; }
 #pragma unroll
-        for (int eg = 0; eg < 4; ++eg) {
-            const float4 v = make_float4(oacc[db][4 * eg] * inv, oacc[db][4 * eg + 1] * inv, oacc[db][4 * eg + 2] * inv, oacc[db][4 * eg + 3] * inv);
-            const int d = 32 * db + 8 * eg + 4 * h;
-            if (!SPLIT) *reinterpret_cast<uint2*>(p.o + row * D + d) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-            if (f32) *reinterpret_cast<float4*>(f32 + d) = v;
-        }
+        for (int eg = 0; eg < 4; ++eg)
+            *reinterpret_cast<float4*>(p.part + (part + row) * D + 32 * db + 8 * eg + 4 * h) =
+                make_float4(oacc[db][4 * eg] * inv, oacc[db][4 * eg + 1] * inv, oacc[db][4 * eg + 2] * inv, oacc[db][4 * eg + 3] * inv);
+    }
 }
 
 // joins the parts of a row: o = sum_s 2^(lse_s - top) o_s / sum_s 2^(lse_s - top); one wave per row, its lanes hold the parts' weights (nsplit <= 64), then D / 64 channels each
@@ -302,20 +354,28 @@ __global__ void __launch_bounds__(NT) varlen_join_kernel(const VarlenParams p) {
     float a[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) a[c] = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < p.nsplit; ++s) {
-        const float ws = __shfl(w, s, 64);
-        const bool stored = __shfl(ls, s, 64) != -INFINITY;    // a part that saw nothing stored nothing: what is read there does not count
-        const float* src = p.part + (s * rows + row) * D + lane * C;
+    for (int s0 = 0; s0 < p.nsplit; s0 += 16) {                // 16 parts' reads in flight
+        float v[16][C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) { const float v = src[c]; a[c] += stored ? ws * v : 0.f; }
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+            for (int c = 0; c < C; ++c) v[j][c] = p.part[(min(s0 + j, p.nsplit - 1) * rows + row) * D + lane * C + c];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {                         // a part that saw nothing has stored nothing: what is read there does not count
+            const int s = min(s0 + j, 63);
+            const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
+            const bool stored = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ls), s)) != -INFINITY;      // (lanes from nsplit on hold -inf)
+#pragma unroll
+            for (int c = 0; c < C; ++c) a[c] += stored ? ws * v[j][c] : 0.f;
+        }
     }
     const float inv = sum > 0.f ? 1.f / sum : sum;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         a[c] *= inv;
-        p.o[row * D + lane * C + c] = f32_to_bf16(a[c]);
-        if (p.o32) p.o32[row * D + lane * C + c] = a[c];
+        const bf16_t hi = f32_to_bf16(a[c]);
+        p.o[row * D + lane * C + c] = hi;
+        if (p.o_lo) p.o_lo[row * D + lane * C + c] = f32_to_bf16(a[c] - bf16_to_f32(hi));
     }
     if (lane == 0 && p.lse) p.lse[at] = sum == 0.f ? INFINITY : base + __builtin_amdgcn_logf(sum);
 }
@@ -347,10 +407,9 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const VarlenParams p) 
         qf[ks] = r.live ? *reinterpret_cast<const bf16x8_t*>(Q + 16 * ks + 8 * h) : zero_frag();
         dof[ks] = r.live ? *reinterpret_cast<const bf16x8_t*>(DO + 16 * ks + 8 * h) : zero_frag();
         if (r.live) {
-            const float4 a = *reinterpret_cast<const float4*>(p.o32 + row * D + 16 * ks + 8 * h), c = *reinterpret_cast<const float4*>(p.o32 + row * D + 16 * ks + 8 * h + 4);
-            const float of[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+            const bf16x8_t oh = *reinterpret_cast<const bf16x8_t*>(p.o + row * D + 16 * ks + 8 * h), ol = *reinterpret_cast<const bf16x8_t*>(p.o_lo + row * D + 16 * ks + 8 * h);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dl += of[e] * bf16_to_f32((bf16_t)dof[ks][e]);
+            for (int e = 0; e < 8; ++e) dl += (bf16_to_f32((bf16_t)oh[e]) + bf16_to_f32((bf16_t)ol[e])) * bf16_to_f32((bf16_t)dof[ks][e]);
         }
     }
     dl = sum_halves(dl);
@@ -380,11 +439,12 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const VarlenParams p) 
             const int key0 = kt * KT + 32 * kb;
             if (key0 >= seen.wave) break;
             f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) {
-                s = mfma16(by_rows(Kl, 32 * kb, ks, lane), qf[ks], s);
-                dp = mfma16(by_rows(Vl, 32 * kb, ks, lane), dof[ks], dp);
-            }
+            bf16x8_t f[AQ], kt[AQ];
+            auto load = [&](int j) { return by_rows(j & 1 ? Vl : Kl, 32 * kb, j >> 1, lane); };
+            auto load_t = [&](int j) { return by_cols(Kl, 32 * (j % NDB), 32 * kb + 16 * (j / NDB), lane); };
+            ahead_start(f, load);
+            ahead_run<2 * NKS>(f, load, [&](int j, const bf16x8_t& x) { if (j & 1) dp = mfma16(x, dof[j >> 1], dp); else s = mfma16(x, qf[j >> 1], s); });
+            ahead_start(kt, load_t);
             if (key0 + 32 > seen.all) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = key0 + (e & 3) + 8 * (e >> 2) + 4 * h <= r.last ? s[e] : -INFINITY;
@@ -392,30 +452,24 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const VarlenParams p) 
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * sl2 - lse) * (dp[e] - dl);
             const bf16x8_t ds[2] = {pack_frag(s, 0), pack_frag(s, 8)};
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int db = 0; db < NDB; ++db) dq[db] = mfma16(by_cols(Kl, 32 * db, 32 * kb + 16 * u, lane), ds[u], dq[db]);
+            __builtin_amdgcn_sched_barrier(0);
+            ahead_run<2 * NDB>(kt, load_t, [&](int j, const bf16x8_t& x) { dq[j % NDB] = mfma16(x, ds[j / NDB], dq[j % NDB]); });
         }
     }
     if (!r.live) return;
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int eg = 0; eg < 4; ++eg)
-            *reinterpret_cast<uint2*>(p.dq + row * D + 32 * db + 8 * eg + 4 * h) =
-                make_uint2(pack_bf16x2(dq[db][4 * eg] * p.scale, dq[db][4 * eg + 1] * p.scale), pack_bf16x2(dq[db][4 * eg + 2] * p.scale, dq[db][4 * eg + 3] * p.scale));
+    for (int db = 0; db < NDB; ++db) store_row(p.dq + row * D + 32 * db, nullptr, dq[db], p.scale, h);
 }
 
 // ================================================================================================ backward: dK, dV
-// Key-outer; a lane owns one key column:  S = Q . K^T, dP = dO . V^T, dV^T += dO^T . P, dK^T += Q^T . dS.  Per 64-query tile Q and dO, both read by rows and transposed, and the
+// Key-outer; a lane owns one key column, K stays in LDS, V and both accumulators in registers:  S = Q . K^T, dP = dO . V^T, dV^T += dO^T . P, dK^T += Q^T . dS.  Per 64-query tile Q and dO, both read by rows and transposed, and the
 // tile's lse / delta.  Query rows past the sequence arrive as zeros (Q, dO, lse, delta): P = 1 there, but dO = 0 and dS = 0.
-template <int D>
-__global__ void __launch_bounds__(NT, 2) varlen_dkv_kernel(const VarlenParams p) {
+template <int D, int NW>
+__global__ void __launch_bounds__(NW * 64, D == 64 ? 3 : 2) varlen_dkv_kernel(const VarlenParams p) {
     constexpr int QT = KT, NKS = D / 16, NDB = D / 32, IMG = QT * D * 2, O_STAT = 2 * IMG, STAGE = O_STAT + 1024;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE + NW / 2 * IMG];
     const Work w = find_work(blockIdx.x, p.hk, p.nsplit);
-    const Tile t = find_tile<ROWS>(p, w.slot, true, false);
+    const Tile t = find_tile<32 * NW>(p, w.slot, true, false);
     if (!t.live) return;
 
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
@@ -423,14 +477,10 @@ __global__ void __launch_bounds__(NT, 2) varlen_dkv_kernel(const VarlenParams p)
     const bool live = key < t.lk;
     const int ahead = t.lk - t.lq;                             // causal: query x sees keys 0 .. x + ahead
     const float sl2 = p.scale * LOG2E;
-    const bf16_t* K = p.k + (t.k0 + (live ? key : 0)) * p.k_ss + w.head * p.k_sh;
     const bf16_t* V = p.v + (t.k0 + (live ? key : 0)) * p.v_ss + w.head * p.v_sh;
-    bf16x8_t kf[NKS], vf[NKS];
+    bf16x8_t vf[NKS];
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-        kf[ks] = live ? *reinterpret_cast<const bf16x8_t*>(K + 16 * ks + 8 * h) : zero_frag();
-        vf[ks] = live ? *reinterpret_cast<const bf16x8_t*>(V + 16 * ks + 8 * h) : zero_frag();
-    }
+    for (int ks = 0; ks < NKS; ++ks) vf[ks] = live ? *reinterpret_cast<const bf16x8_t*>(V + 16 * ks + 8 * h) : zero_frag();
     f32x16 dk[NDB], dv[NDB];
 #pragma unroll
     for (int db = 0; db < NDB; ++db) { dk[db] = zero16(); dv[db] = zero16(); }
@@ -445,7 +495,14 @@ __global__ void __launch_bounds__(NT, 2) varlen_dkv_kernel(const VarlenParams p)
     const bf16_t* DO = p.dout + t.q0 * p.do_ss + w.head * p.g * p.do_sh;
     const long stat = (long)w.head * p.g * p.tq + t.q0;
 
-    Offsets<D, 4> oQ, oD;
+    const char* Kl = lds + 2 * STAGE + wid / 2 * IMG;         // this wave's keys: rows 32 (wid & 1) .. of the image
+    if (count > 0) {
+        Offsets<D, NW> oK;
+        oK.init(wid, lane, p.k_ss);
+#pragma unroll
+        for (int c = 0; c < NW / 2; ++c) oK.issue(rows_rsrc<D>(p.k + t.k0 * p.k_ss + w.head * p.k_sh, p.k_ss, (int)t.row0 + KT * c, t.lk), lds + 2 * STAGE + c * IMG, wid);
+    }
+    Offsets<D, NW> oQ, oD;
     oQ.init(wid, lane, p.q_ss); oD.init(wid, lane, p.do_ss);
     auto issue = [&](int buf) {
         char* base = lds + buf * STAGE;
@@ -474,11 +531,15 @@ __global__ void __launch_bounds__(NT, 2) varlen_dkv_kernel(const VarlenParams p)
             if (q0 >= t.lq) break;
             if (p.causal && q0 + 31 + ahead < k0w) continue;   // no query of the block sees a key of this wave
             f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) {
-                s = mfma16(by_rows(Ql, 32 * qb, ks, lane), kf[ks], s);
-                dp = mfma16(by_rows(DOl, 32 * qb, ks, lane), vf[ks], dp);
-            }
+            struct Frags { bf16x8_t q, d, k; };
+            Frags f[AK], g[AK];
+            auto load = [&](int j) { return Frags{by_rows(Ql, 32 * qb, j, lane), by_rows(DOl, 32 * qb, j, lane), by_rows(Kl, 32 * (wid & 1), j, lane)}; };
+            auto load_t = [&](int j) {
+                return Frags{by_cols(Ql, 32 * (j % NDB), 32 * qb + 16 * (j / NDB), lane), by_cols(DOl, 32 * (j % NDB), 32 * qb + 16 * (j / NDB), lane), {}};
+            };
+            ahead_start(f, load);
+            ahead_run<NKS>(f, load, [&](int j, const Frags& x) { s = mfma16(x.q, x.k, s); dp = mfma16(x.d, vf[j], dp); });
+            ahead_start(g, load_t);
             if (p.causal && q0 + ahead < k0w + 31) {           // some query of the block does not see every key of this wave
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = key <= q0 + 8 * (e >> 2) + 4 * h + (e & 3) + ahead ? s[e] : -INFINITY;
@@ -496,32 +557,26 @@ __global__ void __launch_bounds__(NT, 2) varlen_dkv_kernel(const VarlenParams p)
                 }
             }
             const bf16x8_t pf[2] = {pack_frag(pr, 0), pack_frag(pr, 8)}, ds[2] = {pack_frag(s, 0), pack_frag(s, 8)};
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int db = 0; db < NDB; ++db) {
-                    dv[db] = mfma16(by_cols(DOl, 32 * db, 32 * qb + 16 * u, lane), pf[u], dv[db]);
-                    dk[db] = mfma16(by_cols(Ql, 32 * db, 32 * qb + 16 * u, lane), ds[u], dk[db]);
-                }
+            __builtin_amdgcn_sched_barrier(0);
+            ahead_run<2 * NDB>(g, load_t, [&](int j, const Frags& x) { dv[j % NDB] = mfma16(x.d, pf[j / NDB], dv[j % NDB]); dk[j % NDB] = mfma16(x.q, ds[j / NDB], dk[j % NDB]); });
         }
     }
     if (!live) return;
     const long row = ((t.k0 + key) * p.hk + w.head) * D, slice = p.tk * p.hk * D;
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
+    for (int db = 0; db < NDB; ++db) {
+        if (p.nsplit == 1) {
+            store_row(p.dk + row + 32 * db, nullptr, dk[db], p.scale, h);
+            store_row(p.dv + row + 32 * db, nullptr, dv[db], 1.f, h);
+            continue;
+        }
 #pragma unroll
         for (int eg = 0; eg < 4; ++eg) {
             const long at = row + 32 * db + 8 * eg + 4 * h;
-            const float4 a = make_float4(dk[db][4 * eg] * p.scale, dk[db][4 * eg + 1] * p.scale, dk[db][4 * eg + 2] * p.scale, dk[db][4 * eg + 3] * p.scale);
-            const float4 c = make_float4(dv[db][4 * eg], dv[db][4 * eg + 1], dv[db][4 * eg + 2], dv[db][4 * eg + 3]);
-            if (p.nsplit > 1) {
-                *reinterpret_cast<float4*>(p.part + 2 * w.part * slice + at) = a;
-                *reinterpret_cast<float4*>(p.part + (2 * w.part + 1) * slice + at) = c;
-            } else {
-                *reinterpret_cast<uint2*>(p.dk + at) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
-                *reinterpret_cast<uint2*>(p.dv + at) = make_uint2(pack_bf16x2(c.x, c.y), pack_bf16x2(c.z, c.w));
-            }
+            *reinterpret_cast<float4*>(p.part + 2 * w.part * slice + at) = make_float4(dk[db][4 * eg] * p.scale, dk[db][4 * eg + 1] * p.scale, dk[db][4 * eg + 2] * p.scale, dk[db][4 * eg + 3] * p.scale);
+            *reinterpret_cast<float4*>(p.part + (2 * w.part + 1) * slice + at) = make_float4(dv[db][4 * eg], dv[db][4 * eg + 1], dv[db][4 * eg + 2], dv[db][4 * eg + 3]);
         }
+    }
 }
 
 // dK / dV = sum of the parts in order, one thread per 4 channels
@@ -587,7 +642,8 @@ template <int D> void forward(const VarlenParams& p, hipStream_t s) {
 template <int D> void backward(VarlenParams& p, int parts, hipStream_t s) {
     varlen_dq_kernel<D><<<(unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, 1), NT, 0, s>>>(p);
     p.nsplit = parts;
-    varlen_dkv_kernel<D><<<(unsigned)work_groups(row_slots(p.tk, 1, p.n, ROWS), p.hk, parts), NT, 0, s>>>(p);
+    constexpr int NW = D == 128 ? 8 : 4;
+    varlen_dkv_kernel<D, NW><<<(unsigned)work_groups(row_slots(p.tk, 1, p.n, 32 * NW), p.hk, parts), 64 * NW, 0, s>>>(p);
     if (parts > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
 }
 
@@ -606,32 +662,32 @@ long dpipe_attn_varlen_bwd_workspace_floats(long tq, long tk, int n, int hq, int
     return s > 1 ? 2l * s * tk * hk * D : 0;
 }
 
-int dpipe_attn_varlen_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, float* lse, float* o_f32, float* ws, long ws_floats, long tq,
+int dpipe_attn_varlen_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, void* o_lo, float* lse, float* ws, long ws_floats, long tq,
                           long tk, int n, int hq, int hk, int D, long q_ss, long q_sh, long k_ss, long k_sh, long v_ss, long v_sh, float scale, int causal, void* stream) {
     VarlenParams p = {};
     const int rc = fill(p, "dpipe_attn_varlen_fwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal);
     if (rc) return rc;
     const long need = dpipe_attn_varlen_fwd_workspace_floats(tq, tk, n, hq, hk, D);
-    if (!o || !aligned16(o) || !aligned16(o_f32) || (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) {
+    if (!o || !aligned16(o) || !aligned16(o_lo) || (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) {
         set_last_error("dpipe_attn_varlen_fwd: bad output or workspace"); return DPIPE_ERR_ARG; }
     if (ablated(ABL_ATTN)) return DPIPE_OK;
-    p.o = (bf16_t*)o; p.lse = lse; p.o32 = o_f32;
+    p.o = (bf16_t*)o; p.o_lo = (bf16_t*)o_lo; p.lse = lse;
     if (need > 0) { p.nsplit = fwd_splits(tq, tk, n, hq, hk); p.part = ws; p.part_lse = ws + (long)p.nsplit * tq * hq * D; }
     if (D == 64) forward<64>(p, reinterpret_cast<hipStream_t>(stream)); else forward<128>(p, reinterpret_cast<hipStream_t>(stream));
     return check_launch("dpipe_attn_varlen_fwd");
 }
 
-int dpipe_attn_varlen_bwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, const float* o_f32, const void* dout, const float* lse, float* delta,
+int dpipe_attn_varlen_bwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, const void* o, const void* o_lo, const void* dout, const float* lse, float* delta,
                           void* dq, void* dk, void* dv, float* ws, long ws_floats, long tq, long tk, int n, int hq, int hk, int D, long q_ss, long q_sh, long k_ss, long k_sh,
                           long v_ss, long v_sh, long do_ss, long do_sh, float scale, int causal, void* stream) {
     VarlenParams p = {};
     const int rc = fill(p, "dpipe_attn_varlen_bwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal);
     if (rc) return rc;
     const long need = dpipe_attn_varlen_bwd_workspace_floats(tq, tk, n, hq, hk, D);
-    if (!o_f32 || !dout || !lse || !delta || !dq || !dk || !dv || !aligned16(o_f32) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !rows_ok(dout, do_ss, do_sh, D) ||
+    if (!o || !o_lo || !dout || !lse || !delta || !dq || !dk || !dv || !aligned16(o) || !aligned16(o_lo) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !rows_ok(dout, do_ss, do_sh, D) ||
         (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) { set_last_error("dpipe_attn_varlen_bwd: bad gradient or workspace"); return DPIPE_ERR_ARG; }
     if (ablated(ABL_ATTN)) return DPIPE_OK;
-    p.o32 = const_cast<float*>(o_f32); p.dout = (const bf16_t*)dout; p.lse = const_cast<float*>(lse); p.delta = delta;
+    p.o = (bf16_t*)o; p.o_lo = (bf16_t*)o_lo; p.dout = (const bf16_t*)dout; p.lse = const_cast<float*>(lse); p.delta = delta;
     p.dq = (bf16_t*)dq; p.dk = (bf16_t*)dk; p.dv = (bf16_t*)dv; p.do_ss = do_ss; p.do_sh = do_sh; p.part = ws;
     const int splits = need > 0 ? dkv_splits(tq, tk, n, hq, hk) : 1;
     if (D == 64) backward<64>(p, splits, reinterpret_cast<hipStream_t>(stream)); else backward<128>(p, splits, reinterpret_cast<hipStream_t>(stream));

@@ -1771,7 +1771,7 @@ def attention(q, k, v, kv_len=None, scale=None, impl='auto', causal=False):
 
 
 def _varlen_forward(q, k, v, cu_q, cu_k, scale, causal, keep):
-    """-> (o, what the backward reads, what its call repeats); keep: the unrounded output and the row statistics are stored for the backward's delta and P"""
+    """-> (o, what the backward reads, what its call repeats); keep: the row statistics and what the output's rounding left are stored for the backward's P and delta"""
     device = q.device
     (q, tq, hq, D, *qs), (k, tk, hk, _, *ks), (v, _, _, _, *vs) = _head_rows(q), _head_rows(k), _head_rows(v)
     if tq == 0 or tk == 0:                        # nothing to read: every row is empty
@@ -1779,16 +1779,16 @@ def _varlen_forward(q, k, v, cu_q, cu_k, scale, causal, keep):
     sizes, strides = (tq, tk, cu_q.shape[0] - 1, hq, hk, D), (*qs, *ks, *vs)
     o = torch.empty((tq, hq, D), device=device, dtype=q.dtype)
     lse = torch.empty((hq, tq), device=device, dtype=torch.float32) if keep else None
-    o32 = torch.empty((tq, hq, D), device=device, dtype=torch.float32) if keep else None
+    o_lo = torch.empty((tq, hq, D), device=device, dtype=q.dtype) if keep else None
     need = lib().dpipe_attn_varlen_fwd_workspace_floats(*sizes)
     ws = torch.empty(need, device=device, dtype=torch.float32) if need else None
-    check(lib().dpipe_attn_varlen_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _addr(lse), _addr(o32), _addr(ws), need, *sizes,
+    check(lib().dpipe_attn_varlen_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _addr(o_lo), _addr(lse), _addr(ws), need, *sizes,
                                       *strides, scale, causal, hip.raw_stream(device)), 'attn_varlen_fwd')
-    return o, (q, k, v, cu_q, cu_k, o32, lse), (sizes, strides, scale, causal)
+    return o, (q, k, v, cu_q, cu_k, o, o_lo, lse), (sizes, strides, scale, causal)
 
 
 class _AttnVarlenFn(Function):
-    """see attention_varlen; keeps the unrounded output for the backward's delta, as _FlashAttnFn does"""
+    """see attention_varlen; keeps the output to 16 bits of significand (o and what its rounding left) for the backward's delta, where _FlashAttnFn keeps an fp32 copy"""
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale, causal):
@@ -1803,7 +1803,7 @@ class _AttnVarlenFn(Function):
         if ctx.call is None:
             *shapes, dtype = ctx.shapes
             return (*(torch.zeros(sh, device=device, dtype=dtype) for sh in shapes), None, None, None, None)
-        q, k, v, cu_q, cu_k, o32, lse = ctx.saved_tensors
+        q, k, v, cu_q, cu_k, o, o_lo, lse = ctx.saved_tensors
         sizes, strides, scale, causal = ctx.call
         with _on(device):
             do, _, _, _, *ds = _head_rows(do)
@@ -1811,7 +1811,7 @@ class _AttnVarlenFn(Function):
             delta = torch.empty_like(lse)
             need = lib().dpipe_attn_varlen_bwd_workspace_floats(*sizes)
             ws = torch.empty(need, device=device, dtype=torch.float32) if need else None
-            check(lib().dpipe_attn_varlen_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o32.data_ptr(), do.data_ptr(), lse.data_ptr(),
+            check(lib().dpipe_attn_varlen_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), o_lo.data_ptr(), do.data_ptr(), lse.data_ptr(),
                                               delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _addr(ws), need, *sizes, *strides, *ds, scale, causal,
                                               hip.raw_stream(device)), 'attn_varlen_bwd')
         return dq, dk, dv, None, None, None, None

@@ -104,9 +104,9 @@ def _varlen_c(name='fwd', **kw):
     from diffusion_pipe_amd import hip
     a = dict(q=256, k=256, v=256, cu_q=256, cu_k=256)
     if name == 'fwd':
-        a.update(o=256, lse=256, o32=256)
+        a.update(o=256, o_lo=256, lse=256)
     else:
-        a.update(o32=256, do=256, lse=256, delta=256, dq=256, dk=256, dv=256)
+        a.update(o=256, o_lo=256, do=256, lse=256, delta=256, dq=256, dk=256, dv=256)
     a.update(ws=None, floats=0, tq=6, tk=6, n=1, hq=2, hk=1, D=64, q_ss=128, q_sh=64, k_ss=64, k_sh=64, v_ss=64, v_sh=64)
     if name == 'bwd':
         a.update(do_ss=128, do_sh=64)
