@@ -22,8 +22,9 @@ namespace {
 
 constexpr int NB = 256;
 constexpr int MAX_PAIRS = 128;           // head dim <= 256
-constexpr int TABLE = 256;               // (cos, sin) pairs in LDS: TB * pairs <= TABLE
-constexpr int MAX_BWD_BLOCKS = 1024;     // partial rows of the weight gradient: 4 workgroups per CU
+constexpr int TABLE = 256;               // (cos, sin) pairs in LDS: tokens of a tile * pairs (rounded up to 4) <= TABLE
+constexpr int AHEAD = 4;                 // rows of a lane group that are in flight
+constexpr int MAX_BWD_BLOCKS = 512;      // partial rows of a weight's gradient: with both tensors 4 workgroups per CU
 
 struct RopeAxesParams {
     const void *x[2], *gy[2], *w[2];     // [0] query, [1] key
@@ -34,7 +35,8 @@ struct RopeAxesParams {
     long tokens, period;                 // positions repeat every `period` tokens
     int heads[2];
     int D, pairs, axes, tb, pos_type, w_f32[2];
-    unsigned magic[2];                   // ceil(2^32 / heads): row / heads for rows < 2^16
+    unsigned pair_magic;                 // ceil(2^32 / pairs): entry / pairs of a table by multiplication
+    int step_t[2], step_h[2];            // lane groups per workgroup = step_t heads + step_h: a lane group's next row is step_t tokens and step_h heads further
     float eps, sign;                     // sign = -1: the inverse rotation
     double freq[MAX_PAIRS];
     unsigned char axis[MAX_PAIRS];
@@ -84,39 +86,47 @@ template <typename T, bool HALF> struct Raw8 {
     }
 };
 
+// sum over groups of LPR lanes, in every lane: exchanges inside 16 lanes are operand modifiers of the add (no LDS)
+template <int CTRL> __device__ __forceinline__ float add_dpp(float v) { return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
 template <int LPR> __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    v = add_dpp<0xb1>(v);                                    // lane ^ 1
+    v = add_dpp<0x4e>(v);                                    // lane ^ 2
+    v = add_dpp<0x141>(v);                                   // mirrored in 8: the other four
+    if (LPR > 8) v = add_dpp<0x140>(v);                      // mirrored in 16: the other eight
+    if (LPR > 16) v += __shfl_xor(v, 16, 64);
     return v;
 }
 
 __device__ __forceinline__ double position(const RopeAxesParams& p, long token, int axis) {
-    const long i = (token % p.period) * p.axes + axis;
+    const long i = (token < p.period ? token : token % p.period) * p.axes + axis;
     if (p.pos_type == 2) return (double)reinterpret_cast<const long long*>(p.pos)[i];
     if (p.pos_type == 1) return (double)reinterpret_cast<const int*>(p.pos)[i];
     return (double)reinterpret_cast<const float*>(p.pos)[i];
 }
 
-// (cos, sin) of the tile's tokens into LDS; `sign` turns the rotation round
-__device__ __forceinline__ void fill_table(const RopeAxesParams& p, float2* table, long t0, int ntok) {
+// (cos, sin) of the tile's tokens into LDS, `pitch` entries a token; `sign` turns the rotation round
+__device__ __forceinline__ int table_pitch(int pairs) { return (pairs + 3) & ~3; }
+__device__ __forceinline__ void fill_table(const RopeAxesParams& p, float* table, long t0, int ntok) {
     for (int e = threadIdx.x; e < ntok * p.pairs; e += NB) {
-        const int t = e / p.pairs, pr = e - t * p.pairs;
+        const int t = p.pairs == 1 ? e : (int)__umulhi((unsigned)e, p.pair_magic), pr = e - t * p.pairs;
         double turns = position(p, t0 + t, p.axis[pr]) * p.freq[pr];
         turns -= rint(turns);
         float s, c;
         sincospif(2.f * (float)turns, &s, &c);
-        table[e] = make_float2(c, p.sign * s);
+        table[t * table_pitch(p.pairs) + pr] = c;
+        table[TABLE + t * table_pitch(p.pairs) + pr] = p.sign * s;
     }
 }
 
-// pair j of the lane: f[.] rotated in place where `rot`; PAIR j = channels (2 j, 2 j + 1) of the lane's 8, or (j, 4 + j) with halves pairing
-template <bool HALF> __device__ __forceinline__ void rotate(float* f, const float2* cs, int p0, int pairs) {
+// the lane's four pairs, from p0 on, of one token: channels (2 j, 2 j + 1) of its 8, or (j, 4 + j) with halves pairing.  Pairs behind the rotated ones keep their bits.
+template <bool HALF> __device__ __forceinline__ void rotate(float* f, const float* table, int p0, int pairs, bool full) {
+    const float4 vc = *reinterpret_cast<const float4*>(table + p0), vs = *reinterpret_cast<const float4*>(table + TABLE + p0);
+    const float c[4] = {vc.x, vc.y, vc.z, vc.w}, s[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int a = HALF ? j : 2 * j, b = HALF ? 4 + j : 2 * j + 1;
-        const bool rot = p0 + j < pairs;
-        const float2 t = cs[rot ? p0 + j : 0];
-        const float y0 = f[a] * t.x - f[b] * t.y, y1 = f[b] * t.x + f[a] * t.y;
+        const float y0 = f[a] * c[j] - f[b] * s[j], y1 = f[b] * c[j] + f[a] * s[j];
+        const bool rot = full || p0 + j < pairs;
         f[a] = rot ? y0 : f[a]; f[b] = rot ? y1 : f[b];
     }
 }
@@ -131,177 +141,218 @@ __device__ __forceinline__ void load_weight(const RopeAxesParams& p, int which, 
     else { load4(reinterpret_cast<const bf16_t*>(p.w[which]) + c0, w); load4(reinterpret_cast<const bf16_t*>(p.w[which]) + c1, w + 4); }
 }
 
-// y = R(sign * theta) [norm](x): the forward, and the backward of rows without a norm (sign = -1)
+// A lane group's walk over the head rows of a tile (row = token * heads + head, one row every GROUPS): offsets inside the tile fit 32 bits (the launcher sees to it)
+struct Walk {
+    int token, head;
+    __device__ __forceinline__ void start(int grp, int heads) { token = grp / heads; head = grp - token * heads; }
+    __device__ __forceinline__ void next(int step_t, int step_h, int heads) {
+        token += step_t; head += step_h;
+        const bool over = head >= heads;
+        token += over ? 1 : 0; head -= over ? heads : 0;
+    }
+    __device__ __forceinline__ unsigned offset(int ss, int sh) const { return (unsigned)(token * ss + head * sh); }
+};
+
+// What a lane keeps of its place in the workgroup
+template <bool HALF, int LPR> struct Lane {
+    int sub, grp, c0 = 0, c1 = 4, p0;
+    bool in, full;
+    __device__ __forceinline__ Lane(const RopeAxesParams& p) {
+        sub = threadIdx.x % LPR; grp = threadIdx.x / LPR;
+        in = 8 * sub < p.D; full = 2 * p.pairs == p.D;
+        if (in) lane_channels<HALF>(p, sub, c0, c1);
+        p0 = 4 * sub < p.pairs ? 4 * sub : 0;                // (lanes behind the rotated channels read the table somewhere and keep their values)
+    }
+};
+
+// The rows of one tensor of a tile: y = R [norm](x)
 template <typename T, int LPR, bool HALF, bool NORM>
-__global__ void __launch_bounds__(NB) rope_axes_kernel(const RopeAxesParams p) {
-    constexpr int GROUPS = NB / LPR, U = 4;                   // U rows of a lane group in flight
-    __shared__ float2 table[TABLE];
-    const int sub = threadIdx.x % LPR, grp = threadIdx.x / LPR;
-    const long t0 = (long)blockIdx.x * p.tb;
-    const int ntok = (int)min((long)p.tb, p.tokens - t0);
-    fill_table(p, table, t0, ntok);
-    __syncthreads();
-    const bool in = 8 * sub < p.D;
-    int c0 = 0, c1 = 4;
-    if (in) lane_channels<HALF>(p, sub, c0, c1);
+__device__ __forceinline__ void rows_forward(const RopeAxesParams& p, const Lane<HALF, LPR>& ln, const float* table, int which, long t0, int ntok, Raw8<T, HALF>* raw, bool loaded) {
+    constexpr int GROUPS = NB / LPR;
+    const int heads = p.heads[which], rows = ntok * heads, iters = (rows + GROUPS - 1) / GROUPS, pitch = table_pitch(p.pairs);
+    const int ss = (int)p.x_ss[which], sh = (int)p.x_sh[which], st = p.step_t[which], sd = p.step_h[which];
+    const T* x = reinterpret_cast<const T*>(p.x[which]) + t0 * p.x_ss[which];
+    T* y = reinterpret_cast<T*>(p.y[which]) + t0 * heads * (long)p.D;
     const float inv_d = 1.f / (float)p.D;
+    float w[8];
+    if (NORM) load_weight(p, which, ln.c0, ln.c1, w);
+    Walk get, put;
+    get.start(ln.grp, heads); put.start(ln.grp, heads);
+    auto fetch = [&](Raw8<T, HALF>& r) {
+        if (get.token < ntok) r.load(x + get.offset(ss, sh), ln.c0, ln.c1);
+        get.next(st, sd, heads);
+    };
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        const int heads = p.heads[which];
-        const bool norm = NORM && p.w[which] != nullptr;
-        float w[8];
-        if (norm) load_weight(p, which, c0, c1, w);
-        const T* x = reinterpret_cast<const T*>(p.x[which]) + t0 * p.x_ss[which];
-        T* y = reinterpret_cast<T*>(p.y[which]) + t0 * heads * (long)p.D;
-        const int rows = ntok * heads;
-        for (int r0 = grp; r0 < rows; r0 += GROUPS * U) {
-            Raw8<T, HALF> raw[U];
-            int tl[U];
+    for (int u = 0; u < AHEAD; ++u) fetch(raw[u]);
+    if (!loaded) __syncthreads();                            // the table is complete
+    for (int i = 0; i < iters; i += AHEAD) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int r = min(r0 + u * GROUPS, rows - 1);
-                tl[u] = heads == 1 ? r : (int)__umulhi((unsigned)r, p.magic[which]);
-                raw[u].load(x + tl[u] * p.x_ss[which] + (r - tl[u] * heads) * p.x_sh[which], c0, c1);
+        for (int u = 0; u < AHEAD; ++u) {
+            if (i + u >= iters) break;                       // (uniform)
+            float f[8];
+            raw[u].unpack(f);
+            fetch(raw[u]);
+            if (NORM) {
+                float sq = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sq += f[j] * f[j];
+                const float rstd = rsqrtf(group_sum<LPR>(ln.in ? sq : 0.f) * inv_d + p.eps);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = f[j] * rstd * w[j];
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int r = r0 + u * GROUPS;
-                float f[8];
-                raw[u].unpack(f);
-                if (norm) {
-                    float ss = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
-                    const float rstd = rsqrtf(group_sum<LPR>(in ? ss : 0.f) * inv_d + p.eps);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = f[j] * rstd * w[j];
-                }
-                rotate<HALF>(f, table + tl[u] * p.pairs, 4 * sub, p.pairs);
-                raw[u].pack(f);
-                if (in && r < rows) raw[u].store(y + (long)r * p.D, c0, c1);
-            }
+            const bool live = ln.in && put.token < ntok;
+            rotate<HALF>(f, table + (put.token < ntok ? put.token * pitch : 0), ln.p0, ln.in && 4 * ln.sub < p.pairs ? p.pairs : 0, ln.full);
+            Raw8<T, HALF> out;
+            out.pack(f);
+            if (live) out.store(y + (unsigned)((put.token * heads + put.head) * p.D), ln.c0, ln.c1);
+            put.next(st, sd, heads);
         }
     }
 }
 
-// the backward with norms: dx, and per workgroup one partial row of either weight's gradient (summed in a fixed order by rope_axes_dw_kernel)
+// y = R(sign * theta) [norm](x): the forward, and the backward of rows without a norm (sign = -1)
 template <typename T, int LPR, bool HALF>
-__global__ void __launch_bounds__(NB) rope_axes_bwd_kernel(const RopeAxesParams p) {
-    constexpr int GROUPS = NB / LPR, U = 2;
-    __shared__ float2 table[TABLE];
-    __shared__ float red[GROUPS][LPR * 8];
-    const int sub = threadIdx.x % LPR, grp = threadIdx.x / LPR;
-    const bool in = 8 * sub < p.D;
-    int c0 = 0, c1 = 4;
-    if (in) lane_channels<HALF>(p, sub, c0, c1);
+__global__ void __launch_bounds__(NB) rope_axes_kernel(const RopeAxesParams p) {
+    __shared__ __attribute__((aligned(16))) float table[2 * TABLE];     // cosines, then sines
+    const Lane<HALF, LPR> ln(p);
+    const long t0 = (long)blockIdx.x * p.tb;
+    const int ntok = (int)min((long)p.tb, p.tokens - t0);
+    fill_table(p, table, t0, ntok);
+    Raw8<T, HALF> raw[AHEAD];
+    if (p.w[0]) rows_forward<T, LPR, HALF, true>(p, ln, table, 0, t0, ntok, raw, false); else rows_forward<T, LPR, HALF, false>(p, ln, table, 0, t0, ntok, raw, false);
+    if (p.heads[1] == 0) return;
+    if (p.w[1]) rows_forward<T, LPR, HALF, true>(p, ln, table, 1, t0, ntok, raw, true); else rows_forward<T, LPR, HALF, false>(p, ln, table, 1, t0, ntok, raw, true);
+}
+
+// The backward of one tensor's rows of a tile: dx, and the weight's gradient added to the lane's dw
+template <typename T, int LPR, bool HALF, bool NORM>
+__device__ __forceinline__ void rows_backward(const RopeAxesParams& p, const Lane<HALF, LPR>& ln, const float* table, int which, long t0, int ntok, const float* w, float* dw) {
+    constexpr int GROUPS = NB / LPR, A = 2;
+    const int heads = p.heads[which], rows = ntok * heads, iters = (rows + GROUPS - 1) / GROUPS, pitch = table_pitch(p.pairs);
+    const int ss = (int)p.x_ss[which], sh = (int)p.x_sh[which], gs = (int)p.g_ss[which], gh = (int)p.g_sh[which], st = p.step_t[which], sd = p.step_h[which];
+    const T* x = reinterpret_cast<const T*>(p.x[which]) + t0 * p.x_ss[which];
+    const T* gy = reinterpret_cast<const T*>(p.gy[which]) + t0 * p.g_ss[which];
+    T* dx = reinterpret_cast<T*>(p.y[which]) + t0 * heads * (long)p.D;
     const float inv_d = 1.f / (float)p.D;
-    float w[2][8], dw[2][8];
+    Raw8<T, HALF> rx[A], rg[A];
+    Walk get, put;
+    get.start(ln.grp, heads); put.start(ln.grp, heads);
+    auto fetch = [&](int u) {
+        if (get.token < ntok) {
+            if (NORM) rx[u].load(x + get.offset(ss, sh), ln.c0, ln.c1);
+            rg[u].load(gy + get.offset(gs, gh), ln.c0, ln.c1);
+        }
+        get.next(st, sd, heads);
+    };
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
+    for (int u = 0; u < A; ++u) fetch(u);
+    __syncthreads();                                         // the table is complete
+    for (int i = 0; i < iters; i += A) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { w[which][j] = 1.f; dw[which][j] = 0.f; }
-        if (p.w[which]) load_weight(p, which, c0, c1, w[which]);
+        for (int u = 0; u < A; ++u) {
+            if (i + u >= iters) break;
+            float f[8], g[8];
+            rg[u].unpack(g);
+            if (NORM) rx[u].unpack(f);
+            fetch(u);
+            const bool live = ln.in && put.token < ntok;
+            rotate<HALF>(g, table + (put.token < ntok ? put.token * pitch : 0), ln.p0, ln.in && 4 * ln.sub < p.pairs ? p.pairs : 0, ln.full);
+            if (NORM) {
+                float sq = 0.f, dot = 0.f;                   // sum x^2 and sum u x:  mean(u xhat) = r * dot / D
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { sq += f[j] * f[j]; dot += g[j] * w[j] * f[j]; }
+                sq = group_sum<LPR>(ln.in ? sq : 0.f); dot = group_sum<LPR>(ln.in ? dot : 0.f);
+                const float rstd = rsqrtf(sq * inv_d + p.eps), m = rstd * dot * inv_d;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float xh = f[j] * rstd;
+                    dw[j] += live ? g[j] * xh : 0.f;
+                    g[j] = rstd * (g[j] * w[j] - xh * m);
+                }
+            }
+            Raw8<T, HALF> out;
+            out.pack(g);
+            if (live) out.store(dx + (unsigned)((put.token * heads + put.head) * p.D), ln.c0, ln.c1);
+            put.next(st, sd, heads);
+        }
     }
+}
+
+// the backward with norms: dx, and per workgroup one partial row of the weight's gradient (summed in a fixed order by rope_axes_dw_kernel).  A workgroup takes the tiles of one
+// tensor (blockIdx.y): with both, the weights and their gradients of both sit in registers and 4 waves a SIMD spill.
+template <typename T, int LPR, bool HALF>
+__global__ void __launch_bounds__(NB, 4) rope_axes_bwd_kernel(const RopeAxesParams p) {
+    constexpr int GROUPS = NB / LPR;
+    __shared__ __attribute__((aligned(16))) float table[2 * TABLE];     // cosines, then sines
+    __shared__ float red[GROUPS][LPR * 8];
+    const Lane<HALF, LPR> ln(p);
+    const int which = blockIdx.y;
+    const bool norm = p.w[which] != nullptr;
+    float w[8], dw[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { w[j] = 1.f; dw[j] = 0.f; }
+    if (norm) load_weight(p, which, ln.c0, ln.c1, w);
     for (long t0 = (long)blockIdx.x * p.tb; t0 < p.tokens; t0 += (long)gridDim.x * p.tb) {
         const int ntok = (int)min((long)p.tb, p.tokens - t0);
         __syncthreads();                                       // the previous tile's rows are done with the table
         fill_table(p, table, t0, ntok);
-        __syncthreads();
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const int heads = p.heads[which];
-            const bool norm = p.w[which] != nullptr;
-            const T* x = reinterpret_cast<const T*>(p.x[which]) + t0 * p.x_ss[which];
-            const T* gy = reinterpret_cast<const T*>(p.gy[which]) + t0 * p.g_ss[which];
-            T* dx = reinterpret_cast<T*>(p.y[which]) + t0 * heads * (long)p.D;
-            const int rows = ntok * heads;
-            for (int r0 = grp; r0 < rows; r0 += GROUPS * U) {
-                Raw8<T, HALF> rx[U], rg[U];
-                int tl[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int r = min(r0 + u * GROUPS, rows - 1);
-                    tl[u] = heads == 1 ? r : (int)__umulhi((unsigned)r, p.magic[which]);
-                    const int hd = r - tl[u] * heads;
-                    if (norm) rx[u].load(x + tl[u] * p.x_ss[which] + hd * p.x_sh[which], c0, c1);
-                    rg[u].load(gy + tl[u] * p.g_ss[which] + hd * p.g_sh[which], c0, c1);
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int r = r0 + u * GROUPS;
-                    const bool live = in && r < rows;
-                    float f[8], g[8];
-                    rg[u].unpack(g);
-                    rotate<HALF>(g, table + tl[u] * p.pairs, 4 * sub, p.pairs);
-                    if (norm) {
-                        rx[u].unpack(f);
-                        float ss = 0.f, dot = 0.f;             // sum x^2 and sum u x:  mean(u xhat) = r * dot / D
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) { ss += f[j] * f[j]; dot += g[j] * w[which][j] * f[j]; }
-                        ss = group_sum<LPR>(in ? ss : 0.f); dot = group_sum<LPR>(in ? dot : 0.f);
-                        const float rstd = rsqrtf(ss * inv_d + p.eps), m = rstd * dot * inv_d;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float xh = f[j] * rstd;
-                            dw[which][j] += live ? g[j] * xh : 0.f;
-                            g[j] = rstd * (g[j] * w[which][j] - xh * m);
-                        }
-                    }
-                    rg[u].pack(g);
-                    if (live) rg[u].store(dx + (long)r * p.D, c0, c1);
-                }
-            }
-        }
+        if (norm) rows_backward<T, LPR, HALF, true>(p, ln, table, which, t0, ntok, w, dw);
+        else rows_backward<T, LPR, HALF, false>(p, ln, table, which, t0, ntok, w, dw);
     }
+    __syncthreads();
+    if (ln.in) {
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        __syncthreads();
-        if (in) {
+        for (int j = 0; j < 4; ++j) { red[ln.grp][ln.c0 + j] = dw[j]; red[ln.grp][ln.c1 + j] = dw[4 + j]; }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < p.D) {
+        float s = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { red[grp][c0 + j] = dw[which][j]; red[grp][c1 + j] = dw[which][4 + j]; }
-        }
-        __syncthreads();
-        if ((int)threadIdx.x < p.D) {
-            float s = 0.f;
-            for (int g = 0; g < GROUPS; ++g) s += red[g][threadIdx.x];
-            p.part[((long)blockIdx.x * 2 + which) * p.D + threadIdx.x] = s;
-        }
+        for (int g = 0; g < GROUPS; ++g) s += red[g][threadIdx.x];
+        p.part[((long)blockIdx.x * 2 + which) * p.D + threadIdx.x] = s;
     }
 }
 
-// dw[c] (+)= sum over `blocks` partial rows, in a fixed order: 32 columns x 8 slices of rows per workgroup
+// dw[c] (+)= sum over `blocks` partial rows, in a fixed order: 32 columns (8 lanes of 4) x 32 slices of the rows per workgroup
 __global__ void __launch_bounds__(NB) rope_axes_dw_kernel(const float* __restrict__ part, void* dq, void* dk, int q_f32, int k_f32, int accumulate_q, int accumulate_k,
                                                           int blocks, int D) {
-    __shared__ float red[8][32];
-    const int ct = threadIdx.x & 31, sl = threadIdx.x >> 5, c = blockIdx.x * 32 + ct, which = blockIdx.y;
-    float a = 0.f;
+    __shared__ __attribute__((aligned(16))) float red[32][32];
+    const int ct = 4 * (threadIdx.x & 7), sl = threadIdx.x >> 3, which = blockIdx.y, c = blockIdx.x * 32 + ct;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     if (c < D) {
 #pragma unroll 16
-        for (int s = sl; s < blocks; s += 8) a += part[((long)s * 2 + which) * D + c];
+        for (int s = sl; s < blocks; s += 32) {
+            const float4 v = *reinterpret_cast<const float4*>(part + ((long)s * 2 + which) * D + c);
+            a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+        }
     }
-    red[sl][ct] = a;
+    *reinterpret_cast<float4*>(&red[sl][ct]) = a;
     __syncthreads();
     void* out = which ? dk : dq;
-    if (threadIdx.x < 32 && c < D && out) {
+    const int col = blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x < 32 && col < D && out) {
         float s = 0.f;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) s += red[r][ct];
+        for (int r = 0; r < 32; ++r) s += red[r][threadIdx.x];
         const bool f32 = which ? k_f32 : q_f32, acc = which ? accumulate_k : accumulate_q;
-        if (f32) { float* o = reinterpret_cast<float*>(out) + c; *o = acc ? *o + s : s; }
-        else { bf16_t* o = reinterpret_cast<bf16_t*>(out) + c; *o = f32_to_bf16(acc ? bf16_to_f32(*o) + s : s); }
+        if (f32) { float* o = reinterpret_cast<float*>(out) + col; *o = acc ? *o + s : s; }
+        else { bf16_t* o = reinterpret_cast<bf16_t*>(out) + col; *o = f32_to_bf16(acc ? bf16_to_f32(*o) + s : s); }
     }
 }
 
 // tokens per workgroup: as many as the table holds, while 1 024 workgroups (4 per CU) are left
-int tile_tokens(long tokens, int pairs, int D, int heads) {
-    int tb = pairs > 0 ? TABLE / pairs : 8;
+int tile_tokens(long tokens, int pairs) {
+    int tb = TABLE / ((pairs + 3) & ~3);
     if (tb > 8) tb = 8;
     while (tb > 1 && (tokens + tb - 1) / tb < 1024) --tb;
-    while (tb > 1 && (long)tb * heads > 65535) --tb;          // row / heads by multiplication
     return tb;
 }
 
+// 8 tokens and all heads stay within 2^29 elements of the tile's first (32-bit byte offsets)
+bool rows_fit(long ss, long sh, int heads) { return ss >= 0 && sh >= 0 && ss < (1l << 25) && sh * heads < (1l << 28); }
 bool rows_ok(const void* p, long ss, long sh) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ss % 8 == 0 && sh % 8 == 0; }
+
+int lanes_per_row(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
 // checks shared by both entry points; fills everything but the gradient operands
 int fill(RopeAxesParams& p, const char* what, const void* q, const void* k, const void* pos, int pos_type, const double* freq, const int* axis, long tokens, long period,
@@ -316,32 +367,33 @@ int fill(RopeAxesParams& p, const char* what, const void* q, const void* k, cons
     if (pos_type < 0 || pos_type > 2) return bad("positions must be fp32, int32 or int64");
     if (!rows_ok(q, q_ss, q_sh) || (heads_k > 0 && !rows_ok(k, k_ss, k_sh)) || (reinterpret_cast<uintptr_t>(wq) & 15) || (reinterpret_cast<uintptr_t>(wk) & 15))
         return bad("tensors must be 16-byte aligned with strides multiple of 8 elements");
+    if (!rows_fit(q_ss, q_sh, heads_q) || (heads_k > 0 && !rows_fit(k_ss, k_sh, heads_k))) return bad("strides too large");
     if ((wq && wq_dt != DPIPE_BF16 && wq_dt != DPIPE_F32) || (wk && wk_dt != DPIPE_BF16 && wk_dt != DPIPE_F32)) return bad("weights must be bf16 or fp32");
     p.x[0] = q; p.x[1] = k; p.x_ss[0] = q_ss; p.x_sh[0] = q_sh; p.x_ss[1] = k_ss; p.x_sh[1] = k_sh;
     p.pos = pos; p.pos_type = pos_type; p.tokens = tokens; p.period = period; p.axes = axes; p.pairs = pairs; p.D = D;
     p.heads[0] = heads_q; p.heads[1] = heads_k; p.w[0] = wq; p.w[1] = heads_k > 0 ? wk : nullptr;
     p.w_f32[0] = wq_dt == DPIPE_F32; p.w_f32[1] = wk_dt == DPIPE_F32; p.eps = eps;
-    for (int w = 0; w < 2; ++w) p.magic[w] = p.heads[w] > 1 ? (unsigned)((0x100000000ull + p.heads[w] - 1) / p.heads[w]) : 0u;
+    p.pair_magic = (unsigned)((0x100000000ull + pairs - 1) / pairs);
+    const int groups = NB / lanes_per_row(D);
+    for (int w = 0; w < 2; ++w) { const int h = p.heads[w] > 0 ? p.heads[w] : 1; p.step_t[w] = groups / h; p.step_h[w] = groups % h; }
     for (int i = 0; i < pairs; ++i) {
         if (axis[i] < 0 || axis[i] >= axes) return bad("axis index out of range");
         p.freq[i] = freq[i]; p.axis[i] = (unsigned char)axis[i];
     }
-    p.tb = tile_tokens(tokens, pairs, D, heads_q > heads_k ? heads_q : heads_k);
+    p.tb = tile_tokens(tokens, pairs);
     return DPIPE_OK;
 }
 
-template <typename T, int LPR> void launch_fwd(const RopeAxesParams& p, bool half, unsigned grid, hipStream_t s) {
-    const bool norm = p.w[0] || p.w[1];
-    if (half) { if (norm) rope_axes_kernel<T, LPR, true, true><<<grid, NB, 0, s>>>(p); else rope_axes_kernel<T, LPR, true, false><<<grid, NB, 0, s>>>(p); }
-    else { if (norm) rope_axes_kernel<T, LPR, false, true><<<grid, NB, 0, s>>>(p); else rope_axes_kernel<T, LPR, false, false><<<grid, NB, 0, s>>>(p); }
-}
 template <typename T> void launch_fwd(const RopeAxesParams& p, bool half, hipStream_t s) {
     const unsigned grid = (unsigned)cdiv(p.tokens, p.tb);
-    if (p.D <= 64) launch_fwd<T, 8>(p, half, grid, s); else if (p.D <= 128) launch_fwd<T, 16>(p, half, grid, s); else launch_fwd<T, 32>(p, half, grid, s);
+#define LAUNCH(LPR) do { if (half) rope_axes_kernel<T, LPR, true><<<grid, NB, 0, s>>>(p); else rope_axes_kernel<T, LPR, false><<<grid, NB, 0, s>>>(p); } while (0)
+    switch (lanes_per_row(p.D)) { case 8: LAUNCH(8); break; case 16: LAUNCH(16); break; default: LAUNCH(32); }
+#undef LAUNCH
 }
-template <typename T> void launch_bwd(const RopeAxesParams& p, bool half, unsigned grid, hipStream_t s) {
+template <typename T> void launch_bwd(const RopeAxesParams& p, bool half, unsigned blocks, hipStream_t s) {
+    const dim3 grid(blocks, p.heads[1] > 0 ? 2 : 1);
 #define LAUNCH(LPR) do { if (half) rope_axes_bwd_kernel<T, LPR, true><<<grid, NB, 0, s>>>(p); else rope_axes_bwd_kernel<T, LPR, false><<<grid, NB, 0, s>>>(p); } while (0)
-    if (p.D <= 64) LAUNCH(8); else if (p.D <= 128) LAUNCH(16); else LAUNCH(32);
+    switch (lanes_per_row(p.D)) { case 8: LAUNCH(8); break; case 16: LAUNCH(16); break; default: LAUNCH(32); }
 #undef LAUNCH
 }
 
@@ -372,8 +424,9 @@ int dpipe_rope_axes_bwd(const void* q, const void* k, const void* gq, const void
     const int rc = fill(p, "dpipe_rope_axes_bwd", q, k, positions, pos_type, freq, axis, tokens, period, axes, pairs, heads_q, heads_k, D, q_ss, q_sh, k_ss, k_sh, wq, wk,
                         wq_dtype, wk_dtype, eps, half, dtype);
     if (rc) return rc;
-    if (!gq || (heads_k > 0 && !gk) || !rows_ok(gq, gq_ss, gq_sh) || (heads_k > 0 && !rows_ok(gk, gk_ss, gk_sh)) || !dq || (heads_k > 0 && !dk) || !aligned16(dq) || !aligned16(dk)) {
-        set_last_error("dpipe_rope_axes_bwd: gradients must be 16-byte aligned with strides multiple of 8 elements"); return DPIPE_ERR_ARG; }
+    if (!gq || (heads_k > 0 && !gk) || !rows_ok(gq, gq_ss, gq_sh) || !rows_fit(gq_ss, gq_sh, heads_q) ||
+        (heads_k > 0 && (!rows_ok(gk, gk_ss, gk_sh) || !rows_fit(gk_ss, gk_sh, heads_k))) || !dq || (heads_k > 0 && !dk) || !aligned16(dq) || !aligned16(dk)) {
+        set_last_error("dpipe_rope_axes_bwd: gradients must be 16-byte aligned with strides multiple of 8 elements, not too large"); return DPIPE_ERR_ARG; }
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     p.y[0] = dq; p.y[1] = dk; p.sign = -1.f;
     if (!p.w[0] && !p.w[1]) {                                  // no norm: the inverse rotation of the gradient

@@ -1423,7 +1423,7 @@ def _head_rows(x):
                 elif s != ss * tokens:
                     ok = False
             tokens *= size
-    if not ok or ss % 8 or not D <= ss < 2 ** 23:
+    if not ok or ss % 8 or not D <= ss < 2 ** 23 or st[-2] * H >= 2 ** 28:
         x = x.clone(memory_format=torch.contiguous_format)
         return x, tokens, H, D, H * D, D
     return x, tokens, H, D, ss, st[-2]
