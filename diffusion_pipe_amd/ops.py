@@ -1458,13 +1458,17 @@ def _on(device):
 
 
 @functools.lru_cache(maxsize=64)
-def _rope_axes_tables(axes_dim, theta, shared):
-    """host tables of the kernel: (turns per unit of position, axis) of every channel pair, in fp64"""
+def _rope_axes_tables(axes_dim, theta, shared, D, interleaved):
+    """host tables of the kernel: (turns per unit of position in fp64, axis) of every channel pair, and their count; the checks of what they are made from"""
+    thetas = theta if isinstance(theta, tuple) else (theta,) * len(axes_dim)
+    if not axes_dim or any(a <= 0 or a % 2 for a in axes_dim) or sum(axes_dim) > D or (not interleaved and sum(axes_dim) % 8) or len(thetas) != len(axes_dim) \
+            or any(not (t > 0.0 and math.isfinite(t)) for t in thetas) or (shared and len(set(thetas)) > 1):
+        raise DpipeHipError(f'rope_axes: even axis sizes that fit the head dim {D} (halves pairing: together a multiple of 8) and a positive theta (shared: one); got {axes_dim}, {theta}')
     total, freq, axis = sum(axes_dim), [], []
     for a, dim in enumerate(axes_dim):
         for j in range(dim // 2):
             e = -2.0 * len(freq) / total if shared else -2.0 * j / dim
-            freq.append(theta[a] ** e / (2.0 * math.pi))
+            freq.append(thetas[a] ** e / (2.0 * math.pi))
             axis.append(a)
     return (ctypes.c_double * len(freq))(*freq), (ctypes.c_int * len(axis))(*axis), len(freq)
 
@@ -1551,30 +1555,28 @@ def rope_axes(q, k, positions, axes_dim, theta=10000.0, q_weight=None, k_weight=
     interleaved: pairs are neighbouring channels (2 p, 2 p + 1); False: the halves (p, p + sum(axes_dim) / 2) of the rotated channels, whose count is a multiple of 8.
     Angles are formed in fp64 from the positions: far positions keep their precision.  (models/wan/model.py:40-67; diffusers FluxPosEmbed; models/hunyuan_video.py:35-81)
     -> (q', k'), contiguous; k' is None without k."""
-    axes_dim = tuple(int(a) for a in axes_dim)
-    theta = (float(theta),) * len(axes_dim) if not isinstance(theta, (tuple, list)) else tuple(float(t) for t in theta)
-    if q.dim() < 3 or (k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype)):
-        raise DpipeHipError(f'rope_axes: q [..., H, D] and k [..., Hk, D] of one dtype; got {tuple(q.shape)} {q.dtype} and {(tuple(k.shape), k.dtype) if k is not None else None}')
-    dtype_code(q.dtype)
-    D = q.shape[-1]
-    if D % 8 or not 0 < D <= 256 or q.shape[-2] == 0 or (k is not None and k.shape[-2] == 0):
-        raise DpipeHipError(f'rope_axes: the head dim must be a multiple of 8 up to 256, with at least one head; got {tuple(q.shape)}')
-    if not axes_dim or any(a <= 0 or a % 2 for a in axes_dim) or sum(axes_dim) > D or (not interleaved and sum(axes_dim) % 8) or len(theta) != len(axes_dim) \
-            or any(not (t > 0.0 and math.isfinite(t)) for t in theta) or (shared and len(set(theta)) > 1):
-        raise DpipeHipError(f'rope_axes: even axis sizes that fit the head dim {D} (halves pairing: together a multiple of 8) and a positive theta (shared: one); got {axes_dim}, {theta}')
+    qs, dtype = q.shape, q.dtype
+    if len(qs) < 3 or (k is not None and (k.shape[:-2] != qs[:-2] or k.shape[-1] != qs[-1] or k.dtype != dtype)):
+        raise DpipeHipError(f'rope_axes: q [..., H, D] and k [..., Hk, D] of one dtype; got {tuple(qs)} {dtype} and {(tuple(k.shape), k.dtype) if k is not None else None}')
+    dtype_code(dtype)
+    D = qs[-1]
+    if D % 8 or not 0 < D <= 256 or qs[-2] == 0 or (k is not None and k.shape[-2] == 0):
+        raise DpipeHipError(f'rope_axes: the head dim must be a multiple of 8 up to 256, with at least one head; got {tuple(qs)}')
+    tables = _rope_axes_tables(tuple(axes_dim), tuple(theta) if isinstance(theta, list) else theta, bool(shared), D, bool(interleaved))
+    ps = positions.shape
     if positions.dtype not in _POSITION_TYPES or positions.requires_grad:
         raise DpipeHipError(f'rope_axes: positions are fp32, int32 or int64 and have no gradient; got {positions.dtype}')
-    lead = tuple(q.shape[:-2])
-    if positions.dim() < 2 or positions.shape[-1] != len(axes_dim) or tuple(positions.shape[:-1]) != lead[len(lead) - positions.dim() + 1:]:
-        raise DpipeHipError(f'rope_axes: positions {tuple(positions.shape)} do not fit tokens {lead} and {len(axes_dim)} axes')
+    if len(ps) < 2 or ps[-1] != len(axes_dim) or len(ps) > len(qs) - 1 or ps[:-1] != qs[len(qs) - 1 - len(ps):-2]:
+        raise DpipeHipError(f'rope_axes: positions {tuple(ps)} do not fit tokens {tuple(qs[:-2])} and {len(axes_dim)} axes')
     for w in (q_weight, k_weight):
         if w is not None and tuple(w.shape) != (D,):
             raise DpipeHipError(f'rope_axes: norm weights have shape [{D}]; got {tuple(w.shape)}')
     if k is None and k_weight is not None:
         raise DpipeHipError('rope_axes: a key weight needs k')
-    args = (q, k, _contig(positions), q_weight, k_weight, _rope_axes_tables(axes_dim, theta, bool(shared)), float(eps), int(not interleaved))
+    args = (q, k, _contig(positions), q_weight, k_weight, tables, float(eps), 0 if interleaved else 1)
     with _on(_one_device(q, k, positions, q_weight, k_weight)):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad) or (q_weight is not None and q_weight.requires_grad)
+                                        or (k_weight is not None and k_weight.requires_grad)):
             return _RopeAxesFn.apply(*args)
         return _rope_axes_forward(*args)[:2]
 
