@@ -41,6 +41,11 @@ struct VarlenParams {
 constexpr int NT = 256, ROWS = 128;       // threads, query rows (dK / dV: keys) of a workgroup: 4 waves of 32
 constexpr int KT = 64;                   // keys (dK / dV: queries) per LDS tile
 constexpr int AQ = 4, AK = 1;            // steps of LDS operands read ahead of their products in the dQ and the dK / dV kernels
+// CORNER: in a row of few keys (a column of few queries) nothing averages the rounding of P and dS away, and the forward's reaches the row's dS through delta.  The forward and dQ
+// therefore multiply what the rounding of a sequence's first tile of keys left as well: one tile in lk / 64 (long sequences: within 1 %), and the rows that only see that tile, which
+// in causal sequences carry the largest gradients, are rounded once.  dK / dV do it for the first tile of keys against the first of queries where the sequences average at most one
+// tile (a variant: its registers cost the long ones 8 %, at D = 64 30 %).  Error against 64 bits, dQ / dK / dV, 24 causal sequences of 1 - 2 tokens: 2.53e-3 / 2.32e-3 / 1.82e-3 ->
+// 1.7e-3 each (one rounding); 457 + 16 + 32 + 172 + 208 causal tokens: dQ 2.40e-3 -> 1.8e-3.
 constexpr float M_INIT = -3.0e38f;       // running maximum before the first key: finite, so that exp2(-inf - m) is 0 and never NaN
 constexpr float RESCALE_AT = 8.f;        // the accumulator is rescaled when the maximum grew by more than 2^8: P stays below 256, its relative rounding is the same
 
@@ -207,6 +212,18 @@ __device__ __forceinline__ void ahead_run(Frag (&f)[AHEAD], Load load, Use use) 
     }
 }
 
+// what pack_frag's rounding leaves of 8 accumulator entries, itself as an operand
+__device__ __forceinline__ bf16x8_t pack_rest(const f32x16& s, int e0) {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = s[e0 + 2 * i], y = s[e0 + 2 * i + 1];
+        const uint32_t w = pack_bf16x2(x, y);
+        r[i] = pack_bf16x2(x - __uint_as_float(w << 16), y - __uint_as_float(w & 0xffff0000u));
+    }
+    return __builtin_bit_cast(bf16x8_t, make_uint4(r[0], r[1], r[2], r[3]));
+}
+
 __device__ __forceinline__ float max_halves(float x) {        // max over lane and lane ^ 32, in both
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -320,6 +337,14 @@ __global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const VarlenParams p)
             const bf16x8_t pf = pack_frag(s[u >> 1], 8 * (u & 1));
 #pragma unroll
             for (int db = 0; db < NDB; ++db) oacc[db] = mfma16(by_cols(Vl, 32 * db, 16 * u, lane), pf, oacc[db]);
+        }
+        if (kt == 0) {                                         // the first tile adds what the rounding left (see CORNER)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bf16x8_t pl = pack_rest(s[u >> 1], 8 * (u & 1));
+#pragma unroll
+                for (int db = 0; db < NDB; ++db) oacc[db] = mfma16(by_cols(Vl, 32 * db, 16 * u, lane), pl, oacc[db]);
+            }
         }
     }
 
@@ -451,6 +476,13 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const VarlenParams p) 
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * sl2 - lse) * (dp[e] - dl);
+            if (key0 < KT) {                                   // (CORNER)
+                const bf16x8_t rest[2] = {pack_rest(s, 0), pack_rest(s, 8)};
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int db = 0; db < NDB; ++db) dq[db] = mfma16(by_cols(Kl, 32 * db, 32 * kb + 16 * u, lane), rest[u], dq[db]);
+            }
             const bf16x8_t ds[2] = {pack_frag(s, 0), pack_frag(s, 8)};
             __builtin_amdgcn_sched_barrier(0);
             ahead_run<2 * NDB>(kt, load_t, [&](int j, const bf16x8_t& x) { dq[j % NDB] = mfma16(x, ds[j / NDB], dq[j % NDB]); });
@@ -464,8 +496,8 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const VarlenParams p) 
 // ================================================================================================ backward: dK, dV
 // Key-outer; a lane owns one key column, K stays in LDS, V and both accumulators in registers:  S = Q . K^T, dP = dO . V^T, dV^T += dO^T . P, dK^T += Q^T . dS.  Per 64-query tile Q and dO, both read by rows and transposed, and the
 // tile's lse / delta.  Query rows past the sequence arrive as zeros (Q, dO, lse, delta): P = 1 there, but dO = 0 and dS = 0.
-template <int D, int NW>
-__global__ void __launch_bounds__(NW * 64, D == 64 ? 3 : 2) varlen_dkv_kernel(const VarlenParams p) {
+template <int D, int NW, bool CORNER>
+__global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dkv_kernel(const VarlenParams p) {
     constexpr int QT = KT, NKS = D / 16, NDB = D / 32, IMG = QT * D * 2, O_STAT = 2 * IMG, STAGE = O_STAT + 1024;
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE + NW / 2 * IMG];
     const Work w = find_work(blockIdx.x, p.hk, p.nsplit);
@@ -556,6 +588,16 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? 3 : 2) varlen_dkv_kernel(co
                     s[e] = pr[e] * (dp[e] - dd[j]);
                 }
             }
+            if (CORNER && qt == 0 && k0w < KT) {
+                const bf16x8_t pl[2] = {pack_rest(pr, 0), pack_rest(pr, 8)}, sl[2] = {pack_rest(s, 0), pack_rest(s, 8)};
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int db = 0; db < NDB; ++db) {
+                        dv[db] = mfma16(by_cols(DOl, 32 * db, 32 * qb + 16 * u, lane), pl[u], dv[db]);
+                        dk[db] = mfma16(by_cols(Ql, 32 * db, 32 * qb + 16 * u, lane), sl[u], dk[db]);
+                    }
+            }
             const bf16x8_t pf[2] = {pack_frag(pr, 0), pack_frag(pr, 8)}, ds[2] = {pack_frag(s, 0), pack_frag(s, 8)};
             __builtin_amdgcn_sched_barrier(0);
             ahead_run<2 * NDB>(g, load_t, [&](int j, const Frags& x) { dv[j % NDB] = mfma16(x.d, pf[j / NDB], dv[j % NDB]); dk[j % NDB] = mfma16(x.q, ds[j / NDB], dk[j % NDB]); });
@@ -643,7 +685,8 @@ template <int D> void backward(VarlenParams& p, int parts, hipStream_t s) {
     varlen_dq_kernel<D><<<(unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, 1), NT, 0, s>>>(p);
     p.nsplit = parts;
     constexpr int NW = D == 128 ? 8 : 4;
-    varlen_dkv_kernel<D, NW><<<(unsigned)work_groups(row_slots(p.tk, 1, p.n, 32 * NW), p.hk, parts), 64 * NW, 0, s>>>(p);
+    const unsigned grid = (unsigned)work_groups(row_slots(p.tk, 1, p.n, 32 * NW), p.hk, parts);
+    if (p.tk / p.n <= KT) varlen_dkv_kernel<D, NW, true><<<grid, 64 * NW, 0, s>>>(p); else varlen_dkv_kernel<D, NW, false><<<grid, 64 * NW, 0, s>>>(p);
     if (parts > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
 }
 
