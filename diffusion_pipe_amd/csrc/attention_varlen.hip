@@ -272,14 +272,6 @@ __global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const VarlenParams p)
     const bf16_t* Q = p.q + r.token * p.q_ss + r.head * p.q_sh;
     const float sl2 = p.scale * LOG2E;
 
-    bf16x8_t qf[NKS];
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) qf[ks] = r.live ? *reinterpret_cast<const bf16x8_t*>(Q + 16 * ks + 8 * h) : zero_frag();
-    f32x16 oacc[NDB];
-#pragma unroll
-    for (int db = 0; db < NDB; ++db) oacc[db] = zero16();
-    float m = M_INIT, l = 0.f;                                 // running maximum in log2 units; this lane's part of the sum
-
     int kt0 = 0, kt1 = (seen.group + KT - 1) / KT;
     if (SPLIT) {                                               // every part of the sequence's key tiles, cut by its full length
         const int all = (t.lk + KT - 1) / KT, per = (all + p.nsplit - 1) / p.nsplit;
@@ -292,7 +284,15 @@ __global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const VarlenParams p)
         oK.issue(rows_rsrc<D>(K, p.k_ss, kt * KT, t.lk), base, wid);
         oV.issue(rows_rsrc<D>(V, p.v_ss, kt * KT, t.lk), base + IMG, wid);
     };
-    if (kt0 < kt1) issue(kt0);
+    if (kt0 < kt1) issue(kt0);                                 // (in flight under the query's own loads)
+    bf16x8_t qf[NKS];
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) qf[ks] = r.live ? *reinterpret_cast<const bf16x8_t*>(Q + 16 * ks + 8 * h) : zero_frag();
+    f32x16 oacc[NDB];
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) oacc[db] = zero16();
+    float m = M_INIT, l = 0.f;                                 // running maximum in log2 units; this lane's part of the sum
+
     for (int kt = kt0; kt < kt1; ++kt) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's pieces of tile kt
         __builtin_amdgcn_s_barrier();                          // everyone's pieces landed; everyone is done with the other buffer
@@ -425,6 +425,15 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const VarlenParams p) 
     const long row = r.token * p.hq + r.head, at = r.head * p.tq + r.token;
     const float sl2 = p.scale * LOG2E;
 
+    const int nkt = (seen.group + KT - 1) / KT;
+    Offsets<D, 4> oK, oV;
+    oK.init(wid, lane, p.k_ss); oV.init(wid, lane, p.v_ss);
+    auto issue = [&](int kt) {
+        char* base = lds + (kt & 1) * STAGE;
+        oK.issue(rows_rsrc<D>(K, p.k_ss, kt * KT, t.lk), base, wid);
+        oV.issue(rows_rsrc<D>(V, p.v_ss, kt * KT, t.lk), base + IMG, wid);
+    };
+    if (nkt > 0) issue(0);
     bf16x8_t qf[NKS], dof[NKS];
     float dl = 0.f;
 #pragma unroll
@@ -444,15 +453,6 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const VarlenParams p) 
 #pragma unroll
     for (int db = 0; db < NDB; ++db) dq[db] = zero16();
 
-    const int nkt = (seen.group + KT - 1) / KT;
-    Offsets<D, 4> oK, oV;
-    oK.init(wid, lane, p.k_ss); oV.init(wid, lane, p.v_ss);
-    auto issue = [&](int kt) {
-        char* base = lds + (kt & 1) * STAGE;
-        oK.issue(rows_rsrc<D>(K, p.k_ss, kt * KT, t.lk), base, wid);
-        oV.issue(rows_rsrc<D>(V, p.v_ss, kt * KT, t.lk), base + IMG, wid);
-    };
-    if (nkt > 0) issue(0);
     for (int kt = 0; kt < nkt; ++kt) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -509,14 +509,6 @@ __global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dk
     const bool live = key < t.lk;
     const int ahead = t.lk - t.lq;                             // causal: query x sees keys 0 .. x + ahead
     const float sl2 = p.scale * LOG2E;
-    const bf16_t* V = p.v + (t.k0 + (live ? key : 0)) * p.v_ss + w.head * p.v_sh;
-    bf16x8_t vf[NKS];
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) vf[ks] = live ? *reinterpret_cast<const bf16x8_t*>(V + 16 * ks + 8 * h) : zero_frag();
-    f32x16 dk[NDB], dv[NDB];
-#pragma unroll
-    for (int db = 0; db < NDB; ++db) { dk[db] = zero16(); dv[db] = zero16(); }
-
     // query tiles: from the first one that sees a key of this workgroup, for each of the g heads; this part's share of them
     const int first = p.causal ? max(0, (int)t.row0 - ahead) / QT * QT : 0;
     const int per_head = max(0, (t.lq - first + QT - 1) / QT);
@@ -545,6 +537,13 @@ __global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dk
         if (wid == 1) dma4(tile_rsrc(p.delta + stat + hd * p.tq + q, bytes), base + O_STAT + 256, lane * 4);
     };
     if (count > 0) issue(0);
+    const bf16_t* V = p.v + (t.k0 + (live ? key : 0)) * p.v_ss + w.head * p.v_sh;
+    bf16x8_t vf[NKS];
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) vf[ks] = live ? *reinterpret_cast<const bf16x8_t*>(V + 16 * ks + 8 * h) : zero_frag();
+    f32x16 dk[NDB], dv[NDB];
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) { dk[db] = zero16(); dv[db] = zero16(); }
     for (int it = 0; it < count; ++it) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
