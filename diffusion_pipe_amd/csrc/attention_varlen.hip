@@ -47,6 +47,8 @@ constexpr int AQ = 4, AK = 1;            // steps of LDS operands read ahead of 
 // tile (a variant: its registers cost the long ones 8 %, at D = 64 30 %).  Error against 64 bits, dQ / dK / dV, 24 causal sequences of 1 - 2 tokens: 2.53e-3 / 2.32e-3 / 1.82e-3 ->
 // 1.7e-3 each (one rounding); 457 + 16 + 32 + 172 + 208 causal tokens: dQ 2.40e-3 -> 1.8e-3.
 constexpr float M_INIT = -3.0e38f;       // running maximum before the first key: finite, so that exp2(-inf - m) is 0 and never NaN
+constexpr int SORTED = 32;               // sequences up to which their tiles are ordered by work (a forward of 1311 + 2560 + 4608 tokens as packed 378 us, ordered 347; 64 sequences of 128
+                                         // tokens 47 as packed, 72 ordered: the order costs a workgroup up to 90 ns a sequence)
 constexpr float RESCALE_AT = 8.f;        // the accumulator is rescaled when the maximum grew by more than 2^8: P stays below 256, its relative rounding is the same
 
 // ------------------------------------------------------------------------------------------------ which sequence, which rows
@@ -59,7 +61,7 @@ __device__ __forceinline__ int bound(const int* cu, int i, int n, int total) {
     const int c = cu[i];
     return c < 0 ? 0 : c > total ? total : c;
 }
-// slot -> sequence and first row; PER = rows per tile, gg = rows per token on the tiled side.  Up to 64 sequences (a lane each): the tiles of the sequences with the longest other
+// slot -> sequence and first row; PER = rows per tile, gg = rows per token on the tiled side.  Up to SORTED sequences (a lane each): the tiles of the sequences with the longest other
 // side first -- the workgroups with the most work start first -- each sequence's tiles from its ascending sum on, the rows behind the last sequence (n) after them.  More sequences:
 // the slots from  start / PER + b  on, in order.  `reversed`: the last tile of a sequence (causal: the one that sees most) first.
 template <int PER>
@@ -68,14 +70,15 @@ __device__ __forceinline__ Tile find_tile(const VarlenParams& p, int slot, bool 
     const int total = (int)(keys ? p.tk : p.tq), total2 = (int)(keys ? p.tq : p.tk), n = p.n;
     const int gg = keys ? 1 : p.g, lane = threadIdx.x & 63;
     int b, at, s0, s1, o0 = 0, o1 = 0;   // sequence, tile of it, its range on the tiled side and on the other (the rows behind the last sequence have no other side)
-    if (n <= 64) {
+    if (n <= SORTED) {
         const int i0 = min(lane, n - 1);
         const int my_s0 = bound(cu, i0, n, total), my_s1 = max(my_s0, bound(cu, i0 + 1, n, total)), my_o0 = bound(cu2, i0, n, total2), my_o1 = max(my_o0, bound(cu2, i0 + 1, n, total2));
-        const int nt = ((my_s1 - my_s0) * gg + PER - 1) / PER, work = my_o1 - my_o0;
+        const int nt = lane < n ? ((my_s1 - my_s0) * gg + PER - 1) / PER : 0, work = my_o1 - my_o0;
         int start = 0, all = 0;
-        for (int i = 0; i < n; ++i) {
+#pragma unroll 8
+        for (int i = 0; i < ((n + 7) & ~7); ++i) {             // (lanes from n on hold no tiles)
             const int nt_i = __builtin_amdgcn_readlane(nt, i), work_i = __builtin_amdgcn_readlane(work, i);
-            start += work_i > work || (work_i == work && i < lane) ? nt_i : 0;
+            start += nt_i & -(int)((work_i > work) | ((work_i == work) & (i < lane)));
             all += nt_i;
         }
         const unsigned long long here = __ballot(lane < n && slot >= start && slot < start + nt);
@@ -646,12 +649,15 @@ int fwd_splits(long tq, long tk, int n, int hq, int hk) {
     if (s > tiles / 4) s = tiles / 4;
     return (int)(s > 64 ? 64 : s);
 }
-// parts of the query tiles (of all g heads) for dK / dV, likewise; with grouped heads up to g parts also where the key tiles alone are fewer than 4 a CU
-int dkv_splits(long tq, long tk, int n, int hq, int hk) {
-    const long wgs = cdiv(tk, ROWS) * hk, g = hq / hk, tiles = tq / n / KT * g;
+// keys of a dK / dV workgroup: 8 waves at D = 128, whose K image and registers leave room for one workgroup per CU, 4 at 64
+constexpr int key_tile(int D) { return D == 128 ? 256 : 128; }
+// parts of the query tiles (of all g heads) for dK / dV, likewise; with grouped heads up to g parts also where the key tiles alone are fewer than 3 a CU and the sequences long enough
+// that the parts' fp32 sums do not cost more than the balance gives (4 x 2048 causal tokens, 32 / 8 heads, backward: 648 -> 604 us; 16 x 512: 310 unsplit, 332 split)
+int dkv_splits(long tq, long tk, int n, int hq, int hk, int D) {
+    const long wgs = cdiv(tk, key_tile(D)) * hk, g = hq / hk, tiles = tq / n / KT * g;
     long s = 1;
     if (wgs < 256 && tiles >= 8) { s = cdiv(512, wgs); if (s > tiles / 4) s = tiles / 4; }
-    if (wgs < 1024 && g > 1 && tiles >= 8 * g) { long m = cdiv(1024, wgs); if (m > g) m = g; if (m > s) s = m; }
+    if (wgs < 768 && g > 1 && tiles >= 16 * g) { long m = cdiv(768, wgs); if (m > g) m = g; if (m > s) s = m; }
     return (int)(s > 64 ? 64 : s);
 }
 
@@ -665,8 +671,8 @@ int fill(VarlenParams& p, const char* what, const void* q, const void* k, const 
     if (!q || !k || !v || !cu_q || !cu_k || tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk) return bad("bad argument");
     if (D != 64 && D != 128) return bad("head dim must be 64 or 128", DPIPE_ERR_UNSUPPORTED);
     if (!(scale > 0.f) || scale > 1e30f) return bad("scale must be positive and finite");
-    const int fs = fwd_splits(tq, tk, n, hq, hk), bs = dkv_splits(tq, tk, n, hq, hk);
-    if (tq * (hq / hk) >= (1l << 31) || tk >= (1l << 31) || work_groups(tq * (hq / hk) / ROWS + n + 1, hk, fs) >= (1l << 23) || work_groups(tk / ROWS + n + 1, hk, bs) >= (1l << 23))
+    const int fs = fwd_splits(tq, tk, n, hq, hk), bs = dkv_splits(tq, tk, n, hq, hk, D);
+    if (tq * (hq / hk) >= (1l << 31) - 256 || tk >= (1l << 31) - 256 || work_groups(tq * (hq / hk) / ROWS + n + 1, hk, fs) >= (1l << 23) || work_groups(tk / ROWS + n + 1, hk, bs) >= (1l << 23))
         return bad("too many rows or sequences", DPIPE_ERR_UNSUPPORTED);
     if (!rows_ok(q, q_ss, q_sh, D) || !rows_ok(k, k_ss, k_sh, D) || !rows_ok(v, v_ss, v_sh, D)) return bad("tensors must be 16-byte aligned with strides multiple of 8 elements");
     p.q = (const bf16_t*)q; p.k = (const bf16_t*)k; p.v = (const bf16_t*)v; p.cu_q = cu_q; p.cu_k = cu_k; p.tq = tq; p.tk = tk; p.n = n; p.hq = hq; p.hk = hk; p.g = hq / hk;
@@ -683,7 +689,7 @@ template <int D> void forward(const VarlenParams& p, hipStream_t s) {
 template <int D> void backward(VarlenParams& p, int parts, hipStream_t s) {
     varlen_dq_kernel<D><<<(unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, 1), NT, 0, s>>>(p);
     p.nsplit = parts;
-    constexpr int NW = D == 128 ? 8 : 4;
+    constexpr int NW = key_tile(D) / 32;
     const unsigned grid = (unsigned)work_groups(row_slots(p.tk, 1, p.n, 32 * NW), p.hk, parts);
     if (p.tk / p.n <= KT) varlen_dkv_kernel<D, NW, true><<<grid, 64 * NW, 0, s>>>(p); else varlen_dkv_kernel<D, NW, false><<<grid, 64 * NW, 0, s>>>(p);
     if (parts > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
@@ -700,7 +706,7 @@ long dpipe_attn_varlen_fwd_workspace_floats(long tq, long tk, int n, int hq, int
 }
 long dpipe_attn_varlen_bwd_workspace_floats(long tq, long tk, int n, int hq, int hk, int D) {
     if (tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk || (D != 64 && D != 128)) return 0;
-    const int s = dkv_splits(tq, tk, n, hq, hk);
+    const int s = dkv_splits(tq, tk, n, hq, hk, D);
     return s > 1 ? 2l * s * tk * hk * D : 0;
 }
 
@@ -731,7 +737,7 @@ int dpipe_attn_varlen_bwd(const void* q, const void* k, const void* v, const int
     if (ablated(ABL_ATTN)) return DPIPE_OK;
     p.o = (bf16_t*)o; p.o_lo = (bf16_t*)o_lo; p.dout = (const bf16_t*)dout; p.lse = const_cast<float*>(lse); p.delta = delta;
     p.dq = (bf16_t*)dq; p.dk = (bf16_t*)dk; p.dv = (bf16_t*)dv; p.do_ss = do_ss; p.do_sh = do_sh; p.part = ws;
-    const int splits = need > 0 ? dkv_splits(tq, tk, n, hq, hk) : 1;
+    const int splits = need > 0 ? dkv_splits(tq, tk, n, hq, hk, D) : 1;
     if (D == 64) backward<64>(p, splits, reinterpret_cast<hipStream_t>(stream)); else backward<128>(p, splits, reinterpret_cast<hipStream_t>(stream));
     return check_launch("dpipe_attn_varlen_bwd");
 }

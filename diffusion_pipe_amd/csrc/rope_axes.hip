@@ -381,6 +381,7 @@ int fill(RopeAxesParams& p, const char* what, const void* q, const void* k, cons
         p.freq[i] = freq[i]; p.axis[i] = (unsigned char)axis[i];
     }
     p.tb = tile_tokens(tokens, pairs);
+    if (cdiv(tokens, p.tb) >= (1l << 23)) return bad("too many tokens");
     return DPIPE_OK;
 }
 

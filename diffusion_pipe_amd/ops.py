@@ -1429,6 +1429,10 @@ def _head_rows(x):
     return x, tokens, H, D, ss, st[-2]
 
 
+def _dense(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _addr(t):
     return None if t is None else t.data_ptr()
 
@@ -1480,12 +1484,12 @@ def _rope_axes_forward(q, k, positions, q_weight, k_weight, tables, eps, half):
     """-> (yq, yk, (q, k as read), what the backward's call repeats)"""
     device = q.device
     q, tokens, hq, D, q_ss, q_sh = _head_rows(q)
-    yq = torch.empty(q.shape, device=device, dtype=q.dtype)
+    yq = _dense(q)
     hk = k_ss = k_sh = 0
     yk = None
     if k is not None:
         k, _, hk, _, k_ss, k_sh = _head_rows(k)
-        yk = torch.empty(k.shape, device=device, dtype=k.dtype)
+        yk = _dense(k)
     freq, axis, pairs = tables
     axes = positions.shape[-1]
     meta = (tokens, positions.numel() // axes, axes, pairs, hq, hk, D)
@@ -1504,7 +1508,6 @@ class _RopeAxesFn(Function):
 
     @staticmethod
     def forward(ctx, q, k, positions, q_weight, k_weight, tables, eps, half):
-        ctx.shapes = (q.shape, None if k is None else k.shape, q.dtype)
         yq, yk, q, k, ctx.call = _rope_axes_forward(q, k, positions, q_weight, k_weight, tables, eps, half)
         normed = q_weight is not None or k_weight is not None
         ctx.save_for_backward(q if normed else None, k if normed else None, positions, q_weight, k_weight)
@@ -1514,15 +1517,14 @@ class _RopeAxesFn(Function):
     def backward(ctx, gq, gk):
         q, k, positions, q_weight, k_weight = ctx.saved_tensors
         meta, strides, tail, (freq, axis, _) = ctx.call
-        q_shape, k_shape, dtype = ctx.shapes
-        tokens, D, device = meta[0], meta[-1], gq.device
+        tokens, has_k, D, device = meta[0], meta[5] > 0, meta[6], gq.device
         with _on(device):
             gq, _, _, _, gq_ss, gq_sh = _head_rows(gq)
-            dq = torch.empty(q_shape, device=device, dtype=dtype)
+            dq = _dense(gq)
             dk, gk_ss, gk_sh = None, 0, 0
-            if k_shape is not None:
+            if has_k:
                 gk, _, _, _, gk_ss, gk_sh = _head_rows(gk)
-                dk = torch.empty(k_shape, device=device, dtype=dtype)
+                dk = _dense(gk)
             else:
                 gk = None
             normed = q is not None
@@ -1532,6 +1534,8 @@ class _RopeAxesFn(Function):
             for i, w in enumerate((q_weight, k_weight)):
                 if w is not None and ctx.needs_input_grad[3 + i]:
                     dw[i] = _accum_target(w)
+                    if dw[i] is not None and i == 1 and fused[0] and dw[0].data_ptr() == dw[1].data_ptr():
+                        dw[i] = None                      # one weight for queries and keys: the kernel must not add into its gradient from two workgroups at once
                     fused[i] = dw[i] is not None
                     if dw[i] is None:
                         dw[i] = torch.empty_like(w) if tokens else torch.zeros_like(w)
@@ -1573,6 +1577,7 @@ def rope_axes(q, k, positions, axes_dim, theta=10000.0, q_weight=None, k_weight=
             raise DpipeHipError(f'rope_axes: norm weights have shape [{D}]; got {tuple(w.shape)}')
     if k is None and k_weight is not None:
         raise DpipeHipError('rope_axes: a key weight needs k')
+    q_weight, k_weight = (w if w is None or w.is_contiguous() else w.contiguous() for w in (q_weight, k_weight))
     args = (q, k, _contig(positions), q_weight, k_weight, tables, float(eps), 0 if interleaved else 1)
     with _on(_one_device(q, k, positions, q_weight, k_weight)):
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad) or (q_weight is not None and q_weight.requires_grad)
@@ -1779,9 +1784,8 @@ def _varlen_forward(q, k, v, cu_q, cu_k, scale, causal, keep):
     if tq == 0 or tk == 0:                        # nothing to read: every row is empty
         return torch.zeros(q.shape, device=device, dtype=q.dtype), (), None
     sizes, strides = (tq, tk, cu_q.shape[0] - 1, hq, hk, D), (*qs, *ks, *vs)
-    o = torch.empty((tq, hq, D), device=device, dtype=q.dtype)
-    lse = torch.empty((hq, tq), device=device, dtype=torch.float32) if keep else None
-    o_lo = torch.empty((tq, hq, D), device=device, dtype=q.dtype) if keep else None
+    o = _dense(q)
+    o_lo, lse = (torch.empty_like(o), q.new_empty((hq, tq), dtype=torch.float32)) if keep else (None, None)
     need = lib().dpipe_attn_varlen_fwd_workspace_floats(*sizes)
     ws = torch.empty(need, device=device, dtype=torch.float32) if need else None
     check(lib().dpipe_attn_varlen_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _addr(o_lo), _addr(lse), _addr(ws), need, *sizes,
@@ -1809,7 +1813,7 @@ class _AttnVarlenFn(Function):
         sizes, strides, scale, causal = ctx.call
         with _on(device):
             do, _, _, _, *ds = _head_rows(do)
-            dq, dk, dv = (torch.empty(sh, device=device, dtype=q.dtype) for sh in ctx.shapes[:3])
+            dq, dk, dv = _dense(q), _dense(k), _dense(v)
             delta = torch.empty_like(lse)
             need = lib().dpipe_attn_varlen_bwd_workspace_floats(*sizes)
             ws = torch.empty(need, device=device, dtype=torch.float32) if need else None

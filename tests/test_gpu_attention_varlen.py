@@ -88,6 +88,8 @@ CASES = [  # (queries, keys (None: the same), H, Hk, causal)
     ([0, 70], [33, 64], 2, 1, True),                       # a sequence without queries
     ([1, 1, 2, 1], [700, 64, 65, 1], 8, 1, True),          # single tokens, eight heads to a key head
     ([130] * 70, None, 2, 1, True),                        # more sequences than a wave has lanes
+    ([5, 70, 1, 128, 33, 64, 65, 2] * 5, None, 6, 2, True),      # more sequences than are ordered by length
+    ([129, 1, 64] * 11 , [7, 300, 65] * 11, 2, 2, False),
     ([1000, 600], None, 24, 24, False),                    # 8-wave tiles
     ([900, 1100], None, 32, 8, True),
 ]
@@ -272,6 +274,26 @@ def test_offsets_that_do_not_ascend_stay_inside_the_tensors(gpu):
     for bad in ([0, 150, 100], [0, -5, 900], [0, 2000000000, -2000000000], [50, 20, 200]):
         _run(q, k, v, do, torch.tensor(bad, dtype=torch.int32, device=gpu), None, True)
     torch.cuda.synchronize()
+
+
+def test_sequences_of_one_tile_are_rounded_once(gpu):
+    """sequences of up to 64 tokens multiply what the rounding of P and dS left as well: o, dQ, dK, dV are off by their own rounding (h) and by products of two roundings (h^2),
+    the same terms as the bounds above with h^2 for h, and fp32's"""
+    lens, H, Hk, D = [1, 2, 1, 9, 5, 64, 1, 12, 40, 2], 4, 2, 128
+    q, k, v, do, cu, _ = _inputs(gpu, lens, lens, H, Hk, D)
+    got = _run(q, k, v, do, cu, None, True)
+    global H_BF16, R_P
+    keep = H_BF16, R_P
+    want = _exact(q, k, v, do, lens, lens, True, 1.0 / math.sqrt(D))
+    try:
+        H_BF16, R_P = 2.0 ** -16, 2.0 ** -10
+        once = _exact(q, k, v, do, lens, lens, True, 1.0 / math.sqrt(D))
+    finally:
+        H_BF16, R_P = keep
+    for n, t in got.items():
+        value, bound = once[n]
+        assert ((t.detach().double() - value).abs() <= bound + H_BF16 * (value.abs() + bound)).all(), n
+    _check(got, want, 'one tile')
 
 
 def test_empty_tensors(gpu):

@@ -192,6 +192,31 @@ def test_views_gradients_and_accumulation(gpu):
     assert ((wq.grad.to(f) - 3.0 - second[1].to(f)).abs() <= 2.0 ** -7 * (3.0 + second[1].to(f).abs())).all()
 
 
+def test_one_weight_for_queries_and_keys(gpu):
+    """a shared, strided weight gets the sum of both gradients, also where the parameter gradients are accumulated inside the kernels"""
+    from diffusion_pipe_amd import ops
+    g = torch.Generator().manual_seed(7)
+    q, k = (torch.randn(300, h, 64, generator=g).to(gpu) for h in (4, 2))
+    gq, gk = torch.randn(300, 4, 64, generator=g).to(gpu), torch.randn(300, 2, 64, generator=g).to(gpu)
+    pos = _positions(gpu, (300,), 1, torch.int64)
+    wide = torch.nn.Parameter(1 + 0.2 * torch.randn(128, generator=g).to(gpu))
+    w = torch.nn.Parameter(wide.detach()[::2].contiguous())
+    angles = _angles(pos, (64,), 10000.0)
+    (vq, bq), (vk, bk) = (_exact(x, w, gy, angles, 1e-6, True, 300)['dw'] for x, gy in ((q, gq), (k, gk)))
+    y = ops.rope_axes(q, k, pos, (64,), q_weight=wide[::2], k_weight=wide[::2])
+    got, = torch.autograd.grad(y, wide, (gq, gk))
+    assert ((got[::2].double() - vq - vk).abs() <= bq + bk + F * (vq + vk).abs()).all() and (got[1::2] == 0).all()
+    for fuse in (False, True):
+        w.grad = torch.full_like(w, 5.0)
+        y = ops.rope_axes(q, k, pos, (64,), q_weight=w, k_weight=w)
+        ops.FUSE_GRAD_ACCUM = fuse
+        try:
+            torch.autograd.backward(y, (gq, gk))
+        finally:
+            ops.FUSE_GRAD_ACCUM = False
+        assert ((w.grad.double() - 5.0 - vq - vk).abs() <= bq + bk + 4 * F * (5.0 + vq.abs() + vk.abs())).all(), fuse
+
+
 def test_gradients_against_differences(gpu):
     from diffusion_pipe_amd import ops
     g = torch.Generator().manual_seed(8)
