@@ -35,6 +35,7 @@ struct RopeAxesParams {
     long tokens, period;                 // positions repeat every `period` tokens
     int heads[2];
     int D, pairs, axes, tb, pos_type, w_f32[2];
+    int stream;                          // the tensors are larger than the last-level cache
     unsigned pair_magic;                 // ceil(2^32 / pairs): entry / pairs of a table by multiplication
     int step_t[2], step_h[2];            // lane groups per workgroup = step_t heads + step_h: a lane group's next row is step_t tokens and step_h heads further
     float eps, sign;                     // sign = -1: the inverse rotation
@@ -53,36 +54,45 @@ template <> __device__ __forceinline__ void load4<float>(const float* p, float* 
 }
 
 // the 8 channels of a lane as loaded, 16 (bf16) or 32 (fp32) bytes: neighbours pairing = channels 8 l .. 8 l + 7, halves pairing = 4 channels of either half
-template <typename T, bool HALF> struct Raw8 {
-    uint4 v[sizeof(T) / 2];
+// STREAM: past the caches (tensors that no cache holds until they are read again)
+template <bool STREAM, typename V> __device__ __forceinline__ V get_vec(const void* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p)); else return *reinterpret_cast<const V*>(p);
+}
+template <bool STREAM, typename V> __device__ __forceinline__ void put_vec(void* p, V v) {
+    if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<V*>(p)); else *reinterpret_cast<V*>(p) = v;
+}
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2_t;
+
+template <typename T, bool HALF, bool STREAM> struct Raw8 {
+    u32x4_t v[sizeof(T) / 2];
     __device__ __forceinline__ void load(const T* p, int c0, int c1) {
         if constexpr (sizeof(T) == 4) {
-            v[0] = *reinterpret_cast<const uint4*>(p + c0); v[1] = *reinterpret_cast<const uint4*>(p + c1);
+            v[0] = get_vec<STREAM, u32x4_t>(p + c0); v[1] = get_vec<STREAM, u32x4_t>(p + c1);
         } else if constexpr (HALF) {
-            const uint2 a = *reinterpret_cast<const uint2*>(p + c0), b = *reinterpret_cast<const uint2*>(p + c1);
-            v[0] = make_uint4(a.x, a.y, b.x, b.y);
+            const u32x2_t a = get_vec<STREAM, u32x2_t>(p + c0), b = get_vec<STREAM, u32x2_t>(p + c1);
+            v[0] = u32x4_t{a.x, a.y, b.x, b.y};
         } else {
-            v[0] = *reinterpret_cast<const uint4*>(p + c0);
+            v[0] = get_vec<STREAM, u32x4_t>(p + c0);
         }
     }
     __device__ __forceinline__ void store(T* p, int c0, int c1) const {
         if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<uint4*>(p + c0) = v[0]; *reinterpret_cast<uint4*>(p + c1) = v[1];
+            put_vec<STREAM>(p + c0, v[0]); put_vec<STREAM>(p + c1, v[1]);
         } else if constexpr (HALF) {
-            *reinterpret_cast<uint2*>(p + c0) = make_uint2(v[0].x, v[0].y); *reinterpret_cast<uint2*>(p + c1) = make_uint2(v[0].z, v[0].w);
+            put_vec<STREAM>(p + c0, u32x2_t{v[0].x, v[0].y}); put_vec<STREAM>(p + c1, u32x2_t{v[0].z, v[0].w});
         } else {
-            *reinterpret_cast<uint4*>(p + c0) = v[0];
+            put_vec<STREAM>(p + c0, v[0]);
         }
     }
     __device__ __forceinline__ void unpack(float* f) const {
         Vec16<T> u;
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) { u.raw = v[i]; u.unpack(f + i * Vec16<T>::N); }
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) { u.raw = __builtin_bit_cast(uint4, v[i]); u.unpack(f + i * Vec16<T>::N); }
     }
     __device__ __forceinline__ void pack(const float* f) {
         Vec16<T> u;
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) { u.pack(f + i * Vec16<T>::N); v[i] = u.raw; }
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) { u.pack(f + i * Vec16<T>::N); v[i] = __builtin_bit_cast(u32x4_t, u.raw); }
     }
 };
 
@@ -166,8 +176,8 @@ template <bool HALF, int LPR> struct Lane {
 };
 
 // The rows of one tensor of a tile: y = R [norm](x)
-template <typename T, int LPR, bool HALF, bool NORM>
-__device__ __forceinline__ void rows_forward(const RopeAxesParams& p, const Lane<HALF, LPR>& ln, const float* table, int which, long t0, int ntok, Raw8<T, HALF>* raw, bool loaded) {
+template <typename T, int LPR, bool HALF, bool STREAM, bool NORM>
+__device__ __forceinline__ void rows_forward(const RopeAxesParams& p, const Lane<HALF, LPR>& ln, const float* table, int which, long t0, int ntok, Raw8<T, HALF, STREAM>* raw, bool loaded) {
     constexpr int GROUPS = NB / LPR;
     const int heads = p.heads[which], rows = ntok * heads, iters = (rows + GROUPS - 1) / GROUPS, pitch = table_pitch(p.pairs);
     const int ss = (int)p.x_ss[which], sh = (int)p.x_sh[which], st = p.step_t[which], sd = p.step_h[which];
@@ -178,7 +188,7 @@ __device__ __forceinline__ void rows_forward(const RopeAxesParams& p, const Lane
     if (NORM) load_weight(p, which, ln.c0, ln.c1, w);
     Walk get, put;
     get.start(ln.grp, heads); put.start(ln.grp, heads);
-    auto fetch = [&](Raw8<T, HALF>& r) {
+    auto fetch = [&](Raw8<T, HALF, STREAM>& r) {
         if (get.token < ntok) r.load(x + get.offset(ss, sh), ln.c0, ln.c1);
         get.next(st, sd, heads);
     };
@@ -202,7 +212,7 @@ __device__ __forceinline__ void rows_forward(const RopeAxesParams& p, const Lane
             }
             const bool live = ln.in && put.token < ntok;
             rotate<HALF>(f, table + (put.token < ntok ? put.token * pitch : 0), ln.p0, ln.in && 4 * ln.sub < p.pairs ? p.pairs : 0, ln.full);
-            Raw8<T, HALF> out;
+            Raw8<T, HALF, STREAM> out;
             out.pack(f);
             if (live) out.store(y + (unsigned)((put.token * heads + put.head) * p.D), ln.c0, ln.c1);
             put.next(st, sd, heads);
@@ -211,21 +221,21 @@ __device__ __forceinline__ void rows_forward(const RopeAxesParams& p, const Lane
 }
 
 // y = R(sign * theta) [norm](x): the forward, and the backward of rows without a norm (sign = -1)
-template <typename T, int LPR, bool HALF>
+template <typename T, int LPR, bool HALF, bool STREAM>
 __global__ void __launch_bounds__(NB) rope_axes_kernel(const RopeAxesParams p) {
     __shared__ __attribute__((aligned(16))) float table[2 * TABLE];     // cosines, then sines
     const Lane<HALF, LPR> ln(p);
     const long t0 = (long)blockIdx.x * p.tb;
     const int ntok = (int)min((long)p.tb, p.tokens - t0);
     fill_table(p, table, t0, ntok);
-    Raw8<T, HALF> raw[AHEAD];
-    if (p.w[0]) rows_forward<T, LPR, HALF, true>(p, ln, table, 0, t0, ntok, raw, false); else rows_forward<T, LPR, HALF, false>(p, ln, table, 0, t0, ntok, raw, false);
+    Raw8<T, HALF, STREAM> raw[AHEAD];
+    if (p.w[0]) rows_forward<T, LPR, HALF, STREAM, true>(p, ln, table, 0, t0, ntok, raw, false); else rows_forward<T, LPR, HALF, STREAM, false>(p, ln, table, 0, t0, ntok, raw, false);
     if (p.heads[1] == 0) return;
-    if (p.w[1]) rows_forward<T, LPR, HALF, true>(p, ln, table, 1, t0, ntok, raw, true); else rows_forward<T, LPR, HALF, false>(p, ln, table, 1, t0, ntok, raw, true);
+    if (p.w[1]) rows_forward<T, LPR, HALF, STREAM, true>(p, ln, table, 1, t0, ntok, raw, true); else rows_forward<T, LPR, HALF, STREAM, false>(p, ln, table, 1, t0, ntok, raw, true);
 }
 
 // The backward of one tensor's rows of a tile: dx, and the weight's gradient added to the lane's dw
-template <typename T, int LPR, bool HALF, bool NORM>
+template <typename T, int LPR, bool HALF, bool STREAM, bool NORM>
 __device__ __forceinline__ void rows_backward(const RopeAxesParams& p, const Lane<HALF, LPR>& ln, const float* table, int which, long t0, int ntok, const float* w, float* dw) {
     constexpr int GROUPS = NB / LPR, A = 2;
     const int heads = p.heads[which], rows = ntok * heads, iters = (rows + GROUPS - 1) / GROUPS, pitch = table_pitch(p.pairs);
@@ -234,7 +244,7 @@ __device__ __forceinline__ void rows_backward(const RopeAxesParams& p, const Lan
     const T* gy = reinterpret_cast<const T*>(p.gy[which]) + t0 * p.g_ss[which];
     T* dx = reinterpret_cast<T*>(p.y[which]) + t0 * heads * (long)p.D;
     const float inv_d = 1.f / (float)p.D;
-    Raw8<T, HALF> rx[A], rg[A];
+    Raw8<T, HALF, STREAM> rx[A], rg[A];
     Walk get, put;
     get.start(ln.grp, heads); put.start(ln.grp, heads);
     auto fetch = [&](int u) {
@@ -270,7 +280,7 @@ __device__ __forceinline__ void rows_backward(const RopeAxesParams& p, const Lan
                     g[j] = rstd * (g[j] * w[j] - xh * m);
                 }
             }
-            Raw8<T, HALF> out;
+            Raw8<T, HALF, STREAM> out;
             out.pack(g);
             if (live) out.store(dx + (unsigned)((put.token * heads + put.head) * p.D), ln.c0, ln.c1);
             put.next(st, sd, heads);
@@ -280,7 +290,7 @@ __device__ __forceinline__ void rows_backward(const RopeAxesParams& p, const Lan
 
 // the backward with norms: dx, and per workgroup one partial row of the weight's gradient (summed in a fixed order by rope_axes_dw_kernel).  A workgroup takes the tiles of one
 // tensor (blockIdx.y): with both, the weights and their gradients of both sit in registers and 4 waves a SIMD spill.
-template <typename T, int LPR, bool HALF>
+template <typename T, int LPR, bool HALF, bool STREAM>
 __global__ void __launch_bounds__(NB, 4) rope_axes_bwd_kernel(const RopeAxesParams p) {
     constexpr int GROUPS = NB / LPR;
     __shared__ __attribute__((aligned(16))) float table[2 * TABLE];     // cosines, then sines
@@ -296,8 +306,8 @@ __global__ void __launch_bounds__(NB, 4) rope_axes_bwd_kernel(const RopeAxesPara
         const int ntok = (int)min((long)p.tb, p.tokens - t0);
         __syncthreads();                                       // the previous tile's rows are done with the table
         fill_table(p, table, t0, ntok);
-        if (norm) rows_backward<T, LPR, HALF, true>(p, ln, table, which, t0, ntok, w, dw);
-        else rows_backward<T, LPR, HALF, false>(p, ln, table, which, t0, ntok, w, dw);
+        if (norm) rows_backward<T, LPR, HALF, STREAM, true>(p, ln, table, which, t0, ntok, w, dw);
+        else rows_backward<T, LPR, HALF, STREAM, false>(p, ln, table, which, t0, ntok, w, dw);
     }
     __syncthreads();
     if (ln.in) {
@@ -373,6 +383,9 @@ int fill(RopeAxesParams& p, const char* what, const void* q, const void* k, cons
     p.pos = pos; p.pos_type = pos_type; p.tokens = tokens; p.period = period; p.axes = axes; p.pairs = pairs; p.D = D;
     p.heads[0] = heads_q; p.heads[1] = heads_k; p.w[0] = wq; p.w[1] = heads_k > 0 ? wk : nullptr;
     p.w_f32[0] = wq_dt == DPIPE_F32; p.w_f32[1] = wk_dt == DPIPE_F32; p.eps = eps;
+    // 256 MB of last-level cache: below, what is written here is read from it by the attention that follows, and the forward's rows by the backward; above, streaming past it is faster
+    // (755 MB of heads: forward 271 -> 255 us = 5.9 TB/s, backward 443 -> 413; 57 MB: 21.3 us cached, 22.6 streamed)
+    p.stream = tokens * (long)(heads_q + heads_k) * D * (dt == DPIPE_F32 ? 4 : 2) > (256l << 20);
     p.pair_magic = (unsigned)((0x100000000ull + pairs - 1) / pairs);
     const int groups = NB / lanes_per_row(D);
     for (int w = 0; w < 2; ++w) { const int h = p.heads[w] > 0 ? p.heads[w] : 1; p.step_t[w] = groups / h; p.step_h[w] = groups % h; }
@@ -385,17 +398,20 @@ int fill(RopeAxesParams& p, const char* what, const void* q, const void* k, cons
     return DPIPE_OK;
 }
 
-template <typename T> void launch_fwd(const RopeAxesParams& p, bool half, hipStream_t s) {
-    const unsigned grid = (unsigned)cdiv(p.tokens, p.tb);
-#define LAUNCH(LPR) do { if (half) rope_axes_kernel<T, LPR, true><<<grid, NB, 0, s>>>(p); else rope_axes_kernel<T, LPR, false><<<grid, NB, 0, s>>>(p); } while (0)
+template <typename T, bool HALF, bool STREAM> void launch(const RopeAxesParams& p, bool backward, unsigned blocks, hipStream_t s) {
+    const dim3 grid(blocks, backward && p.heads[1] > 0 ? 2 : 1);
+#define LAUNCH(LPR) do { if (backward) rope_axes_bwd_kernel<T, LPR, HALF, STREAM><<<grid, NB, 0, s>>>(p); else rope_axes_kernel<T, LPR, HALF, STREAM><<<grid, NB, 0, s>>>(p); } while (0)
     switch (lanes_per_row(p.D)) { case 8: LAUNCH(8); break; case 16: LAUNCH(16); break; default: LAUNCH(32); }
 #undef LAUNCH
 }
-template <typename T> void launch_bwd(const RopeAxesParams& p, bool half, unsigned blocks, hipStream_t s) {
-    const dim3 grid(blocks, p.heads[1] > 0 ? 2 : 1);
-#define LAUNCH(LPR) do { if (half) rope_axes_bwd_kernel<T, LPR, true><<<grid, NB, 0, s>>>(p); else rope_axes_bwd_kernel<T, LPR, false><<<grid, NB, 0, s>>>(p); } while (0)
-    switch (lanes_per_row(p.D)) { case 8: LAUNCH(8); break; case 16: LAUNCH(16); break; default: LAUNCH(32); }
-#undef LAUNCH
+// backward: the kernel with norms (without, the backward is the forward's kernel with the sign turned round)
+void launch(const RopeAxesParams& p, int dtype, bool half, bool backward, unsigned blocks, hipStream_t s) {
+    auto with = [&](auto type) {
+        typedef decltype(type) T;
+        if (half) { if (p.stream) launch<T, true, true>(p, backward, blocks, s); else launch<T, true, false>(p, backward, blocks, s); }
+        else { if (p.stream) launch<T, false, true>(p, backward, blocks, s); else launch<T, false, false>(p, backward, blocks, s); }
+    };
+    if (dtype == DPIPE_BF16) with(bf16_t{}); else with(float{});
 }
 
 }  // namespace
@@ -411,7 +427,7 @@ int dpipe_rope_axes_fwd(const void* q, const void* k, const void* positions, int
     if (rc) return rc;
     if (!yq || (heads_k > 0 && !yk) || !aligned16(yq) || !aligned16(yk)) { set_last_error("dpipe_rope_axes_fwd: bad output"); return DPIPE_ERR_ARG; }
     p.y[0] = yq; p.y[1] = yk; p.sign = 1.f;
-    if (dtype == DPIPE_BF16) launch_fwd<bf16_t>(p, half, reinterpret_cast<hipStream_t>(stream)); else launch_fwd<float>(p, half, reinterpret_cast<hipStream_t>(stream));
+    launch(p, dtype, half, false, (unsigned)cdiv(p.tokens, p.tb), reinterpret_cast<hipStream_t>(stream));
     return check_launch("dpipe_rope_axes_fwd");
 }
 
@@ -432,14 +448,14 @@ int dpipe_rope_axes_bwd(const void* q, const void* k, const void* gq, const void
     p.y[0] = dq; p.y[1] = dk; p.sign = -1.f;
     if (!p.w[0] && !p.w[1]) {                                  // no norm: the inverse rotation of the gradient
         p.x[0] = gq; p.x[1] = gk; p.x_ss[0] = gq_ss; p.x_sh[0] = gq_sh; p.x_ss[1] = gk_ss; p.x_sh[1] = gk_sh;
-        if (dtype == DPIPE_BF16) launch_fwd<bf16_t>(p, half, s); else launch_fwd<float>(p, half, s);
+        launch(p, dtype, half, false, (unsigned)cdiv(p.tokens, p.tb), s);
         return check_launch("dpipe_rope_axes_bwd");
     }
     if (!ws) { set_last_error("dpipe_rope_axes_bwd: a normed row needs the workspace"); return DPIPE_ERR_ARG; }
     p.gy[0] = gq; p.gy[1] = gk; p.g_ss[0] = gq_ss; p.g_sh[0] = gq_sh; p.g_ss[1] = gk_ss; p.g_sh[1] = gk_sh; p.part = ws;
     const long tiles = cdiv(tokens, p.tb);
     const unsigned grid = (unsigned)(tiles < MAX_BWD_BLOCKS ? tiles : MAX_BWD_BLOCKS);
-    if (dtype == DPIPE_BF16) launch_bwd<bf16_t>(p, half, grid, s); else launch_bwd<float>(p, half, grid, s);
+    launch(p, dtype, half, true, grid, s);
     if (dwq || dwk)
         rope_axes_dw_kernel<<<dim3((unsigned)cdiv(D, 32), 2), NB, 0, s>>>(ws, dwq, dwk, wq_dtype == DPIPE_F32, wk_dtype == DPIPE_F32, accumulate_wq, accumulate_wk, (int)grid, D);
     return check_launch("dpipe_rope_axes_bwd");

@@ -265,6 +265,33 @@ def test_captured_and_replayed_with_other_positions(gpu):
         assert all(torch.equal(x, y) for x, y in zip(out, step())), turn
 
 
+@pytest.mark.parametrize('dtype,interleaved', [(torch.bfloat16, True), (torch.bfloat16, False), (torch.float32, True), (torch.float32, False)], ids=['bf16', 'bf16_halves', 'f32', 'f32_halves'])
+def test_more_than_the_caches_hold(gpu, dtype, interleaved):
+    """heads of more than 256 MB take the kernels that stream past the caches: the same bits as the two halves of the tokens by themselves; the weight's gradient is the sum of the halves'
+    (each fp32 sum off by at most depth F of its terms' absolute sum, see _exact)"""
+    from diffusion_pipe_amd import ops
+    n = 24000 if dtype == torch.bfloat16 else 12000
+    g = torch.Generator(device=gpu).manual_seed(13)
+    q, gq = (torch.randn(n, 40, 128, device=gpu, generator=g).to(dtype) for _ in range(2))
+    k, gk = (torch.randn(n, 8, 128, device=gpu, generator=g).to(dtype) for _ in range(2))
+    assert (q.numel() + k.numel()) * q.element_size() > 2 ** 28 > (q[:n // 2].numel() + k[:n // 2].numel()) * q.element_size()
+    w = (1 + 0.2 * torch.randn(128, device=gpu, generator=g)).requires_grad_(True)
+    pos = _positions(gpu, (n,), 3, torch.float32)
+
+    def step(rows, weight):
+        leaves = [q[rows].detach().requires_grad_(True), k[rows].detach().requires_grad_(True)]
+        y = ops.rope_axes(*leaves, pos[rows], (16, 56, 56), q_weight=weight, k_weight=weight, interleaved=interleaved)
+        return [y[0].detach(), y[1].detach(), *torch.autograd.grad(y, leaves + ([weight] if weight is not None else []), (gq[rows], gk[rows]))]
+    for weight in (w, None):
+        whole, first, second = (step(r, weight) for r in (slice(None), slice(0, n // 2), slice(n // 2, n)))
+        for i in range(4):
+            assert torch.equal(whole[i], torch.cat([first[i], second[i]])), (weight is None, i)
+    whole, first, second = (step(r, w)[4].double() for r in (slice(None), slice(0, n // 2), slice(n // 2, n)))
+    xh = q.float() * torch.rsqrt((q.float() ** 2).mean(-1, keepdim=True) + 1e-6)
+    terms = 2.0 * _pair_size(gq.float(), 128, interleaved).mul_(xh.abs()).sum((0, 1)).double()          # queries' terms, and the fewer keys' within as much again
+    assert ((whole - first - second).abs() <= (n * 40 // 16 // 256 + 600) * F * terms).all()
+
+
 def test_no_tokens(gpu):
     from diffusion_pipe_amd import ops
     q = torch.empty(0, 4, 64, device=gpu).requires_grad_(True)
