@@ -27,7 +27,7 @@ _UNROLL = ['-mllvm', '-pragma-unroll-threshold=200000']
 # without packed fp32 the contraction of their a * b + c changes, and with it results that existing bounds pin.
 _NO_PK_F32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 EXTRA_CFLAGS = {'gemm_pipe.hip': _UNROLL, 'gemm_pipe_group.hip': _UNROLL, 'gemm_pipe_256.hip': _UNROLL, 'conv_pipe.hip': _UNROLL,
-                'rope_axes.hip': _NO_PK_F32, 'attention_varlen.hip': _NO_PK_F32}
+                'rope_axes.hip': _NO_PK_F32, 'attention_varlen.hip': _NO_PK_F32, 'attention_varlen_f32.hip': _NO_PK_F32}
 
 
 def _sources():

@@ -1,4 +1,5 @@
-// attention_varlen.hip -- attention over sequences of different lengths packed back to back, with grouped heads, causal or not, forward + backward; bf16.
+// attention_varlen.hip -- attention over sequences of different lengths packed back to back, with grouped heads, causal or not, forward + backward; bf16 (fp32:
+// attention_varlen_f32.hip, the same contract).
 //
 //   q [Tq, Hq, D], k / v [Tk, Hk, D] (head dim contiguous, D in {64, 128}), sequence b = query tokens cu_q[b] .. cu_q[b + 1] and key tokens cu_k[b] .. cu_k[b + 1];
 //   query head h reads key head h / g, g = Hq / Hk;  o_i = sum_j softmax_j(scale q_i . k_j) v_j;  causal: key j (counted in its sequence) is seen from query i
@@ -19,26 +20,17 @@
 #include "dpipe_common.h"
 #include "lds_dma_tiles.h"
 #include "attention_tiles.h"
+#include "attention_varlen.h"
 #include "../../include/dpipe_hip.h"
 
 using namespace dpipe;
 using namespace dpipe_tiles;
+using namespace dpipe_varlen;
 
 namespace {
 
-struct VarlenParams {
-    const bf16_t *q, *k, *v, *dout;
-    bf16_t *o, *o_lo, *dq, *dk, *dv;     // o_lo: what the rounding of o left, rounded: o + o_lo is the output to 2^-17, which the backward's delta is formed from (forward: may be null)
-    float *lse, *delta;                  // [Hq][Tq]
-    const int *cu_q, *cu_k;
-    float *part, *part_lse;              // split forms: forward rows [split][Tq][Hq][D] and their lse [split][Hq][Tq]; dK / dV [split][2][Tk][Hk][D]
-    long tq, tk;
-    int n, hq, hk, g, nsplit, causal;
-    long q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, do_ss, do_sh;    // o, dq, dk, dv are contiguous
-    float scale;
-};
+typedef VarlenParams<bf16_t> Params;
 
-constexpr int NT = 256, ROWS = 128;       // threads, query rows (dK / dV: keys) of a workgroup: 4 waves of 32
 constexpr int KT = 64;                   // keys (dK / dV: queries) per LDS tile
 constexpr int AQ = 4, AK = 1;            // steps of LDS operands read ahead of their products in the dQ and the dK / dV kernels
 // CORNER: in a row of few keys (a column of few queries) nothing averages the rounding of P and dS away, and the forward's reaches the row's dS through delta.  The forward and dQ
@@ -46,103 +38,6 @@ constexpr int AQ = 4, AK = 1;            // steps of LDS operands read ahead of 
 // in causal sequences carry the largest gradients, are rounded once.  dK / dV do it for the first tile of keys against the first of queries where the sequences average at most one
 // tile (a variant: its registers cost the long ones 8 %, at D = 64 30 %).  Error against 64 bits, dQ / dK / dV, 24 causal sequences of 1 - 2 tokens: 2.53e-3 / 2.32e-3 / 1.82e-3 ->
 // 1.7e-3 each (one rounding); 457 + 16 + 32 + 172 + 208 causal tokens: dQ 2.40e-3 -> 1.8e-3.
-constexpr float M_INIT = -3.0e38f;       // running maximum before the first key: finite, so that exp2(-inf - m) is 0 and never NaN
-constexpr int SORTED = 32;               // sequences up to which their tiles are ordered by work (a forward of 1311 + 2560 + 4608 tokens as packed 378 us, ordered 347; 64 sequences of 128
-                                         // tokens 47 as packed, 72 ordered: the order costs a workgroup up to 90 ns a sequence)
-constexpr float RESCALE_AT = 8.f;        // the accumulator is rescaled when the maximum grew by more than 2^8: P stays below 256, its relative rounding is the same
-
-// ------------------------------------------------------------------------------------------------ which sequence, which rows
-struct Tile { long row0, rows, q0, k0; int lq, lk; bool live; };
-
-// offset i of the ascending sums, kept inside the tensor (i > n: its end)
-__device__ __forceinline__ int bound(const int* cu, int i, int n, int total) {
-    if (i == 0) return 0;
-    if (i > n) return total;
-    const int c = cu[i];
-    return c < 0 ? 0 : c > total ? total : c;
-}
-// slot -> sequence and first row; PER = rows per tile, gg = rows per token on the tiled side.  Up to SORTED sequences (a lane each): the tiles of the sequences with the longest other
-// side first -- the workgroups with the most work start first -- each sequence's tiles from its ascending sum on, the rows behind the last sequence (n) after them.  More sequences:
-// the slots from  start / PER + b  on, in order.  `reversed`: the last tile of a sequence (causal: the one that sees most) first.
-template <int PER>
-__device__ __forceinline__ Tile find_tile(const VarlenParams& p, int slot, bool keys, bool reversed) {
-    const int *cu = keys ? p.cu_k : p.cu_q, *cu2 = keys ? p.cu_q : p.cu_k;
-    const int total = (int)(keys ? p.tk : p.tq), total2 = (int)(keys ? p.tq : p.tk), n = p.n;
-    const int gg = keys ? 1 : p.g, lane = threadIdx.x & 63;
-    int b, at, s0, s1, o0 = 0, o1 = 0;   // sequence, tile of it, its range on the tiled side and on the other (the rows behind the last sequence have no other side)
-    if (n <= SORTED) {
-        const int i0 = min(lane, n - 1);
-        const int my_s0 = bound(cu, i0, n, total), my_s1 = max(my_s0, bound(cu, i0 + 1, n, total)), my_o0 = bound(cu2, i0, n, total2), my_o1 = max(my_o0, bound(cu2, i0 + 1, n, total2));
-        const int nt = lane < n ? ((my_s1 - my_s0) * gg + PER - 1) / PER : 0, work = my_o1 - my_o0;
-        int start = 0, all = 0;
-#pragma unroll 8
-        for (int i = 0; i < ((n + 7) & ~7); ++i) {             // (lanes from n on hold no tiles)
-            const int nt_i = __builtin_amdgcn_readlane(nt, i), work_i = __builtin_amdgcn_readlane(work, i);
-            start += nt_i & -(int)((work_i > work) | ((work_i == work) & (i < lane)));
-            all += nt_i;
-        }
-        const unsigned long long here = __ballot(lane < n && slot >= start && slot < start + nt);
-        b = here ? __builtin_amdgcn_readfirstlane(__builtin_ctzll(here)) : n - 1;
-        s0 = __builtin_amdgcn_readlane(my_s0, b); s1 = __builtin_amdgcn_readlane(my_s1, b);
-        if (here) { at = slot - __builtin_amdgcn_readlane(start, b); o0 = __builtin_amdgcn_readlane(my_o0, b); o1 = __builtin_amdgcn_readlane(my_o1, b); }
-        else { at = slot - all; b = n; s0 = s1; s1 = max(s0, total); }
-    } else {
-        int count = 0;
-        for (int base = 0; base <= n; base += 64) {
-            const int i = base + lane;
-            const int c = __popcll(__ballot(i <= n && (long)bound(cu, i, n, total) * gg / PER + i <= slot));
-            count += c;
-            if (c < 64) break;
-        }
-        b = __builtin_amdgcn_readfirstlane(count - 1);
-        s0 = bound(cu, b, n, total); s1 = max(s0, bound(cu, b + 1, n, total));
-        at = slot - (int)((long)s0 * gg / PER + b);
-        if (b < n) { o0 = bound(cu2, b, n, total2); o1 = max(o0, bound(cu2, b + 1, n, total2)); }
-    }
-    Tile t;
-    t.rows = (long)(s1 - s0) * gg;
-    const int nt = (int)((t.rows + PER - 1) / PER);
-    t.live = at >= 0 && at < nt;         // (offsets that do not ascend reach no row outside their tensor)
-    t.row0 = (long)(reversed ? nt - 1 - at : at) * PER;
-    t.q0 = keys ? o0 : s0; t.k0 = keys ? s0 : o0;
-    t.lq = keys ? o1 - o0 : s1 - s0; t.lk = keys ? s1 - s0 : o1 - o0;
-    return t;
-}
-
-// The lane's query row: token (in the buffer) and query head; `last`: the last key of its sequence it sees (-1: none)
-struct Row { long token, head; int last; bool live; };
-__device__ __forceinline__ Row find_row(const VarlenParams& p, const Tile& t, int kh, int wid, int i) {
-    const long at = t.row0 + 32 * wid + i;
-    Row r;
-    r.live = at < t.rows;
-    const unsigned row = r.live ? (unsigned)at : 0u, tok = row / (unsigned)p.g;
-    r.token = t.q0 + tok; r.head = (long)kh * p.g + (row - tok * p.g);
-    r.last = p.causal ? (int)min((long)tok + t.lk - t.lq, (long)t.lk - 1) : t.lk - 1;
-    return r;
-}
-// How many keys (from the first on) some row of the workgroup sees, some row of the wave, every live row of the wave
-struct Seen { int group, wave, all; };
-__device__ __forceinline__ Seen keys_seen(const VarlenParams& p, const Tile& t, int wid) {
-    const long r0 = t.row0 + 32 * wid, last = min(t.row0 + ROWS, t.rows) - 1, wlast = min(r0 + 32, t.rows) - 1;
-    if (!p.causal) return {t.lk, wlast < r0 ? 0 : t.lk, t.lk};
-    auto upto = [&](long row) { return (int)max(0l, min((long)t.lk, row / p.g + t.lk - t.lq + 1)); };
-    return {upto(last), wlast < r0 ? 0 : upto(wlast), wlast < r0 ? 0 : upto(r0)};
-}
-
-// Workgroup id -> (key head, slot, part).  Consecutive ids go round the 8 XCDs, each with an L2 of its own: an XCD gets whole key heads, or every c-th slot of one when the heads
-// are not a multiple of 8 -- the tiles that stream one head's rows share an L2, and long and short sequences (causal: early and late tiles) are spread evenly over the XCDs.
-struct Work { int head, slot, part; };
-__host__ __device__ __forceinline__ int xcd_classes(int heads) { return heads % 8 == 0 ? 1 : heads % 4 == 0 ? 2 : heads % 2 == 0 ? 4 : 8; }
-__host__ __device__ __forceinline__ long work_groups(long slots, int heads, int parts) { const int c = xcd_classes(heads); return (slots + c - 1) / c * c * heads * parts; }
-__device__ __forceinline__ Work find_work(int id, int heads, int parts) {
-    const int c = xcd_classes(heads), units = heads * c / 8;  // (head, slot class) pairs per XCD
-    int j = id / 8;
-    Work w;
-    w.part = j % parts; j /= parts;
-    const int unit = id % 8 * units + j % units;
-    w.head = unit / c; w.slot = j / units * c + unit % c;
-    return w;
-}
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, long bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
@@ -227,15 +122,6 @@ __device__ __forceinline__ bf16x8_t pack_rest(const f32x16& s, int e0) {
     return __builtin_bit_cast(bf16x8_t, make_uint4(r[0], r[1], r[2], r[3]));
 }
 
-__device__ __forceinline__ float max_halves(float x) {        // max over lane and lane ^ 32, in both
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_halves(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // 32 channels of a lane's row from a transposed accumulator (the lane holds channels 8 e + 4 h + 0 .. 3): halves exchanged with lane ^ 32, two 16-byte stores a lane.
 // `lo`: where the rounding's remainders go (null: nowhere)
 __device__ __forceinline__ void store_row(bf16_t* dst, bf16_t* lo, const f32x16& a, float scale, int h) {
@@ -260,7 +146,7 @@ __device__ __forceinline__ void store_row(bf16_t* dst, bf16_t* lo, const f32x16&
 // ================================================================================================ forward
 // 128 rows per workgroup of 4 waves, two workgroups per CU: one's softmax runs under the other's products without a barrier between them.
 template <int D, bool SPLIT>
-__global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const VarlenParams p) {
+__global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const Params p) {
     constexpr int NKS = D / 16, NDB = D / 32, IMG = KT * D * 2, STAGE = 2 * IMG;
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
     const Work w = find_work(blockIdx.x, p.hk, SPLIT ? p.nsplit : 1);
@@ -368,50 +254,10 @@ __global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const VarlenParams p)
     }
 }
 
-// joins the parts of a row: o = sum_s 2^(lse_s - top) o_s / sum_s 2^(lse_s - top); one wave per row, its lanes hold the parts' weights (nsplit <= 64), then D / 64 channels each
-template <int D>
-__global__ void __launch_bounds__(NT) varlen_join_kernel(const VarlenParams p) {
-    constexpr int C = D / 64;
-    const long rows = p.tq * p.hq, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const int lane = threadIdx.x & 63;
-    const long tok = row / p.hq, at = (row - tok * p.hq) * p.tq + tok;
-    const float ls = lane < p.nsplit ? p.part_lse[lane * rows + at] : -INFINITY;
-    const float top = wave_max(ls), base = top == -INFINITY ? 0.f : top;
-    const float w = __builtin_amdgcn_exp2f(ls - base), sum = wave_sum(w);
-    float a[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) a[c] = 0.f;
-    for (int s0 = 0; s0 < p.nsplit; s0 += 16) {                // 16 parts' reads in flight
-        float v[16][C];
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-#pragma unroll
-            for (int c = 0; c < C; ++c) v[j][c] = p.part[(min(s0 + j, p.nsplit - 1) * rows + row) * D + lane * C + c];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {                         // a part that saw nothing has stored nothing: what is read there does not count
-            const int s = min(s0 + j, 63);
-            const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
-            const bool stored = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ls), s)) != -INFINITY;      // (lanes from nsplit on hold -inf)
-#pragma unroll
-            for (int c = 0; c < C; ++c) a[c] += stored ? ws * v[j][c] : 0.f;
-        }
-    }
-    const float inv = sum > 0.f ? 1.f / sum : sum;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        a[c] *= inv;
-        const bf16_t hi = f32_to_bf16(a[c]);
-        p.o[row * D + lane * C + c] = hi;
-        if (p.o_lo) p.o_lo[row * D + lane * C + c] = f32_to_bf16(a[c] - bf16_to_f32(hi));
-    }
-    if (lane == 0 && p.lse) p.lse[at] = sum == 0.f ? INFINITY : base + __builtin_amdgcn_logf(sum);
-}
-
 // ================================================================================================ backward: dQ (and delta)
 // Per 64-key tile: K, read by rows (S^T = K . Q^T) and transposed (dQ^T += K^T . dS^T), and V by rows (dP^T = V . dO^T).
 template <int D>
-__global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const VarlenParams p) {
+__global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
     constexpr int NKS = D / 16, NDB = D / 32, IMG = KT * D * 2, STAGE = 2 * IMG;
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
     const Work w = find_work(blockIdx.x, p.hk, 1);
@@ -500,7 +346,7 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const VarlenParams p) 
 // Key-outer; a lane owns one key column, K stays in LDS, V and both accumulators in registers:  S = Q . K^T, dP = dO . V^T, dV^T += dO^T . P, dK^T += Q^T . dS.  Per 64-query tile Q and dO, both read by rows and transposed, and the
 // tile's lse / delta.  Query rows past the sequence arrive as zeros (Q, dO, lse, delta): P = 1 there, but dO = 0 and dS = 0.
 template <int D, int NW, bool CORNER>
-__global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dkv_kernel(const VarlenParams p) {
+__global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dkv_kernel(const Params p) {
     constexpr int QT = KT, NKS = D / 16, NDB = D / 32, IMG = QT * D * 2, O_STAT = 2 * IMG, STAGE = O_STAT + 1024;
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE + NW / 2 * IMG];
     const Work w = find_work(blockIdx.x, p.hk, p.nsplit);
@@ -623,24 +469,7 @@ __global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dk
     }
 }
 
-// dK / dV = sum of the parts in order, one thread per 4 channels
-__global__ void __launch_bounds__(256) varlen_dkv_sum_kernel(const VarlenParams p, long elements) {
-    const long at = 4 * ((long)blockIdx.x * 256 + threadIdx.x);
-    if (at >= elements) return;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
-#pragma unroll 4
-    for (int s = 0; s < p.nsplit; ++s) {
-        const float4 x = *reinterpret_cast<const float4*>(p.part + 2 * s * elements + at), y = *reinterpret_cast<const float4*>(p.part + (2 * s + 1) * elements + at);
-        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w; c.x += y.x; c.y += y.y; c.z += y.z; c.w += y.w;
-    }
-    *reinterpret_cast<uint2*>(p.dk + at) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
-    *reinterpret_cast<uint2*>(p.dv + at) = make_uint2(pack_bf16x2(c.x, c.y), pack_bf16x2(c.z, c.w));
-}
-
 // ------------------------------------------------------------------------------------------------ host side
-int row_slots(long tokens, int g, int n, int per) { return (int)(tokens * g / per + n + 1); }
-
-
 // parts of the key range: when the row tiles alone leave CUs idle, enough parts for two workgroups per CU, of at least 4 key tiles of an average sequence each
 int fwd_splits(long tq, long tk, int n, int hq, int hk) {
     const long wgs = cdiv(tq * (hq / hk), ROWS) * hk, tiles = tk / n / KT;
@@ -665,7 +494,8 @@ bool rows_ok(const void* p, long ss, long sh, int D) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ss % 8 == 0 && sh % 8 == 0 && ss >= D && ss < (1l << 23) && sh >= 0;
 }
 
-int fill(VarlenParams& p, const char* what, const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, long tq, long tk, int n, int hq, int hk, int D, long q_ss,
+template <typename T>
+int fill(VarlenParams<T>& p, const char* what, const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, long tq, long tk, int n, int hq, int hk, int D, long q_ss,
          long q_sh, long k_ss, long k_sh, long v_ss, long v_sh, float scale, int causal) {
     auto bad = [&](const char* m, int rc = DPIPE_ERR_ARG) { char buf[160]; snprintf(buf, sizeof(buf), "%s: %s", what, m); set_last_error(buf); return rc; };
     if (!q || !k || !v || !cu_q || !cu_k || tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk) return bad("bad argument");
@@ -675,24 +505,24 @@ int fill(VarlenParams& p, const char* what, const void* q, const void* k, const 
     if (tq * (hq / hk) >= (1l << 31) - 256 || tk >= (1l << 31) - 256 || work_groups(tq * (hq / hk) / ROWS + n + 1, hk, fs) >= (1l << 23) || work_groups(tk / ROWS + n + 1, hk, bs) >= (1l << 23))
         return bad("too many rows or sequences", DPIPE_ERR_UNSUPPORTED);
     if (!rows_ok(q, q_ss, q_sh, D) || !rows_ok(k, k_ss, k_sh, D) || !rows_ok(v, v_ss, v_sh, D)) return bad("tensors must be 16-byte aligned with strides multiple of 8 elements");
-    p.q = (const bf16_t*)q; p.k = (const bf16_t*)k; p.v = (const bf16_t*)v; p.cu_q = cu_q; p.cu_k = cu_k; p.tq = tq; p.tk = tk; p.n = n; p.hq = hq; p.hk = hk; p.g = hq / hk;
+    p.q = (const T*)q; p.k = (const T*)k; p.v = (const T*)v; p.cu_q = cu_q; p.cu_k = cu_k; p.tq = tq; p.tk = tk; p.n = n; p.hq = hq; p.hk = hk; p.g = hq / hk;
     p.q_ss = q_ss; p.q_sh = q_sh; p.k_ss = k_ss; p.k_sh = k_sh; p.v_ss = v_ss; p.v_sh = v_sh; p.scale = scale; p.causal = causal != 0; p.nsplit = 1;
     return DPIPE_OK;
 }
 
-template <int D> void forward(const VarlenParams& p, hipStream_t s) {
+template <int D> void forward(const Params& p, hipStream_t s) {
     const unsigned grid = (unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, p.nsplit);
     if (p.nsplit == 1) { varlen_fwd_kernel<D, false><<<grid, NT, 0, s>>>(p); return; }
     varlen_fwd_kernel<D, true><<<grid, NT, 0, s>>>(p);
-    varlen_join_kernel<D><<<(unsigned)cdiv(p.tq * p.hq, 4), NT, 0, s>>>(p);
+    varlen_join_kernel<bf16_t, D><<<(unsigned)cdiv(p.tq * p.hq, 4), NT, 0, s>>>(p);
 }
-template <int D> void backward(VarlenParams& p, int parts, hipStream_t s) {
+template <int D> void backward(Params& p, int parts, hipStream_t s) {
     varlen_dq_kernel<D><<<(unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, 1), NT, 0, s>>>(p);
     p.nsplit = parts;
     constexpr int NW = key_tile(D) / 32;
     const unsigned grid = (unsigned)work_groups(row_slots(p.tk, 1, p.n, 32 * NW), p.hk, parts);
     if (p.tk / p.n <= KT) varlen_dkv_kernel<D, NW, true><<<grid, 64 * NW, 0, s>>>(p); else varlen_dkv_kernel<D, NW, false><<<grid, 64 * NW, 0, s>>>(p);
-    if (parts > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
+    if (parts > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<bf16_t><<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
 }
 
 }  // namespace
@@ -711,35 +541,51 @@ long dpipe_attn_varlen_bwd_workspace_floats(long tq, long tk, int n, int hq, int
 }
 
 int dpipe_attn_varlen_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, void* o_lo, float* lse, float* ws, long ws_floats, long tq,
-                          long tk, int n, int hq, int hk, int D, long q_ss, long q_sh, long k_ss, long k_sh, long v_ss, long v_sh, float scale, int causal, void* stream) {
-    VarlenParams p = {};
-    const int rc = fill(p, "dpipe_attn_varlen_fwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal);
-    if (rc) return rc;
-    const long need = dpipe_attn_varlen_fwd_workspace_floats(tq, tk, n, hq, hk, D);
-    if (!o || !aligned16(o) || !aligned16(o_lo) || (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) {
-        set_last_error("dpipe_attn_varlen_fwd: bad output or workspace"); return DPIPE_ERR_ARG; }
-    if (ablated(ABL_ATTN)) return DPIPE_OK;
-    p.o = (bf16_t*)o; p.o_lo = (bf16_t*)o_lo; p.lse = lse;
-    if (need > 0) { p.nsplit = fwd_splits(tq, tk, n, hq, hk); p.part = ws; p.part_lse = ws + (long)p.nsplit * tq * hq * D; }
-    if (D == 64) forward<64>(p, reinterpret_cast<hipStream_t>(stream)); else forward<128>(p, reinterpret_cast<hipStream_t>(stream));
-    return check_launch("dpipe_attn_varlen_fwd");
+                          long tk, int n, int hq, int hk, int D, long q_ss, long q_sh, long k_ss, long k_sh, long v_ss, long v_sh, float scale, int causal, int dtype, void* stream) {
+    auto run = [&](auto type, auto launch) {
+        typedef decltype(type) T;
+        VarlenParams<T> p = {};
+        const int rc = fill(p, "dpipe_attn_varlen_fwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal);
+        if (rc) return rc;
+        const long need = dpipe_attn_varlen_fwd_workspace_floats(tq, tk, n, hq, hk, D);
+        if (!o || !aligned16(o) || !aligned16(o_lo) || (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) {
+            set_last_error("dpipe_attn_varlen_fwd: bad output or workspace"); return DPIPE_ERR_ARG; }
+        if (ablated(ABL_ATTN)) return DPIPE_OK;
+        p.o = (T*)o; p.o_lo = sizeof(T) == 2 ? (T*)o_lo : nullptr; p.lse = lse;
+        if (need > 0) { p.nsplit = fwd_splits(tq, tk, n, hq, hk); p.part = ws; p.part_lse = ws + (long)p.nsplit * tq * hq * D; }
+        launch(p);
+        return check_launch("dpipe_attn_varlen_fwd");
+    };
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (dtype == DPIPE_BF16) return run(bf16_t{}, [&](auto& p) { if (D == 64) forward<64>(p, s); else forward<128>(p, s); });
+    if (dtype == DPIPE_F32) return run(float{}, [&](auto& p) { forward_f32(p, D, s); });
+    set_last_error("dpipe_attn_varlen_fwd: dtype must be bf16 or fp32");
+    return DPIPE_ERR_UNSUPPORTED;
 }
 
 int dpipe_attn_varlen_bwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, const void* o, const void* o_lo, const void* dout, const float* lse, float* delta,
                           void* dq, void* dk, void* dv, float* ws, long ws_floats, long tq, long tk, int n, int hq, int hk, int D, long q_ss, long q_sh, long k_ss, long k_sh,
-                          long v_ss, long v_sh, long do_ss, long do_sh, float scale, int causal, void* stream) {
-    VarlenParams p = {};
-    const int rc = fill(p, "dpipe_attn_varlen_bwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal);
-    if (rc) return rc;
-    const long need = dpipe_attn_varlen_bwd_workspace_floats(tq, tk, n, hq, hk, D);
-    if (!o || !o_lo || !dout || !lse || !delta || !dq || !dk || !dv || !aligned16(o) || !aligned16(o_lo) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !rows_ok(dout, do_ss, do_sh, D) ||
-        (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) { set_last_error("dpipe_attn_varlen_bwd: bad gradient or workspace"); return DPIPE_ERR_ARG; }
-    if (ablated(ABL_ATTN)) return DPIPE_OK;
-    p.o = (bf16_t*)o; p.o_lo = (bf16_t*)o_lo; p.dout = (const bf16_t*)dout; p.lse = const_cast<float*>(lse); p.delta = delta;
-    p.dq = (bf16_t*)dq; p.dk = (bf16_t*)dk; p.dv = (bf16_t*)dv; p.do_ss = do_ss; p.do_sh = do_sh; p.part = ws;
-    const int splits = need > 0 ? dkv_splits(tq, tk, n, hq, hk, D) : 1;
-    if (D == 64) backward<64>(p, splits, reinterpret_cast<hipStream_t>(stream)); else backward<128>(p, splits, reinterpret_cast<hipStream_t>(stream));
-    return check_launch("dpipe_attn_varlen_bwd");
+                          long v_ss, long v_sh, long do_ss, long do_sh, float scale, int causal, int dtype, void* stream) {
+    auto run = [&](auto type, auto launch) {
+        typedef decltype(type) T;
+        VarlenParams<T> p = {};
+        const int rc = fill(p, "dpipe_attn_varlen_bwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal);
+        if (rc) return rc;
+        const long need = dpipe_attn_varlen_bwd_workspace_floats(tq, tk, n, hq, hk, D);
+        if (!o || (sizeof(T) == 2 && !o_lo) || !dout || !lse || !delta || !dq || !dk || !dv || !aligned16(o) || !aligned16(o_lo) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
+            !rows_ok(dout, do_ss, do_sh, D) || (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) {
+            set_last_error("dpipe_attn_varlen_bwd: bad gradient or workspace"); return DPIPE_ERR_ARG; }
+        if (ablated(ABL_ATTN)) return DPIPE_OK;
+        p.o = (T*)o; p.o_lo = (T*)o_lo; p.dout = (const T*)dout; p.lse = const_cast<float*>(lse); p.delta = delta;
+        p.dq = (T*)dq; p.dk = (T*)dk; p.dv = (T*)dv; p.do_ss = do_ss; p.do_sh = do_sh; p.part = ws;
+        launch(p, need > 0 ? dkv_splits(tq, tk, n, hq, hk, D) : 1);
+        return check_launch("dpipe_attn_varlen_bwd");
+    };
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (dtype == DPIPE_BF16) return run(bf16_t{}, [&](auto& p, int parts) { if (D == 64) backward<64>(p, parts, s); else backward<128>(p, parts, s); });
+    if (dtype == DPIPE_F32) return run(float{}, [&](auto& p, int parts) { backward_f32(p, D, parts, s); });
+    set_last_error("dpipe_attn_varlen_bwd: dtype must be bf16 or fp32");
+    return DPIPE_ERR_UNSUPPORTED;
 }
 
 }  // extern "C"

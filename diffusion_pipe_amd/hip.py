@@ -105,9 +105,9 @@ _SIGNATURES = {
     'dpipe_attn_bwd_partial_floats': (L, [I, I, I, I, I]),
     'dpipe_attn_bwd': (I, [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I] + [L] * 24 + [F, I, P, L, P, P]),
     'dpipe_attn_varlen_fwd_workspace_floats': (L, [L, L, I, I, I, I]),
-    'dpipe_attn_varlen_fwd': (I, [P] * 9 + [L, L, L, I, I, I, I] + [L] * 6 + [F, I, P]),
+    'dpipe_attn_varlen_fwd': (I, [P] * 9 + [L, L, L, I, I, I, I] + [L] * 6 + [F, I, I, P]),
     'dpipe_attn_varlen_bwd_workspace_floats': (L, [L, L, I, I, I, I]),
-    'dpipe_attn_varlen_bwd': (I, [P] * 14 + [L, L, L, I, I, I, I] + [L] * 8 + [F, I, P]),
+    'dpipe_attn_varlen_bwd': (I, [P] * 14 + [L, L, L, I, I, I, I] + [L] * 8 + [F, I, I, P]),
     'dpipe_rope_axes_fwd': (I, [P, P, P, I, P, P, P, P, P, P, L, L, I, I, I, I, I] + [L] * 4 + [F, I, I, I, I, P]),
     'dpipe_rope_axes_workspace_floats': (L, [I]),
     'dpipe_rope_axes_bwd': (I, [P, P, P, P, P, I] + [P] * 9 + [L, L, I, I, I, I, I] + [L] * 8 + [F] + [I] * 6 + [P]),

@@ -1785,16 +1785,17 @@ def _varlen_forward(q, k, v, cu_q, cu_k, scale, causal, keep):
         return torch.zeros(q.shape, device=device, dtype=q.dtype), (), None
     sizes, strides = (tq, tk, cu_q.shape[0] - 1, hq, hk, D), (*qs, *ks, *vs)
     o = _dense(q)
-    o_lo, lse = (torch.empty_like(o), q.new_empty((hq, tq), dtype=torch.float32)) if keep else (None, None)
+    dt = dtype_code(q.dtype)
+    o_lo, lse = (torch.empty_like(o) if dt == hip.BF16 else None, q.new_empty((hq, tq), dtype=torch.float32)) if keep else (None, None)
     need = lib().dpipe_attn_varlen_fwd_workspace_floats(*sizes)
     ws = torch.empty(need, device=device, dtype=torch.float32) if need else None
     check(lib().dpipe_attn_varlen_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _addr(o_lo), _addr(lse), _addr(ws), need, *sizes,
-                                      *strides, scale, causal, hip.raw_stream(device)), 'attn_varlen_fwd')
-    return o, (q, k, v, cu_q, cu_k, o, o_lo, lse), (sizes, strides, scale, causal)
+                                      *strides, scale, causal, dt, hip.raw_stream(device)), 'attn_varlen_fwd')
+    return o, (q, k, v, cu_q, cu_k, o, o_lo, lse), (sizes, strides, scale, causal, dt)
 
 
 class _AttnVarlenFn(Function):
-    """see attention_varlen; keeps the output to 16 bits of significand (o and what its rounding left) for the backward's delta, where _FlashAttnFn keeps an fp32 copy"""
+    """see attention_varlen; keeps the bf16 output to 16 bits of significand (o and what its rounding left) for the backward's delta, where _FlashAttnFn keeps an fp32 copy"""
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale, causal):
@@ -1810,21 +1811,21 @@ class _AttnVarlenFn(Function):
             *shapes, dtype = ctx.shapes
             return (*(torch.zeros(sh, device=device, dtype=dtype) for sh in shapes), None, None, None, None)
         q, k, v, cu_q, cu_k, o, o_lo, lse = ctx.saved_tensors
-        sizes, strides, scale, causal = ctx.call
+        sizes, strides, scale, causal, dt = ctx.call
         with _on(device):
             do, _, _, _, *ds = _head_rows(do)
             dq, dk, dv = _dense(q), _dense(k), _dense(v)
             delta = torch.empty_like(lse)
             need = lib().dpipe_attn_varlen_bwd_workspace_floats(*sizes)
             ws = torch.empty(need, device=device, dtype=torch.float32) if need else None
-            check(lib().dpipe_attn_varlen_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), o_lo.data_ptr(), do.data_ptr(), lse.data_ptr(),
+            check(lib().dpipe_attn_varlen_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _addr(o_lo), do.data_ptr(), lse.data_ptr(),
                                               delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _addr(ws), need, *sizes, *strides, *ds, scale, causal,
-                                              hip.raw_stream(device)), 'attn_varlen_bwd')
+                                              dt, hip.raw_stream(device)), 'attn_varlen_bwd')
         return dq, dk, dv, None, None, None, None
 
 
 def attention_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=False):
-    """softmax(scale q k^T) v over sequences of different lengths packed back to back; bf16, head dim 64 or 128, differentiable in q, k, v.
+    """softmax(scale q k^T) v over sequences of different lengths packed back to back; bf16, or fp32 throughout, head dim 64 or 128, differentiable in q, k, v.
 
     q [Tq, H, D], k / v [Tk, Hk, D] with H a multiple of Hk: query head h reads key head h // (H // Hk).  Column blocks of a fused projection are read in place.
     cu_q, cu_k: int32 offsets [N + 1] on the device, ascending from 0; sequence b holds query tokens cu_q[b] .. cu_q[b + 1] - 1 and key tokens cu_k[b] .. cu_k[b + 1] - 1, either
@@ -1837,8 +1838,8 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=False):
     qs, ks, dtype = q.shape, k.shape, q.dtype
     if len(qs) != 3 or len(ks) != 3 or ks != v.shape or ks[2] != qs[2] or ks[1] == 0 or qs[1] == 0 or qs[1] % ks[1]:
         raise DpipeHipError(f'attention_varlen: q [Tq, H, D], k and v [Tk, Hk, D] with H a multiple of Hk; got {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}')
-    if not flash_eligible(dtype, qs[2]) or k.dtype != dtype or v.dtype != dtype:
-        raise DpipeHipError(f'attention_varlen computes in bf16 at head dim 64 or 128; got {dtype}, {k.dtype}, {v.dtype}, head dim {qs[2]}')
+    if dtype not in (torch.bfloat16, torch.float32) or qs[2] not in (64, 128) or k.dtype != dtype or v.dtype != dtype:
+        raise DpipeHipError(f'attention_varlen computes in bf16 or fp32 at head dim 64 or 128; got {dtype}, {k.dtype}, {v.dtype}, head dim {qs[2]}')
     for cu in (cu_q, cu_k):
         if cu.dtype not in (torch.int32, torch.int64) or cu.dim() != 1 or cu.shape[0] < 2 or cu.shape[0] != cu_q.shape[0]:
             raise DpipeHipError(f'attention_varlen: offsets are int32 [N + 1], N >= 1, for queries and keys alike; got {cu.dtype} {tuple(cu.shape)}, {tuple(cu_q.shape)}')

@@ -378,20 +378,20 @@ int dpipe_attn_bwd(const void* q, const void* k, const void* v, const void* o, c
 
 /* ---- (ABI 11) attention over sequences of different lengths packed back to back (models/wan/attention.py:91-122 flash_attn_varlen_func; the joint attention over
  * [image ; text] of HunyuanVideo, models/hunyuan_video.py, hands it cu_seqlens), with grouped heads, causal or not
- * q [tq, hq, D], k / v [tk, hk, D] bf16, hq a multiple of hk (query head h reads key head h / (hq / hk)), token / head strides in elements, head dim contiguous, D in {64, 128}.
+ * q [tq, hq, D], k / v [tk, hk, D] of one dtype (bf16 or fp32), hq a multiple of hk (query head h reads key head h / (hq / hk)), token / head strides in elements, head dim contiguous, D in {64, 128}.
  * cu_q, cu_k: device int32 [n + 1], ascending from 0: sequence b = query tokens cu_q[b] .. cu_q[b + 1] - 1 and key tokens cu_k[b] .. cu_k[b + 1] - 1; either may be empty.
  * causal: query i sees key j of its sequence when j - len_k <= i - len_q (the last query sees every key).  A query that sees nothing and the rows behind cu_q[n] get o = 0.
- * o [tq, hq, D] bf16 contiguous; lse [hq, tq] fp32 in log2 units (+inf: nothing seen) and o_lo [tq, hq, D] bf16, what the
+ * o [tq, hq, D] contiguous; lse [hq, tq] fp32 in log2 units (+inf: nothing seen) and, with bf16, o_lo [tq, hq, D] bf16, what the
  * rounding of o left (the backward's delta = rowsum(dO . (o + o_lo)) must not carry that rounding: see dpipe_attn_fwd): kept for the backward, which needs both (NULL: not kept).
  * ws: ..._workspace_floats() fp32, 16-byte aligned, contents irrelevant (0 floats: may be NULL).  Wrong offsets (not ascending, past the end) are clamped to the tensors. */
 long dpipe_attn_varlen_fwd_workspace_floats(long tq, long tk, int n, int hq, int hk, int D);
 int dpipe_attn_varlen_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, void* o_lo, float* lse, float* ws, long ws_floats, long tq,
-                          long tk, int n, int hq, int hk, int D, long q_ss, long q_sh, long k_ss, long k_sh, long v_ss, long v_sh, float scale, int causal, void* stream);
-/* dq [tq, hq, D], dk / dv [tk, hk, D] bf16 contiguous, every row written; delta [hq, tq] fp32 scratch.  No atomics: the same inputs give the same bits. */
+                          long tk, int n, int hq, int hk, int D, long q_ss, long q_sh, long k_ss, long k_sh, long v_ss, long v_sh, float scale, int causal, int dtype, void* stream);
+/* dq [tq, hq, D], dk / dv [tk, hk, D] contiguous, every row written; delta [hq, tq] fp32 scratch.  No atomics: the same inputs give the same bits. */
 long dpipe_attn_varlen_bwd_workspace_floats(long tq, long tk, int n, int hq, int hk, int D);
 int dpipe_attn_varlen_bwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, const void* o, const void* o_lo, const void* dout, const float* lse, float* delta,
                           void* dq, void* dk, void* dv, float* ws, long ws_floats, long tq, long tk, int n, int hq, int hk, int D, long q_ss, long q_sh, long k_ss, long k_sh,
-                          long v_ss, long v_sh, long do_ss, long do_sh, float scale, int causal, void* stream);
+                          long v_ss, long v_sh, long do_ss, long do_sh, float scale, int causal, int dtype, void* stream);
 
 /* ---- (ABI 11) rotary positions with several axes on query and key heads in one launch, with their per-head RMS norms (models/wan/model.py:40-67 rope_apply over (frame, height,
  * width); diffusers FluxPosEmbed + apply_rotary_emb behind models/flux.py; hyvideo get_nd_rotary_pos_embed behind models/hunyuan_video.py:35-81)

@@ -8,7 +8,9 @@ Bounds, element by element, from the roundings the kernels make (h = 2^-8: half 
                                each term off by |dO| times o's first bound above:  + P rowsum |dO| (h + r) sum P |V|                    =: E
     dQ  = scale dS K           dS as above, result rounded:                       scale E |K| + h |dQ|;      dK: scale E^T |Q| + h |dK|
 fp32 parts: a sum of D <= 128 products is off by at most 2^7 2^-24 of its terms' absolute sum (g = 2^-16 with room for both sums); a score's error moves P by
-|error| relatively: |scale q . k| 2^-16 <= 2^-10 for the |scores| <= 64 of these inputs, and sums over keys add 2^-24 a term: P itself carries r = 2^-10 relatively."""
+|error| relatively: |scale q . k| 2^-16 <= 2^-10 for the |scores| <= 64 of these inputs, and sums over keys add 2^-24 a term: P itself carries r = 2^-10 relatively.
+In fp32 (h = 2^-24, nothing rounded but results) r is taken row by row: a row's scores are off by 2^-16 of scale |q| . |k| at most, P and its normalizer each by the largest of
+these, and every sum over n queries of g heads or m keys adds 2^-24 a term, the exponential and the joins less than 2^7 2^-24:  r = 2^-15 max_j scale |q| . |k_j| + (g n + m + 2^7) 2^-24."""
 import math
 
 import pytest
@@ -18,17 +20,19 @@ pytestmark = pytest.mark.gpu
 H_BF16, G_DOT, R_P = 2.0 ** -8, 2.0 ** -16, 2.0 ** -10
 
 
-def _inputs(gpu, lens_q, lens_k, H, Hk, D, seed=0, tail_q=0, tail_k=0, spread=1.0):
+def _inputs(gpu, lens_q, lens_k, H, Hk, D, seed=0, tail_q=0, tail_k=0, spread=1.0, dtype=torch.bfloat16):
     g = torch.Generator().manual_seed(seed + 31 * sum(lens_q) + sum(lens_k) + H)
     tq, tk = sum(lens_q) + tail_q, sum(lens_k) + tail_k
     q, k, v, do = (torch.randn(n, h, D, generator=g) for n, h in ((tq, H), (tk, Hk), (tk, Hk), (tq, H)))
-    q, k, v, do = ((t * s).to(gpu, torch.bfloat16) for t, s in ((q, spread), (k, spread), (v + 0.5, 1.0), (do, 1.0)))
+    q, k, v, do = ((t * s).to(gpu, dtype) for t, s in ((q, spread), (k, spread), (v + 0.5, 1.0), (do, 1.0)))
     cu = [torch.tensor([0] + [sum(lens[:i + 1]) for i in range(len(lens))], dtype=torch.int32, device=gpu) for lens in (lens_q, lens_k)]
     return q, k, v, do, cu[0], cu[1]
 
 
 def _exact(q, k, v, do, lens_q, lens_k, causal, scale):
     """{name: (value, bound)} in fp64"""
+    fp32 = q.dtype == torch.float32
+    u = 2.0 ** -24 if fp32 else H_BF16
     q, k, v, do = (t.detach().double() for t in (q, k, v, do))
     H, Hk = q.shape[1], k.shape[1]
     val = {n: torch.zeros_like(t) for n, t in (('o', q), ('dq', q), ('dk', k), ('dv', v))}
@@ -46,22 +50,25 @@ def _exact(q, k, v, do, lens_q, lens_k, causal, scale):
             O = P @ V
             dP, delta = G @ V.t(), (G * O).sum(-1, keepdim=True)
             dS = P * (dP - delta)
-            E = (H_BF16 + R_P) * dS.abs() + G_DOT * P * (G.abs() @ V.abs().t() + (G.abs() * O.abs()).sum(-1, keepdim=True))
-            E = E + P * (G.abs() * ((H_BF16 + R_P) * (P @ V.abs()))).sum(-1, keepdim=True)
-            val['o'][a:a + n, h], err['o'][a:a + n, h] = O, (H_BF16 + R_P) * (P @ V.abs())
+            r = R_P
+            if fp32:
+                r = 2.0 ** -24 * (H // Hk * n + m + 128) + (2.0 ** -15 * scale * (Q.abs() @ K.abs().t()).amax(-1, keepdim=True) if m else 0.0)
+            E = (u + r) * dS.abs() + G_DOT * P * (G.abs() @ V.abs().t() + (G.abs() * O.abs()).sum(-1, keepdim=True))
+            E = E + P * (G.abs() * ((u + r) * (P @ V.abs()))).sum(-1, keepdim=True)
+            val['o'][a:a + n, h], err['o'][a:a + n, h] = O, (u + r) * (P @ V.abs())
             val['dq'][a:a + n, h], err['dq'][a:a + n, h] = scale * dS @ K, scale * E @ K.abs()
             val['dk'][b:b + m, kh] += scale * dS.t() @ Q
             err['dk'][b:b + m, kh] += scale * E.t() @ Q.abs()
             val['dv'][b:b + m, kh] += P.t() @ G
-            err['dv'][b:b + m, kh] += (H_BF16 + R_P) * (P.t() @ G.abs())
+            err['dv'][b:b + m, kh] += ((u + r) * P).t() @ G.abs()
         a, b = a + n, b + m
-    return {n: (val[n], err[n] + H_BF16 * (val[n].abs() + err[n]) + 1e-30) for n in val}
+    return {n: (val[n], err[n] + u * (val[n].abs() + err[n]) + 1e-30) for n in val}
 
 
-def _check(got, want, label):
+def _check(got, want, label, dtype=torch.bfloat16):
     for name, t in got.items():
         value, bound = want[name]
-        assert t.shape == value.shape and t.dtype == torch.bfloat16
+        assert t.shape == value.shape and t.dtype == dtype
         ratio = ((t.detach().double() - value).abs() / bound).max().item() if t.numel() else 0.0
         print(f'{label} {name}: worst error / bound {ratio:.3f}')
         assert ratio <= 1.0, (label, name, ratio)          # (a NaN fails too)
@@ -105,30 +112,42 @@ def test_forward_and_gradients(gpu, case, D):
 
 
 @pytest.mark.parametrize('D', [64, 128])
-def test_few_rows_against_long_keys(gpu, D):
+@pytest.mark.parametrize('case', CASES, ids=lambda c: f'{"_".join(map(str, c[0][:5]))}x{len(c[0])}_{c[2]}h{c[3]}{"_causal" if c[4] else ""}{"_cross" if c[1] else ""}')
+def test_fp32_forward_and_gradients(gpu, case, D):
+    lens_q, lens_k, H, Hk, causal = case
+    data = _inputs(gpu, lens_q, lens_k or lens_q, H, Hk, D, dtype=torch.float32)
+    got = _run(*data[:5], data[5] if lens_k else None, causal)
+    _check(got, _exact(*data[:4], lens_q, lens_k or lens_q, causal, 1.0 / math.sqrt(D)), f'fp32 {case} D={D}', torch.float32)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+@pytest.mark.parametrize('D', [64, 128])
+def test_few_rows_against_long_keys(gpu, D, dtype):
     """the key range is split over workgroups and joined; some sequences are shorter than the parts"""
     lens_q, lens_k = [1, 3, 1, 1], [9001, 4096, 63, 1]
-    data = _inputs(gpu, lens_q, lens_k, 16, 4, D)
+    data = _inputs(gpu, lens_q, lens_k, 16, 4, D, dtype=dtype)
     from diffusion_pipe_amd import hip
     assert hip.lib().dpipe_attn_varlen_fwd_workspace_floats(data[0].shape[0], data[1].shape[0], 4, 16, 4, D) > 0
     for causal in (True, False):
-        _check(_run(*data, causal), _exact(*data[:4], lens_q, lens_k, causal, 1.0 / math.sqrt(D)), f'few rows D={D} causal={causal}')
+        _check(_run(*data, causal), _exact(*data[:4], lens_q, lens_k, causal, 1.0 / math.sqrt(D)), f'few rows D={D} causal={causal}', dtype)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
 @pytest.mark.parametrize('D', [64, 128])
-def test_few_keys_against_many_queries(gpu, D):
+def test_few_keys_against_many_queries(gpu, D, dtype):
     """the query range of dK / dV is split over workgroups and summed in order"""
     lens_q, lens_k = [3000, 1500], [77, 20]
-    data = _inputs(gpu, lens_q, lens_k, 4, 4, D)
+    data = _inputs(gpu, lens_q, lens_k, 4, 4, D, dtype=dtype)
     from diffusion_pipe_amd import hip
     assert hip.lib().dpipe_attn_varlen_bwd_workspace_floats(data[0].shape[0], data[1].shape[0], 2, 4, 4, D) > 0
-    _check(_run(*data, False), _exact(*data[:4], lens_q, lens_k, False, 1.0 / math.sqrt(D)), f'few keys D={D}')
+    _check(_run(*data, False), _exact(*data[:4], lens_q, lens_k, False, 1.0 / math.sqrt(D)), f'few keys D={D}', dtype)
 
 
-def test_rows_behind_the_last_sequence(gpu):
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+def test_rows_behind_the_last_sequence(gpu, dtype):
     """a buffer of fixed size: what lies behind the last sequence (NaN here) is not read into anything; its outputs and gradients are zero"""
     lens = [70, 130]
-    q, k, v, do, cu, _ = _inputs(gpu, lens, lens, 4, 2, 128, tail_q=90, tail_k=90)
+    q, k, v, do, cu, _ = _inputs(gpu, lens, lens, 4, 2, 128, tail_q=90, tail_k=90, dtype=dtype)
     for t in (q, k, v, do):
         t[200:] = float('nan')
     for causal in (False, True):
@@ -136,13 +155,14 @@ def test_rows_behind_the_last_sequence(gpu):
         for t in got.values():
             assert (t[200:] == 0).all()
         want = _exact(q[:200], k[:200], v[:200], do[:200], lens, lens, causal, 1.0 / math.sqrt(128))
-        _check({n: t[:200] for n, t in got.items()}, want, f'tail causal={causal}')
+        _check({n: t[:200] for n, t in got.items()}, want, f'tail causal={causal}', dtype)
 
 
-def test_neighbouring_sequences_do_not_leak(gpu):
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+def test_neighbouring_sequences_do_not_leak(gpu, dtype):
     """infinities and NaN in one sequence leave the others' outputs and gradients bit for bit as they were"""
     lens = [40, 65, 50]
-    q, k, v, do, cu, _ = _inputs(gpu, lens, lens, 2, 1, 64)
+    q, k, v, do, cu, _ = _inputs(gpu, lens, lens, 2, 1, 64, dtype=dtype)
     clean = _run(q, k, v, do, cu, None, True)
     for t, x in zip((q, k, v, do), (float('nan'), float('inf'), -float('inf'), float('nan'))):
         t[40:105] = x
@@ -151,10 +171,11 @@ def test_neighbouring_sequences_do_not_leak(gpu):
         assert torch.equal(clean[n][:40], dirty[n][:40]) and torch.equal(clean[n][105:], dirty[n][105:]), n
 
 
-def test_large_scores(gpu):
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+def test_large_scores(gpu, dtype):
     """scores whose exponentials span the whole range of fp32: the running maximum moves far and often.  A score error moves P relatively by |score| 2^-16: the bound's r grows with it."""
     lens = [200, 90]
-    q, k, v, do, cu, _ = _inputs(gpu, lens, lens, 2, 2, 64, spread=6.0)
+    q, k, v, do, cu, _ = _inputs(gpu, lens, lens, 2, 2, 64, spread=6.0, dtype=dtype)
     from diffusion_pipe_amd import ops
     o = ops.attention_varlen(q, k, v, cu, causal=True)
     value, bound = _exact(q, k, v, do, lens, lens, True, 0.125)['o']
@@ -222,12 +243,13 @@ def test_same_bits_every_time_and_no_gradient_wanted(gpu):
     assert torch.equal(dv, a['dv'])
 
 
-def test_captured_and_replayed_with_other_offsets(gpu):
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+def test_captured_and_replayed_with_other_offsets(gpu, dtype):
     """forward and backward in one graph; the lengths are data: two graphs, replayed in turn with offsets changed between replays, equal the eager results"""
     from diffusion_pipe_amd import ops
     plans = ([150, 50, 100], [10, 280, 10], [300, 0, 0])
-    q, k, v, do, cu, _ = _inputs(gpu, plans[0], plans[0], 4, 2, 128)
-    few = _inputs(gpu, [1, 2], [5000, 3000], 4, 2, 128)
+    q, k, v, do, cu, _ = _inputs(gpu, plans[0], plans[0], 4, 2, 128, dtype=dtype)
+    few = _inputs(gpu, [1, 2], [5000, 3000], 4, 2, 128, dtype=dtype)
 
     def step(q, k, v, do, cu_q, cu_k):
         leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
@@ -268,9 +290,10 @@ def test_on_another_stream(gpu):
     assert all(torch.equal(got[n], want[n]) for n in want)
 
 
-def test_offsets_that_do_not_ascend_stay_inside_the_tensors(gpu):
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+def test_offsets_that_do_not_ascend_stay_inside_the_tensors(gpu, dtype):
     """wrong offsets give wrong rows, never an access outside: every start and end is clamped by the kernels"""
-    q, k, v, do, cu, _ = _inputs(gpu, [100, 100], [100, 100], 2, 2, 64)
+    q, k, v, do, cu, _ = _inputs(gpu, [100, 100], [100, 100], 2, 2, 64, dtype=dtype)
     for bad in ([0, 150, 100], [0, -5, 900], [0, 2000000000, -2000000000], [50, 20, 200]):
         _run(q, k, v, do, torch.tensor(bad, dtype=torch.int32, device=gpu), None, True)
     torch.cuda.synchronize()
@@ -306,12 +329,13 @@ def test_empty_tensors(gpu):
     assert all((t == 0).all() for t in got.values())
 
 
-def test_long_sequence_past_32_bit_offsets(gpu):
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+def test_long_sequence_past_32_bit_offsets(gpu, dtype):
     """keys and values 2^32 bytes apart within one sequence: a token stride of 2^22 elements"""
     D, n, stride = 64, 700, 2 ** 22
-    buf = torch.zeros(n * stride, dtype=torch.bfloat16, device=gpu)
+    buf = torch.zeros(n * stride, dtype=dtype, device=gpu)
     g = torch.Generator().manual_seed(3)
-    q, k, v, do = (torch.randn(n, 1, D, generator=g).to(gpu, torch.bfloat16) for _ in range(4))
+    q, k, v, do = (torch.randn(n, 1, D, generator=g).to(gpu, dtype) for _ in range(4))
     kv = torch.as_strided(buf, (n, 2, D), (stride, D, 1))
     kv[:, :1], kv[:, 1:] = k, v
     cu = torch.tensor([0, n], dtype=torch.int32, device=gpu)

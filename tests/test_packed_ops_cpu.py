@@ -66,8 +66,9 @@ _Z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)
     ({'v': _Z(5, 2, 64)}, 'multiple of Hk'),
     ({'k': _Z(6, 0, 64), 'v': _Z(6, 0, 64)}, 'multiple of Hk'),
     ({'q': _Z(6, 4, 32), 'k': _Z(6, 2, 32), 'v': _Z(6, 2, 32)}, 'head dim 64 or 128'),
-    ({'q': _Z(6, 4, 64, dt=torch.float32)}, 'bf16'),
-    ({'v': _Z(6, 2, 64, dt=torch.float32)}, 'bf16'),
+    ({'q': _Z(6, 4, 64, dt=torch.float32)}, 'bf16 or fp32'),
+    ({'v': _Z(6, 2, 64, dt=torch.float32)}, 'bf16 or fp32'),
+    ({n: _Z(6, h, 64, dt=torch.float16) for n, h in (('q', 4), ('k', 2), ('v', 2))}, 'bf16 or fp32'),
     ({'cu_q': torch.tensor([0.0, 6.0])}, 'offsets'),
     ({'cu_q': torch.tensor([0], dtype=torch.int32)}, 'offsets'),
     ({'cu_q': torch.tensor([[0, 6]], dtype=torch.int32)}, 'offsets'),
@@ -110,7 +111,7 @@ def _varlen_c(name='fwd', **kw):
     a.update(ws=None, floats=0, tq=6, tk=6, n=1, hq=2, hk=1, D=64, q_ss=128, q_sh=64, k_ss=64, k_sh=64, v_ss=64, v_sh=64)
     if name == 'bwd':
         a.update(do_ss=128, do_sh=64)
-    a.update(scale=0.125, causal=0)
+    a.update(scale=0.125, causal=0, dtype=0)
     a.update(kw)
     rc = getattr(hip.lib(), f'dpipe_attn_varlen_{name}')(*a.values(), None)
     return rc, hip.lib().dpipe_last_error().decode()
@@ -118,7 +119,7 @@ def _varlen_c(name='fwd', **kw):
 
 @pytest.mark.parametrize('name', ['fwd', 'bwd'])
 @pytest.mark.parametrize('kw', [{'q': None}, {'cu_k': None}, {'tq': 0}, {'tk': -1}, {'n': 0}, {'hq': 3, 'hk': 2}, {'D': 96}, {'D': 256}, {'scale': 0.0}, {'scale': math.nan},
-                                {'scale': math.inf}, {'q': 264}, {'q_ss': 132}, {'k_ss': 32}, {'v_ss': 2 ** 23}, {'k_sh': -64}, {'tq': 2 ** 31}, {'n': 2 ** 23}, {'tk': 2 ** 18}])
+                                {'scale': math.inf}, {'q': 264}, {'q_ss': 132}, {'k_ss': 32}, {'v_ss': 2 ** 23}, {'k_sh': -64}, {'tq': 2 ** 31}, {'n': 2 ** 23}, {'dtype': 2}, {'tk': 2 ** 18}])
 def test_attention_varlen_c_entries_refuse(name, kw):
     """(the last: few rows and long keys -- or few keys' gradients -- need the workspace, which is missing)"""
     if name == 'bwd' and kw == {'tk': 2 ** 18}:
