@@ -16,6 +16,15 @@
 // As in attention.hip everything is v_mfma_f32_32x32x16_bf16 on the transposed score tile S^T = K . Q^T (a lane owns one query column: softmax statistics are
 // lane-local), tiles stream global -> LDS by buffer_load ... lds into a two-deep ring; rows past a sequence's end come back as zeros from the
 // buffer bounds check, whatever the neighbouring sequence holds.  Each tile has a buffer descriptor of its own, so a sequence may span more than 4 GiB.
+//
+// Bound: the matrix pipe, and with it the clock -- on long sequences the pipe is 55 - 66 % busy at 1.7 - 1.9 GHz (2.2 where it is less busy), as in a library product of 8192^3
+// (70 % at 1.9 GHz, 1238 TFLOP/s).  TFLOP/s of the products each kernel makes (forward 2, dQ 3, dK / dV 4):
+//   15000 + 6001 tokens, 24 heads of 128         forward 2.91 ms = 1102    dQ 3.90 ms = 1232    dK / dV 5.48 ms = 1171
+//   4608 + 2560 + 1311 tokens, 24 heads of 128            357 us = 1015           490 us = 1111             665 us = 1091
+//   7 causal sequences, 9277 tokens, 32 / 8 heads of 128  250 us =  804           345 us =  874             466 us =  862
+//   4096 + 2501 + 1024 tokens, 10 heads of 64              91 us =  677           114 us =  813             153 us =  806
+// The formulas have seven products, these kernels nine: both backward kernels make S and dP, so that dQ needs neither atomics nor a sum over fp32 parts (at 256 keys a part, len_k / 256
+// times the bytes of an fp32 dQ, written and read).
 #include <cstdio>
 #include "dpipe_common.h"
 #include "lds_dma_tiles.h"
@@ -144,7 +153,11 @@ __device__ __forceinline__ void store_row(bf16_t* dst, bf16_t* lo, const f32x16&
 }
 
 // ================================================================================================ forward
-// 128 rows per workgroup of 4 waves, two workgroups per CU: one's softmax runs under the other's products without a barrier between them.
+// 128 rows per workgroup of 4 waves, two workgroups per CU: one's softmax runs under the other's products without a barrier between them (8 waves of one workgroup: 3137 us where two
+// of 4 take 2991; 64 rows a wave, one wave a SIMD: 3733; the next tile's S issued before this one's softmax within a wave: 3977).  16 + 16 products of 32 cycles a tile against
+// ~300 vector instructions: the vector pipe is 47 % busy at D = 128 and, with half the products, the first limit at D = 64.
+// A sequence of 8 key tiles or fewer is bound by what a workgroup does once -- its sequence, its rows' loads, the stores: 6 of 22 us at 9216 queries on 512 keys.
+// SPLIT, a few rows on long keys: HBM; 8 single tokens on 60 354 keys, 32 / 8 heads of 128: 43 us = 5.7 TB/s.
 template <int D, bool SPLIT>
 __global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const Params p) {
     constexpr int NKS = D / 16, NDB = D / 32, IMG = KT * D * 2, STAGE = 2 * IMG;
@@ -255,6 +268,9 @@ __global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const Params p) {
 }
 
 // ================================================================================================ backward: dQ (and delta)
+// 128 rows per workgroup, two workgroups per CU.  LDS operands four steps ahead of their products: 4050 -> 3956 us on the longest case above.  delta needs O to more than bf16 (dP and delta
+// nearly cancel in dS): the forward keeps what the rounding of O left in bf16 too, 17 bits in 4 bytes a channel and half the traffic of an fp32 copy beside O (9216 queries on 512
+// keys: forward 207 -> 169 us).
 // Per 64-key tile: K, read by rows (S^T = K . Q^T) and transposed (dQ^T += K^T . dS^T), and V by rows (dP^T = V . dO^T).
 template <int D>
 __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
@@ -343,8 +359,10 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
 }
 
 // ================================================================================================ backward: dK, dV
-// Key-outer; a lane owns one key column, K stays in LDS, V and both accumulators in registers:  S = Q . K^T, dP = dO . V^T, dV^T += dO^T . P, dK^T += Q^T . dS.  Per 64-query tile Q and dO, both read by rows and transposed, and the
-// tile's lse / delta.  Query rows past the sequence arrive as zeros (Q, dO, lse, delta): P = 1 there, but dO = 0 and dS = 0.
+// Key-outer; a lane owns one key column, K stays in LDS, V and both accumulators in registers:  S = Q . K^T, dP = dO . V^T, dV^T += dO^T . P, dK^T += Q^T . dS.  Per 64-query tile Q
+// and dO, both read by rows and transposed, and the tile's lse / delta.  Query rows past the sequence arrive as zeros (Q, dO, lse, delta): P = 1 there, but dO = 0 and dS = 0.
+// One kernel for dK and dV shares S and P between them (two kernels made 5 products instead of 4: 7764 -> 6134 us on the longest case above); K in LDS instead of registers gives the
+// operands room one step ahead of their products (5992 -> 5640).  At D = 128 its 8 waves are two a SIMD and the LDS of a CU; 4 waves at D = 64, three a SIMD.
 template <int D, int NW, bool CORNER>
 __global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dkv_kernel(const Params p) {
     constexpr int QT = KT, NKS = D / 16, NDB = D / 32, IMG = QT * D * 2, O_STAT = 2 * IMG, STAGE = O_STAT + 1024;

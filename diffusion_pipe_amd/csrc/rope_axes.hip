@@ -9,9 +9,11 @@
 // of 10^6 keeps 10 digits of its angle), sine and cosine of the remainder fp32.  Pairs are neighbours (2 p, 2 p + 1) or halves (p, p + R / 2) of the R
 // rotated channels; channels behind R pass through (normalised, not rotated).
 //
-// Bound: HBM (forward reads x and writes y once, the backward of a normed row reads x and gy and writes dx).  One workgroup takes TB tokens: its threads
-// make the TB * R / 2 (cos, sin) pairs in LDS once, then every head row of q and of k uses them -- the trigonometry is paid once per token, not
-// per head.  A head row is LPR lanes of 8 channels; the norm's sums stay inside the lane group.
+// Bound: HBM (forward reads x and writes y once, the backward of a normed row reads x and gy and writes dx).  61 456 tokens x (24 + 24) heads of 128 in bf16 with norms: forward
+// 1.51 GB in 258 us = 5.9 TB/s, backward 2.27 GB in 424 us = 5.3 TB/s (a copy of 2 GiB: 4.9); 4608 tokens of the same heads, cached: 21 us.
+// One workgroup takes up to 8 tokens: its threads make the tokens' (cos, sin) pairs in LDS once, then every head row of q and of k uses them -- the trigonometry (fp64 turns) is
+// paid once per token, not per head, and no table is read.  A head row is LPR lanes of 8 channels; the norm's sums stay inside the lane group, by operand modifiers of the add
+// instead of LDS exchanges, and 4 rows a lane group are in flight (forward 286 -> 272 us, then 258 with streaming accesses).
 #include <cstdio>
 #include "dpipe_common.h"
 #include "../../include/dpipe_hip.h"
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(NB, 4) rope_axes_bwd_kernel(const RopeAxesPara
     }
 }
 
-// dw[c] (+)= sum over `blocks` partial rows, in a fixed order: 32 columns (8 lanes of 4) x 32 slices of the rows per workgroup
+// dw[c] (+)= sum over `blocks` partial rows, in a fixed order: 32 columns (8 lanes of 4) x 32 slices of the rows per workgroup.  Latency: 5.6 us for 512 rows.
 __global__ void __launch_bounds__(NB) rope_axes_dw_kernel(const float* __restrict__ part, void* dq, void* dk, int q_f32, int k_f32, int accumulate_q, int accumulate_k,
                                                           int blocks, int D) {
     __shared__ __attribute__((aligned(16))) float red[32][32];
