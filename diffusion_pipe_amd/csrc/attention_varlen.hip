@@ -51,29 +51,29 @@ constexpr int AQ = 4, AK = 1;            // steps of LDS operands read ahead of 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, long bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
 }
-// descriptor of up to KT rows of D bf16 (pitch ss) from row `at` on of `n`
-template <int D>
+// descriptor of up to KR rows of D bf16 (pitch ss) from row `at` on of `n`
+template <int D, int KR = KT>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const bf16_t* base, long ss, int at, int n) {
-    const int rows = min(n - at, KT);
+    const int rows = min(n - at, KR);
     return tile_rsrc(base + (long)at * ss, rows > 0 ? ((rows - 1) * ss + D) * 2 : 0);
 }
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, char* dst, unsigned off) { __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)dst, 16, off, 0, 0, 0); }
 __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, char* dst, unsigned off) { __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)dst, 4, off, 0, 0, 0); }
 
-// LDS image of a 64-row tile, read both by rows and transposed: slices of 64 columns, [64 rows][128 B] each, 16-byte chunk c of row r at chunk c ^ f(r) with
+// LDS image of a tile of KR rows (64 or 32), read both by rows and transposed: slices of 64 columns, [KR rows][128 B] each, 16-byte chunk c of row r at chunk c ^ f(r) with
 // f(r) = (r1 r3 r2) in bits of r.  Rows 0 .. 15 of one chunk (ds_read_b128) then cover the 256 B of all banks once, and so do the 4 rows x 64 B of one transposed read's half wave
 // (rows r .. r + 3 differ in r0 -- the 128-byte half -- and r1 -- the 64-byte granule).  One image where a tile is needed both ways (K in dQ; Q and dO in dK / dV) halves its DMA
 // traffic and its LDS.
 __device__ __forceinline__ int swizzle(int r) { return ((r >> 1) & 1) << 2 | ((r >> 2) & 3); }
 
-template <int D, int NW> struct Offsets {                     // per-lane source offsets of this wave's 1 KiB DMA pieces (8 rows of a slice) of one tile
-    static constexpr int PP = KT * D * 2 / 1024 / NW;
+template <int D, int NW, int KR = KT> struct Offsets {                     // per-lane source offsets of this wave's 1 KiB DMA pieces (8 rows of a slice) of one tile
+    static constexpr int PP = KR * D * 2 / 1024 / NW, BLOCKS = KR / 8;
     unsigned o[PP];
     __device__ __forceinline__ void init(int wid, int lane, long ss) {
 #pragma unroll
         for (int j = 0; j < PP; ++j) {
-            const int P = j * NW + wid, row = 8 * (P % 8) + (lane >> 3);
-            o[j] = (unsigned)(row * ss * 2) + (unsigned)(P / 8) * 128u + (unsigned)(((lane & 7) ^ swizzle(row)) << 4);
+            const int P = j * NW + wid, row = 8 * (P % BLOCKS) + (lane >> 3);
+            o[j] = (unsigned)(row * ss * 2) + (unsigned)(P / BLOCKS) * 128u + (unsigned)(((lane & 7) ^ swizzle(row)) << 4);
         }
     }
     __device__ __forceinline__ void issue(__amdgpu_buffer_rsrc_t rs, char* img, int wid) const {
@@ -83,15 +83,15 @@ template <int D, int NW> struct Offsets {                     // per-lane source
 };
 
 // MFMA operand with k along the row: lane (i, h) gets columns 16 ks + 8 h .. + 8 of row `row + i` (row a multiple of 32)
-__device__ __forceinline__ bf16x8_t by_rows(const char* img, int row, int ks, int lane) {
+template <int KR = KT> __device__ __forceinline__ bf16x8_t by_rows(const char* img, int row, int ks, int lane) {
     const int i = lane & 31;
-    return *reinterpret_cast<const bf16x8_t*>(img + (ks / 4) * (KT * 128) + row * 128 + i * 128 + ((((lane >> 5) ^ swizzle(i)) ^ (2 * (ks & 3))) << 4));
+    return *reinterpret_cast<const bf16x8_t*>(img + (ks / 4) * (KR * 128) + row * 128 + i * 128 + ((((lane >> 5) ^ swizzle(i)) ^ (2 * (ks & 3))) << 4));
 }
 // MFMA operand of the transposed tile: m = column `col + i` (col a multiple of 32), k = the rows of the 16-row block r0 in the order a lane holds them in a score accumulator
 // ({4 h + 0 .. 3, 8 + 4 h + 0 .. 3}), so P / dS go from their accumulators straight into the product
-__device__ __forceinline__ bf16x8_t by_cols(const char* img, int col, int r0, int lane) {
+template <int KR = KT> __device__ __forceinline__ bf16x8_t by_cols(const char* img, int col, int r0, int lane) {
     const int t = lane & 15, g = lane >> 4, r = 4 * (g >> 1) + (t >> 2);
-    const char* p = img + (col / 64) * (KT * 128) + r0 * 128 + r * 128 + (t & 1) * 8;
+    const char* p = img + (col / 64) * (KR * 128) + r0 * 128 + r * 128 + (t & 1) * 8;
     const int c = (((col / 32) & 1) << 2 | (g & 1) << 1 | ((t & 3) >> 1)) ^ swizzle(r);
     const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4_t*)(p + (c << 4)));
     const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4_t*)(p + 8 * 128 + ((c ^ 2) << 4)));
@@ -157,10 +157,11 @@ __device__ __forceinline__ void store_row(bf16_t* dst, bf16_t* lo, const f32x16&
 // of 4 take 2991; 64 rows a wave, one wave a SIMD: 3733; the next tile's S issued before this one's softmax within a wave: 3977).  16 + 16 products of 32 cycles a tile against
 // ~300 vector instructions: the vector pipe is 47 % busy at D = 128 and, with half the products, the first limit at D = 64.
 // A sequence of 8 key tiles or fewer is bound by what a workgroup does once -- its sequence, its rows' loads, the stores: 6 of 22 us at 9216 queries on 512 keys.
-// SPLIT, a few rows on long keys: HBM; 8 single tokens on 60 354 keys, 32 / 8 heads of 128: 43 us = 5.7 TB/s.
-template <int D, bool SPLIT>
-__global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const Params p) {
-    constexpr int NKS = D / 16, NDB = D / 32, IMG = KT * D * 2, STAGE = 2 * IMG;
+// SPLIT, a few rows on long keys: HBM; 8 tokens on 60 354 keys, 32 / 8 heads of 128: 51 us = 4.8 TB/s from HBM, 40 us from the last-level cache.  Tiles of KR = 32 keys there, whose
+// registers and LDS leave room for three workgroups a CU (tiles of 64, two: 54 us), unless the parts are too few to fill them (2 tokens on 3000 keys: 16.3 us, with tiles of 64 15.8).
+template <int D, bool SPLIT, int KR>
+__global__ void __launch_bounds__(NT, KR == KT ? 2 : 3) varlen_fwd_kernel(const Params p) {
+    constexpr int NKB = KR / 32, NKS = D / 16, NDB = D / 32, IMG = KR * D * 2, STAGE = 2 * IMG;
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
     const Work w = find_work(blockIdx.x, p.hk, SPLIT ? p.nsplit : 1);
     const Tile t = find_tile<ROWS>(p, w.slot, false, p.causal);
@@ -174,17 +175,17 @@ __global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const Params p) {
     const bf16_t* Q = p.q + r.token * p.q_ss + r.head * p.q_sh;
     const float sl2 = p.scale * LOG2E;
 
-    int kt0 = 0, kt1 = (seen.group + KT - 1) / KT;
+    int kt0 = 0, kt1 = (seen.group + KR - 1) / KR;
     if (SPLIT) {                                               // every part of the sequence's key tiles, cut by its full length
-        const int all = (t.lk + KT - 1) / KT, per = (all + p.nsplit - 1) / p.nsplit;
+        const int all = (t.lk + KR - 1) / KR, per = (all + p.nsplit - 1) / p.nsplit;
         kt0 = min(kt1, w.part * per); kt1 = min(kt1, kt0 + per);
     }
-    Offsets<D, 4> oK, oV;
+    Offsets<D, 4, KR> oK, oV;
     oK.init(wid, lane, p.k_ss); oV.init(wid, lane, p.v_ss);
     auto issue = [&](int kt) {
         char* base = lds + (kt & 1) * STAGE;
-        oK.issue(rows_rsrc<D>(K, p.k_ss, kt * KT, t.lk), base, wid);
-        oV.issue(rows_rsrc<D>(V, p.v_ss, kt * KT, t.lk), base + IMG, wid);
+        oK.issue(rows_rsrc<D, KR>(K, p.k_ss, kt * KR, t.lk), base, wid);
+        oV.issue(rows_rsrc<D, KR>(V, p.v_ss, kt * KR, t.lk), base + IMG, wid);
     };
     if (kt0 < kt1) issue(kt0);                                 // (in flight under the query's own loads)
     bf16x8_t qf[NKS];
@@ -201,22 +202,24 @@ __global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const Params p) {
         if (kt + 1 < kt1) issue(kt + 1);
         const char* Kl = lds + (kt & 1) * STAGE;
         const char* Vl = Kl + IMG;
-        const int key0 = kt * KT;
+        const int key0 = kt * KR;
         if (key0 >= seen.wave) continue;                       // wave-uniform: no row of this wave sees the tile
-        f32x16 s[2] = {zero16(), zero16()};
+        f32x16 s[NKB];
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) s[kb] = zero16();
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) s[kb] = mfma16(by_rows(Kl, 32 * kb, ks, lane), qf[ks], s[kb]);
-        if (key0 + KT > seen.all) {                            // some row of the wave does not see the whole tile
+            for (int kb = 0; kb < NKB; ++kb) s[kb] = mfma16(by_rows<KR>(Kl, 32 * kb, ks, lane), qf[ks], s[kb]);
+        if (key0 + KR > seen.all) {                            // some row of the wave does not see the whole tile
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[kb][e] = key0 + 32 * kb + (e & 3) + 8 * (e >> 2) + 4 * h <= r.last ? s[kb][e] : -INFINITY;
         }
         float mx = s[0][0];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
         mx = max_halves(mx) * sl2;
@@ -230,22 +233,22 @@ __global__ void __launch_bounds__(NT, 2) varlen_fwd_kernel(const Params p) {
         }
         float rs = 0.f;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
             for (int e = 0; e < 16; ++e) { const float pe = __builtin_amdgcn_exp2f(s[kb][e] * sl2 - m); s[kb][e] = pe; rs += pe; }
         l += rs;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {                          // O^T += V^T . P^T, P rounded to the products' bf16
+        for (int u = 0; u < 2 * NKB; ++u) {                          // O^T += V^T . P^T, P rounded to the products' bf16
             const bf16x8_t pf = pack_frag(s[u >> 1], 8 * (u & 1));
 #pragma unroll
-            for (int db = 0; db < NDB; ++db) oacc[db] = mfma16(by_cols(Vl, 32 * db, 16 * u, lane), pf, oacc[db]);
+            for (int db = 0; db < NDB; ++db) oacc[db] = mfma16(by_cols<KR>(Vl, 32 * db, 16 * u, lane), pf, oacc[db]);
         }
-        if (kt == 0) {                                         // the first tile adds what the rounding left (see CORNER)
+        if (key0 < KT) {                                       // the first 64 keys add what the rounding left (see CORNER)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < 2 * NKB; ++u) {
                 const bf16x8_t pl = pack_rest(s[u >> 1], 8 * (u & 1));
 #pragma unroll
-                for (int db = 0; db < NDB; ++db) oacc[db] = mfma16(by_cols(Vl, 32 * db, 16 * u, lane), pl, oacc[db]);
+                for (int db = 0; db < NDB; ++db) oacc[db] = mfma16(by_cols<KR>(Vl, 32 * db, 16 * u, lane), pl, oacc[db]);
             }
         }
     }
@@ -530,8 +533,9 @@ int fill(VarlenParams<T>& p, const char* what, const void* q, const void* k, con
 
 template <int D> void forward(const Params& p, hipStream_t s) {
     const unsigned grid = (unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, p.nsplit);
-    if (p.nsplit == 1) { varlen_fwd_kernel<D, false><<<grid, NT, 0, s>>>(p); return; }
-    varlen_fwd_kernel<D, true><<<grid, NT, 0, s>>>(p);
+    if (p.nsplit == 1) { varlen_fwd_kernel<D, false, KT><<<grid, NT, 0, s>>>(p); return; }
+    if (D == 128 && p.nsplit * (cdiv(p.tq * p.g, ROWS) + p.n - 1) * p.hk >= 512) varlen_fwd_kernel<D, true, D == 128 ? 32 : KT><<<grid, NT, 0, s>>>(p);
+    else varlen_fwd_kernel<D, true, KT><<<grid, NT, 0, s>>>(p);
     varlen_join_kernel<bf16_t, D><<<(unsigned)cdiv(p.tq * p.hq, 4), NT, 0, s>>>(p);
 }
 template <int D> void backward(Params& p, int parts, hipStream_t s) {

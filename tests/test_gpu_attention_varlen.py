@@ -133,6 +133,18 @@ def test_few_rows_against_long_keys(gpu, D, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+def test_single_tokens_against_very_long_keys(gpu, dtype):
+    """parts enough for three workgroups on a CU: tiles of 32 keys at head size 128 in bf16; a sequence that ends inside the first tile, one of no keys at all"""
+    lens_q, lens_k, H, Hk, D = [2, 1, 3, 1], [40001, 37, 30015, 0], 32, 8, 128
+    data = _inputs(gpu, lens_q, lens_k, H, Hk, D, dtype=dtype)
+    from diffusion_pipe_amd import hip
+    floats = hip.lib().dpipe_attn_varlen_fwd_workspace_floats(7, sum(lens_k), 4, H, Hk, D)
+    assert floats // (7 * H * (D + 1)) * 4 * Hk >= 512
+    for causal in (True, False):
+        _check(_run(*data, causal), _exact(*data[:4], lens_q, lens_k, causal, 1.0 / math.sqrt(D)), f'very long keys causal={causal}', dtype)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
 @pytest.mark.parametrize('D', [64, 128])
 def test_few_keys_against_many_queries(gpu, D, dtype):
     """the query range of dK / dV is split over workgroups and summed in order"""
