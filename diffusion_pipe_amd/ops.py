@@ -1830,6 +1830,7 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=False):
     q [Tq, H, D], k / v [Tk, Hk, D] with H a multiple of Hk: query head h reads key head h // (H // Hk).  Column blocks of a fused projection are read in place.
     cu_q, cu_k: int32 offsets [N + 1] on the device, ascending from 0; sequence b holds query tokens cu_q[b] .. cu_q[b + 1] - 1 and key tokens cu_k[b] .. cu_k[b + 1] - 1, either
     of which may be empty.  cu_k None: the queries' offsets (Tk = Tq).  The lengths are never read on the host: the call can be captured and replayed with other offsets.
+    (As with any operator: while its backward pass is captured, no eager graph of the same leaf tensors may be alive -- their accumulation nodes would run on that graph's stream.)
     causal: query i sees key j of its sequence when j - len_k <= i - len_q (the last query sees every key; with equal lengths j <= i).
     A query that sees no key, and the rows behind the last sequence, give zeros and take and give no gradient, whatever those rows hold (values INSIDE a sequence are expected to be
     finite: a masked infinity or NaN reaches its sequence's other rows).  The same inputs give the same bits (no atomics).  (models/wan/attention.py:91-122)

@@ -302,6 +302,29 @@ def test_on_another_stream(gpu):
     assert all(torch.equal(got[n], want[n]) for n in want)
 
 
+def test_two_threads_on_two_streams_at_once(gpu):
+    """calls in flight at the same time share nothing: parts of split axes, statistics and outputs are each call's own"""
+    import threading
+    cases = [_inputs(gpu, [1, 2], [5000, 3000], 4, 2, 128), _inputs(gpu, [3000, 1500], [77, 20], 4, 4, 64)]
+    want = [_run(*c, True) for c in cases]
+    torch.cuda.synchronize()
+    got, streams = [[], []], [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(8):
+                got[i].append(_run(*cases[i], True))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 8 and all(torch.equal(g[n], want[i][n]) for g in got[i] for n in g)
+
+
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
 def test_offsets_that_do_not_ascend_stay_inside_the_tensors(gpu, dtype):
     """wrong offsets give wrong rows, never an access outside: every start and end is clamped by the kernels"""
