@@ -119,6 +119,12 @@ __device__ __forceinline__ void ahead_run(Frag (&f)[AHEAD], Load load, Use use) 
     }
 }
 
+// Head size 64: a wave at its products goes before the others of its SIMD, whose exponentials fill the gaps (3 images, 10 heads: forward 96.6 -> 93.5 us, dK / dV 164 -> 158, dQ 1 %;
+// at 128, where the clock gives way as the matrix pipe fills, nothing is gained, in dK / dV 3 % lost, and where few rows read long keys 1 %)
+template <int D> __device__ __forceinline__ void products_first(bool on) {
+    if (D == 64) { if (on) __builtin_amdgcn_s_setprio(1); else __builtin_amdgcn_s_setprio(0); }
+}
+
 // what pack_frag's rounding leaves of 8 accumulator entries, itself as an operand
 __device__ __forceinline__ bf16x8_t pack_rest(const f32x16& s, int e0) {
     uint32_t r[4];
@@ -204,6 +210,7 @@ __global__ void __launch_bounds__(NT, KR == KT ? 2 : 3) varlen_fwd_kernel(const 
         const char* Vl = Kl + IMG;
         const int key0 = kt * KR;
         if (key0 >= seen.wave) continue;                       // wave-uniform: no row of this wave sees the tile
+        products_first<SPLIT ? 0 : D>(true);
         f32x16 s[NKB];
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb) s[kb] = zero16();
@@ -211,6 +218,7 @@ __global__ void __launch_bounds__(NT, KR == KT ? 2 : 3) varlen_fwd_kernel(const 
         for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
             for (int kb = 0; kb < NKB; ++kb) s[kb] = mfma16(by_rows<KR>(Kl, 32 * kb, ks, lane), qf[ks], s[kb]);
+        products_first<SPLIT ? 0 : D>(false);
         if (key0 + KR > seen.all) {                            // some row of the wave does not see the whole tile
 #pragma unroll
             for (int kb = 0; kb < NKB; ++kb)
@@ -237,6 +245,7 @@ __global__ void __launch_bounds__(NT, KR == KT ? 2 : 3) varlen_fwd_kernel(const 
 #pragma unroll
             for (int e = 0; e < 16; ++e) { const float pe = __builtin_amdgcn_exp2f(s[kb][e] * sl2 - m); s[kb][e] = pe; rs += pe; }
         l += rs;
+        products_first<SPLIT ? 0 : D>(true);
 #pragma unroll
         for (int u = 0; u < 2 * NKB; ++u) {                          // O^T += V^T . P^T, P rounded to the products' bf16
             const bf16x8_t pf = pack_frag(s[u >> 1], 8 * (u & 1));
@@ -338,9 +347,11 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
             bf16x8_t f[AQ], kt[AQ];
             auto load = [&](int j) { return by_rows(j & 1 ? Vl : Kl, 32 * kb, j >> 1, lane); };
             auto load_t = [&](int j) { return by_cols(Kl, 32 * (j % NDB), 32 * kb + 16 * (j / NDB), lane); };
+            products_first<D>(true);
             ahead_start(f, load);
             ahead_run<2 * NKS>(f, load, [&](int j, const bf16x8_t& x) { if (j & 1) dp = mfma16(x, dof[j >> 1], dp); else s = mfma16(x, qf[j >> 1], s); });
             ahead_start(kt, load_t);
+            products_first<D>(false);
             if (key0 + 32 > seen.all) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = key0 + (e & 3) + 8 * (e >> 2) + 4 * h <= r.last ? s[e] : -INFINITY;
@@ -355,6 +366,7 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
                     for (int db = 0; db < NDB; ++db) dq[db] = mfma16(by_cols(Kl, 32 * db, 32 * kb + 16 * u, lane), rest[u], dq[db]);
             }
             const bf16x8_t ds[2] = {pack_frag(s, 0), pack_frag(s, 8)};
+            products_first<D>(true);
             __builtin_amdgcn_sched_barrier(0);
             ahead_run<2 * NDB>(kt, load_t, [&](int j, const bf16x8_t& x) { dq[j % NDB] = mfma16(x, ds[j / NDB], dq[j % NDB]); });
         }
@@ -441,9 +453,11 @@ __global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dk
             auto load_t = [&](int j) {
                 return Frags{by_cols(Ql, 32 * (j % NDB), 32 * qb + 16 * (j / NDB), lane), by_cols(DOl, 32 * (j % NDB), 32 * qb + 16 * (j / NDB), lane), {}};
             };
+            products_first<D>(true);
             ahead_start(f, load);
             ahead_run<NKS>(f, load, [&](int j, const Frags& x) { s = mfma16(x.q, x.k, s); dp = mfma16(x.d, vf[j], dp); });
             ahead_start(g, load_t);
+            products_first<D>(false);
             if (p.causal && q0 + ahead < k0w + 31) {           // some query of the block does not see every key of this wave
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = key <= q0 + 8 * (e >> 2) + 4 * h + (e & 3) + ahead ? s[e] : -INFINITY;
@@ -471,6 +485,7 @@ __global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dk
                     }
             }
             const bf16x8_t pf[2] = {pack_frag(pr, 0), pack_frag(pr, 8)}, ds[2] = {pack_frag(s, 0), pack_frag(s, 8)};
+            products_first<D>(true);
             __builtin_amdgcn_sched_barrier(0);
             ahead_run<2 * NDB>(g, load_t, [&](int j, const Frags& x) { dv[j % NDB] = mfma16(x.d, pf[j / NDB], dv[j % NDB]); dk[j % NDB] = mfma16(x.q, ds[j / NDB], dk[j % NDB]); });
         }
