@@ -21,8 +21,8 @@
 // (70 % at 1.9 GHz, 1238 TFLOP/s).  TFLOP/s of the products each kernel makes (forward 2, dQ 3, dK / dV 4):
 //   15000 + 6001 tokens, 24 heads of 128         forward 2.91 ms = 1102    dQ 3.90 ms = 1232    dK / dV 5.48 ms = 1171
 //   4608 + 2560 + 1311 tokens, 24 heads of 128            357 us = 1015           490 us = 1111             665 us = 1091
-//   7 causal sequences, 9277 tokens, 32 / 8 heads of 128  250 us =  804           345 us =  874             466 us =  862
-//   4096 + 2501 + 1024 tokens, 10 heads of 64              91 us =  677           114 us =  813             153 us =  806
+//   7 causal sequences, 9277 tokens, 32 / 8 heads of 128  246 us =  817           315 us =  957             446 us =  901
+//   4096 + 2501 + 1024 tokens, 10 heads of 64              89 us =  694           110 us =  843             151 us =  819
 // The formulas have seven products, these kernels nine: both backward kernels make S and dP, so that dQ needs neither atomics nor a sum over fp32 parts (at 256 keys a part, len_k / 256
 // times the bytes of an fp32 dQ, written and read).
 #include <cstdio>
