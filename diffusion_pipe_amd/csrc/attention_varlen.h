@@ -129,8 +129,8 @@ __device__ __forceinline__ float sum_halves(float x) {
 }
 
 // joins the parts of a row: o = sum_s 2^(lse_s - top) o_s / sum_s 2^(lse_s - top); one wave per row, its lanes hold the parts' weights (nsplit <= 64), then D / 64 channels each.
-// 16 parts' reads in flight: latency, 6 us for 8 tokens x 32 heads x 39 parts.
-template <typename T, int D>
+// U parts' reads in flight: latency, 6 us for 8 tokens x 32 heads x 39 parts.
+template <typename T, int D, int U>
 __global__ void __launch_bounds__(NT) varlen_join_kernel(const VarlenParams<T> p) {
     constexpr int C = D / 64;
     const long rows = p.tq * p.hq, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -143,14 +143,14 @@ __global__ void __launch_bounds__(NT) varlen_join_kernel(const VarlenParams<T> p
     float a[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) a[c] = 0.f;
-    for (int s0 = 0; s0 < p.nsplit; s0 += 16) {                // 16 parts' reads in flight
-        float v[16][C];
+    for (int s0 = 0; s0 < p.nsplit; s0 += U) {
+        float v[U][C];
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < U; ++j)
 #pragma unroll
             for (int c = 0; c < C; ++c) v[j][c] = p.part[(min(s0 + j, p.nsplit - 1) * rows + row) * D + lane * C + c];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {                         // a part that saw nothing has stored nothing: what is read there does not count
+        for (int j = 0; j < U; ++j) {                          // a part that saw nothing has stored nothing: what is read there does not count
             const int s = min(s0 + j, 63);
             const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
             const bool stored = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ls), s)) != -INFINITY;      // (lanes from nsplit on hold -inf)
@@ -191,8 +191,13 @@ __global__ void __launch_bounds__(256) varlen_dkv_sum_kernel(const VarlenParams<
 
 inline int row_slots(long tokens, int g, int n, int per) { return (int)(tokens * g / per + n + 1); }
 
+template <typename T, int D> void join(const VarlenParams<T>& p, hipStream_t s) {
+    const unsigned grid = (unsigned)cdiv(p.tq * p.hq, 4);
+    if (p.nsplit <= 4) varlen_join_kernel<T, D, 4><<<grid, NT, 0, s>>>(p); else varlen_join_kernel<T, D, 16><<<grid, NT, 0, s>>>(p);
+}
+
 // attention_varlen_f32.hip
 void forward_f32(const VarlenParams<float>& p, int D, hipStream_t s);
-void backward_f32(VarlenParams<float>& p, int D, int parts, hipStream_t s);
+void backward_f32(const VarlenParams<float>& p, int D, hipStream_t s);
 
 }  // namespace dpipe_varlen

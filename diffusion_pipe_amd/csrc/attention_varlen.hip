@@ -509,22 +509,43 @@ __global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dk
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-// parts of the key range: when the row tiles alone leave CUs idle, enough parts for two workgroups per CU, of at least 4 key tiles of an average sequence each
-int fwd_splits(long tq, long tk, int n, int hq, int hk) {
-    const long wgs = cdiv(tq * (hq / hk), ROWS) * hk, tiles = tk / n / KT;
-    if (wgs >= 256 || tiles < 8) return 1;
-    long s = cdiv(512, wgs);
-    if (s > tiles / 4) s = tiles / 4;
-    return (int)(s > 64 ? 64 : s);
+// In how many parts (own workgroups, fp32 partial results, a kernel that sums them) an axis is cut that workgroups walk in LDS tiles: the least of the estimated times
+//   us(parts) = tile * tiles / parts * max(longest, share * x) + once * x / per_cu + (parts > 1: sum + part * parts),    x = workgroups per CU
+// tile: a tile's time for a workgroup that has its CU to itself; share: what of it is left per workgroup when several share the CU; once: a workgroup's start and end; sum, part: the
+// kernel that sums, and what a part adds.  One sequence: its tiles, and x rounded up (all its workgroups take the same time).  Several: the lengths are on the device, so the average's
+// tiles, the longest taken as 1.5 of it, their rows as one sequence's but for `once`, with at least a workgroup a sequence and head; and of the cuts within 10 % the finest, which
+// balances best.  Measured, with the sums, us, whole / as chosen.  Forward: 8 tokens on 3 x 10 000 keys, 12 / 4 heads of 64: 240 / 17; 4096 tokens, 4 heads of 128: 84 / 61, 7 heads
+// 89 / 89 (four parts 102); 2048 tokens, 12 heads of 64: 33 / 33 (three parts 45); 8000 queries on 512 keys, 4 heads: 21 / 21 (three parts 49).  dK / dV: 1000 tokens, 10 heads: 52 / 41;
+// 4096 tokens, 4 heads 190 / 94, 7 heads 198 / 147; 8000 queries on 512 keys 346 / 44; six causal sequences of 1000, 8 heads: 60 / 60 (three parts 94).
+struct SplitCost { float tile, share, once, sum, part; int per_cu; };
+int best_parts(long row_tiles, long rows, int heads, long tiles, int n, const SplitCost& k) {
+    const float cu = heads / 256.f, all = row_tiles > n ? row_tiles : n < rows ? n : rows;
+    auto us = [&](int s) {
+        const float x = n > 1 ? row_tiles * s * cu : ceilf(row_tiles * s * cu);
+        return k.tile * tiles / s * fmaxf(n > 1 ? 1.5f : 1.f, k.share * x) + k.once * ceilf(all * s * cu / k.per_cu) + (s > 1 ? k.sum + k.part * s : 0.f);
+    };
+    const int most = tiles < 8 ? 1 : tiles < 128 ? (int)tiles / 2 : 64;      // at least two tiles a part
+    int best = 1;
+    for (int s = 2; s <= most; ++s) if (us(s) < us(best)) best = s;
+    if (best == 1 || n == 1) return best;
+    const float close = 1.1f * us(best);
+    for (int s = most; s > best; --s) if (us(s) <= close) return s;
+    return best;
+}
+// parts of the key range, D = 128 / 64: 1.2 / 0.85 us a tile (a workgroup's run over 64 tiles alone on its CU: 84 us, two to a CU 1.9 us a tile each)
+int fwd_splits(long tq, long tk, int n, int hq, int hk, int D) {
+    const float m = tq * hq * (float)D * 1e-6f;               // (millions of partial results a part)
+    const long rows = tq * (hq / hk);
+    return best_parts(cdiv(rows, ROWS), rows, hk, tk / n / KT, n, {D == 128 ? 1.2f : 0.85f, D == 128 ? 0.78f : 0.55f, 7.f, 5.5f + 2.5f * m, 1.5f * m, D == 128 ? 2 : 3});
 }
 // keys of a dK / dV workgroup: 8 waves at D = 128, whose K image and registers leave room for one workgroup per CU, 4 at 64
 constexpr int key_tile(int D) { return D == 128 ? 256 : 128; }
-// parts of the query tiles (of all g heads) for dK / dV, likewise; with grouped heads up to g parts also where the key tiles alone are fewer than 3 a CU and the sequences long enough
-// that the parts' fp32 sums do not cost more than the balance gives (4 x 2048 causal tokens, 32 / 8 heads, backward: 648 -> 604 us; 16 x 512: 310 unsplit, 332 split)
+// parts of the query tiles (of all g heads) for dK / dV, D = 128 / 64: 3.0 / 1.6 us a tile.  With grouped heads up to g parts also where the key tiles alone are fewer than 3 a CU and the
+// sequences long enough that the parts' fp32 sums do not cost more than the balance gives (4 x 2048 causal tokens, 32 / 8 heads, backward: 648 -> 604 us; 16 x 512: 310 unsplit, 332 split)
 int dkv_splits(long tq, long tk, int n, int hq, int hk, int D) {
-    const long wgs = cdiv(tk, key_tile(D)) * hk, g = hq / hk, tiles = tq / n / KT * g;
-    long s = 1;
-    if (wgs < 256 && tiles >= 8) { s = cdiv(512, wgs); if (s > tiles / 4) s = tiles / 4; }
+    const long key_tiles = cdiv(tk, key_tile(D)), wgs = key_tiles * hk, g = hq / hk, tiles = tq / n / KT * g;
+    const float part = 3.1f * (tk * hk * (float)D * 1e-6f);
+    long s = D == 128 ? best_parts(key_tiles, tk, hk, tiles, n, {3.0f, 1.0f, 6.f, 6.f, part, 1}) : best_parts(key_tiles, tk, hk, tiles, n, {1.6f, 0.55f, 6.f, 6.f, part, 3});
     if (wgs < 768 && g > 1 && tiles >= 16 * g) { long m = cdiv(768, wgs); if (m > g) m = g; if (m > s) s = m; }
     return (int)(s > 64 ? 64 : s);
 }
@@ -535,17 +556,18 @@ bool rows_ok(const void* p, long ss, long sh, int D) {
 
 template <typename T>
 int fill(VarlenParams<T>& p, const char* what, const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, long tq, long tk, int n, int hq, int hk, int D, long q_ss,
-         long q_sh, long k_ss, long k_sh, long v_ss, long v_sh, float scale, int causal) {
+         long q_sh, long k_ss, long k_sh, long v_ss, long v_sh, float scale, int causal, bool backward) {
     auto bad = [&](const char* m, int rc = DPIPE_ERR_ARG) { char buf[160]; snprintf(buf, sizeof(buf), "%s: %s", what, m); set_last_error(buf); return rc; };
     if (!q || !k || !v || !cu_q || !cu_k || tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk) return bad("bad argument");
     if (D != 64 && D != 128) return bad("head dim must be 64 or 128", DPIPE_ERR_UNSUPPORTED);
     if (!(scale > 0.f) || scale > 1e30f) return bad("scale must be positive and finite");
-    const int fs = fwd_splits(tq, tk, n, hq, hk), bs = dkv_splits(tq, tk, n, hq, hk, D);
-    if (tq * (hq / hk) >= (1l << 31) - 256 || tk >= (1l << 31) - 256 || work_groups(tq * (hq / hk) / ROWS + n + 1, hk, fs) >= (1l << 23) || work_groups(tk / ROWS + n + 1, hk, bs) >= (1l << 23))
+    p.nsplit = backward ? dkv_splits(tq, tk, n, hq, hk, D) : fwd_splits(tq, tk, n, hq, hk, D);
+    if (tq * (hq / hk) >= (1l << 31) - 256 || tk >= (1l << 31) - 256 || work_groups(tq * (hq / hk) / ROWS + n + 1, hk, backward ? 1 : p.nsplit) >= (1l << 23) ||
+        (backward && work_groups(tk / ROWS + n + 1, hk, p.nsplit) >= (1l << 23)))
         return bad("too many rows or sequences", DPIPE_ERR_UNSUPPORTED);
     if (!rows_ok(q, q_ss, q_sh, D) || !rows_ok(k, k_ss, k_sh, D) || !rows_ok(v, v_ss, v_sh, D)) return bad("tensors must be 16-byte aligned with strides multiple of 8 elements");
     p.q = (const T*)q; p.k = (const T*)k; p.v = (const T*)v; p.cu_q = cu_q; p.cu_k = cu_k; p.tq = tq; p.tk = tk; p.n = n; p.hq = hq; p.hk = hk; p.g = hq / hk;
-    p.q_ss = q_ss; p.q_sh = q_sh; p.k_ss = k_ss; p.k_sh = k_sh; p.v_ss = v_ss; p.v_sh = v_sh; p.scale = scale; p.causal = causal != 0; p.nsplit = 1;
+    p.q_ss = q_ss; p.q_sh = q_sh; p.k_ss = k_ss; p.k_sh = k_sh; p.v_ss = v_ss; p.v_sh = v_sh; p.scale = scale; p.causal = causal != 0;
     return DPIPE_OK;
 }
 
@@ -554,15 +576,14 @@ template <int D> void forward(const Params& p, hipStream_t s) {
     if (p.nsplit == 1) { varlen_fwd_kernel<D, false, KT><<<grid, NT, 0, s>>>(p); return; }
     if (D == 128 && p.nsplit * (cdiv(p.tq * p.g, ROWS) + p.n - 1) * p.hk >= 512) varlen_fwd_kernel<D, true, D == 128 ? 32 : KT><<<grid, NT, 0, s>>>(p);
     else varlen_fwd_kernel<D, true, KT><<<grid, NT, 0, s>>>(p);
-    varlen_join_kernel<bf16_t, D><<<(unsigned)cdiv(p.tq * p.hq, 4), NT, 0, s>>>(p);
+    join<bf16_t, D>(p, s);
 }
-template <int D> void backward(Params& p, int parts, hipStream_t s) {
+template <int D> void backward(const Params& p, hipStream_t s) {
     varlen_dq_kernel<D><<<(unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, 1), NT, 0, s>>>(p);
-    p.nsplit = parts;
     constexpr int NW = key_tile(D) / 32;
-    const unsigned grid = (unsigned)work_groups(row_slots(p.tk, 1, p.n, 32 * NW), p.hk, parts);
+    const unsigned grid = (unsigned)work_groups(row_slots(p.tk, 1, p.n, 32 * NW), p.hk, p.nsplit);
     if (p.tk / p.n <= KT) varlen_dkv_kernel<D, NW, true><<<grid, 64 * NW, 0, s>>>(p); else varlen_dkv_kernel<D, NW, false><<<grid, 64 * NW, 0, s>>>(p);
-    if (parts > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<bf16_t><<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
+    if (p.nsplit > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<bf16_t><<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
 }
 
 }  // namespace
@@ -571,7 +592,7 @@ extern "C" {
 
 long dpipe_attn_varlen_fwd_workspace_floats(long tq, long tk, int n, int hq, int hk, int D) {
     if (tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk || (D != 64 && D != 128)) return 0;
-    const int s = fwd_splits(tq, tk, n, hq, hk);
+    const int s = fwd_splits(tq, tk, n, hq, hk, D);
     return s > 1 ? (long)s * tq * hq * (D + 1) : 0;
 }
 long dpipe_attn_varlen_bwd_workspace_floats(long tq, long tk, int n, int hq, int hk, int D) {
@@ -585,14 +606,14 @@ int dpipe_attn_varlen_fwd(const void* q, const void* k, const void* v, const int
     auto run = [&](auto type, auto launch) {
         typedef decltype(type) T;
         VarlenParams<T> p = {};
-        const int rc = fill(p, "dpipe_attn_varlen_fwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal);
+        const int rc = fill(p, "dpipe_attn_varlen_fwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal, false);
         if (rc) return rc;
-        const long need = dpipe_attn_varlen_fwd_workspace_floats(tq, tk, n, hq, hk, D);
+        const long need = p.nsplit > 1 ? (long)p.nsplit * tq * hq * (D + 1) : 0;
         if (!o || !aligned16(o) || !aligned16(o_lo) || (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) {
             set_last_error("dpipe_attn_varlen_fwd: bad output or workspace"); return DPIPE_ERR_ARG; }
         if (ablated(ABL_ATTN)) return DPIPE_OK;
         p.o = (T*)o; p.o_lo = sizeof(T) == 2 ? (T*)o_lo : nullptr; p.lse = lse;
-        if (need > 0) { p.nsplit = fwd_splits(tq, tk, n, hq, hk); p.part = ws; p.part_lse = ws + (long)p.nsplit * tq * hq * D; }
+        if (need > 0) { p.part = ws; p.part_lse = ws + (long)p.nsplit * tq * hq * D; }
         launch(p);
         return check_launch("dpipe_attn_varlen_fwd");
     };
@@ -609,21 +630,21 @@ int dpipe_attn_varlen_bwd(const void* q, const void* k, const void* v, const int
     auto run = [&](auto type, auto launch) {
         typedef decltype(type) T;
         VarlenParams<T> p = {};
-        const int rc = fill(p, "dpipe_attn_varlen_bwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal);
+        const int rc = fill(p, "dpipe_attn_varlen_bwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal, true);
         if (rc) return rc;
-        const long need = dpipe_attn_varlen_bwd_workspace_floats(tq, tk, n, hq, hk, D);
+        const long need = p.nsplit > 1 ? 2l * p.nsplit * tk * hk * D : 0;
         if (!o || (sizeof(T) == 2 && !o_lo) || !dout || !lse || !delta || !dq || !dk || !dv || !aligned16(o) || !aligned16(o_lo) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
             !rows_ok(dout, do_ss, do_sh, D) || (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) {
             set_last_error("dpipe_attn_varlen_bwd: bad gradient or workspace"); return DPIPE_ERR_ARG; }
         if (ablated(ABL_ATTN)) return DPIPE_OK;
         p.o = (T*)o; p.o_lo = (T*)o_lo; p.dout = (const T*)dout; p.lse = const_cast<float*>(lse); p.delta = delta;
         p.dq = (T*)dq; p.dk = (T*)dk; p.dv = (T*)dv; p.do_ss = do_ss; p.do_sh = do_sh; p.part = ws;
-        launch(p, need > 0 ? dkv_splits(tq, tk, n, hq, hk, D) : 1);
+        launch(p);
         return check_launch("dpipe_attn_varlen_bwd");
     };
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (dtype == DPIPE_BF16) return run(bf16_t{}, [&](auto& p, int parts) { if (D == 64) backward<64>(p, parts, s); else backward<128>(p, parts, s); });
-    if (dtype == DPIPE_F32) return run(float{}, [&](auto& p, int parts) { backward_f32(p, D, parts, s); });
+    if (dtype == DPIPE_BF16) return run(bf16_t{}, [&](auto& p) { if (D == 64) backward<64>(p, s); else backward<128>(p, s); });
+    if (dtype == DPIPE_F32) return run(float{}, [&](auto& p) { backward_f32(p, D, s); });
     set_last_error("dpipe_attn_varlen_bwd: dtype must be bf16 or fp32");
     return DPIPE_ERR_UNSUPPORTED;
 }

@@ -252,18 +252,17 @@ template <int D> void forward(const Params& p, hipStream_t s) {
     const unsigned grid = (unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, p.nsplit);
     if (p.nsplit == 1) { varlen_f32_fwd_kernel<D, false><<<grid, NT, 0, s>>>(p); return; }
     varlen_f32_fwd_kernel<D, true><<<grid, NT, 0, s>>>(p);
-    varlen_join_kernel<float, D><<<(unsigned)cdiv(p.tq * p.hq, 4), NT, 0, s>>>(p);
+    join<float, D>(p, s);
 }
-template <int D> void backward(Params& p, int parts, hipStream_t s) {
+template <int D> void backward(const Params& p, hipStream_t s) {
     varlen_f32_dq_kernel<D><<<(unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, 1), NT, 0, s>>>(p);
-    p.nsplit = parts;
-    varlen_f32_dkv_kernel<D><<<(unsigned)work_groups(row_slots(p.tk, 1, p.n, ROWS), p.hk, parts), NT, 0, s>>>(p);
-    if (parts > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<float><<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
+    varlen_f32_dkv_kernel<D><<<(unsigned)work_groups(row_slots(p.tk, 1, p.n, ROWS), p.hk, p.nsplit), NT, 0, s>>>(p);
+    if (p.nsplit > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<float><<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
 }
 
 }  // namespace
 
 namespace dpipe_varlen {
 void forward_f32(const VarlenParams<float>& p, int D, hipStream_t s) { if (D == 64) forward<64>(p, s); else forward<128>(p, s); }
-void backward_f32(VarlenParams<float>& p, int D, int parts, hipStream_t s) { if (D == 64) backward<64>(p, parts, s); else backward<128>(p, parts, s); }
+void backward_f32(const VarlenParams<float>& p, int D, hipStream_t s) { if (D == 64) backward<64>(p, s); else backward<128>(p, s); }
 }  // namespace dpipe_varlen

@@ -1777,6 +1777,12 @@ def attention(q, k, v, kv_len=None, scale=None, impl='auto', causal=False):
     return _UnfusedAttnFn.apply(q, k, v, scale, causal, kv_len)
 
 
+@functools.lru_cache(maxsize=1024)
+def _varlen_floats(backward, sizes):
+    """fp32 workspace of a call of these sizes"""
+    return (lib().dpipe_attn_varlen_bwd_workspace_floats if backward else lib().dpipe_attn_varlen_fwd_workspace_floats)(*sizes)
+
+
 def _varlen_forward(q, k, v, cu_q, cu_k, scale, causal, keep):
     """-> (o, what the backward reads, what its call repeats); keep: the row statistics and what the output's rounding left are stored for the backward's P and delta"""
     device = q.device
@@ -1787,7 +1793,7 @@ def _varlen_forward(q, k, v, cu_q, cu_k, scale, causal, keep):
     o = _dense(q)
     dt = dtype_code(q.dtype)
     o_lo, lse = (torch.empty_like(o) if dt == hip.BF16 else None, q.new_empty((hq, tq), dtype=torch.float32)) if keep else (None, None)
-    need = lib().dpipe_attn_varlen_fwd_workspace_floats(*sizes)
+    need = _varlen_floats(False, sizes)
     ws = torch.empty(need, device=device, dtype=torch.float32) if need else None
     check(lib().dpipe_attn_varlen_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _addr(o_lo), _addr(lse), _addr(ws), need, *sizes,
                                       *strides, scale, causal, dt, hip.raw_stream(device)), 'attn_varlen_fwd')
@@ -1816,7 +1822,7 @@ class _AttnVarlenFn(Function):
             do, _, _, _, *ds = _head_rows(do)
             dq, dk, dv = _dense(q), _dense(k), _dense(v)
             delta = torch.empty_like(lse)
-            need = lib().dpipe_attn_varlen_bwd_workspace_floats(*sizes)
+            need = _varlen_floats(True, sizes)
             ws = torch.empty(need, device=device, dtype=torch.float32) if need else None
             check(lib().dpipe_attn_varlen_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _addr(o_lo), do.data_ptr(), lse.data_ptr(),
                                               delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _addr(ws), need, *sizes, *strides, *ds, scale, causal,
