@@ -9,9 +9,9 @@ using namespace dpipe;
 struct VarlenShape {
     const int *cu_q, *cu_k;
     float *lse, *delta;                  // [Hq][Tq]
-    float *part, *part_lse;              // split forms: forward rows [split][Tq][Hq][D] and their lse [split][Hq][Tq]; dK / dV [split][2][Tk][Hk][D]
+    float *part, *part_lse;              // split forms: forward rows [split][Tq][Hq][D] and their lse [split][Hq][Tq]; dQ [split][Tq][Hq][D], then dK / dV [split][2][Tk][Hk][D]
     long tq, tk;
-    int n, hq, hk, g, nsplit, causal;
+    int n, hq, hk, g, nsplit, dq_split, causal;
     long q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, do_ss, do_sh;    // o, dq, dk, dv are contiguous
     float scale;
 };
@@ -169,24 +169,23 @@ __global__ void __launch_bounds__(NT) varlen_join_kernel(const VarlenParams<T> p
     if (lane == 0 && p.lse) p.lse[at] = sum == 0.f ? INFINITY : base + __builtin_amdgcn_logf(sum);
 }
 
-// dK / dV = sum of the parts in order, one thread per 4 channels; HBM: 3 parts of 9377 keys x 8 heads x 128 in 43 us = 6.2 TB/s
+// sums of parts in order, one thread per 4 channels, one tensor per blockIdx.y; HBM: dK and dV of 9377 keys x 8 heads x 128 in 3 parts in 42 us = 6.4 TB/s
 template <typename T>
-__global__ void __launch_bounds__(256) varlen_dkv_sum_kernel(const VarlenParams<T> p, long elements) {
+__global__ void __launch_bounds__(256) varlen_sum_kernel(const float* __restrict__ part, T* first, T* second, int parts, long elements) {
     const long at = 4 * ((long)blockIdx.x * 256 + threadIdx.x);
     if (at >= elements) return;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
-#pragma unroll 4
-    for (int s = 0; s < p.nsplit; ++s) {
-        const float4 x = *reinterpret_cast<const float4*>(p.part + 2 * s * elements + at), y = *reinterpret_cast<const float4*>(p.part + (2 * s + 1) * elements + at);
-        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w; c.x += y.x; c.y += y.y; c.z += y.z; c.w += y.w;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < parts; ++s) {
+        const float4 x = *reinterpret_cast<const float4*>(part + ((long)s * gridDim.y + blockIdx.y) * elements + at);
+        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
     }
-    const float fa[4] = {a.x, a.y, a.z, a.w}, fc[4] = {c.x, c.y, c.z, c.w};
-    if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint2*>(p.dk + at) = make_uint2(pack_bf16x2(fa[0], fa[1]), pack_bf16x2(fa[2], fa[3]));
-        *reinterpret_cast<uint2*>(p.dv + at) = make_uint2(pack_bf16x2(fc[0], fc[1]), pack_bf16x2(fc[2], fc[3]));
-    } else {
-        *reinterpret_cast<float4*>(p.dk + at) = a; *reinterpret_cast<float4*>(p.dv + at) = c;
-    }
+    T* out = (blockIdx.y ? second : first) + at;
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+    else *reinterpret_cast<float4*>(out) = a;
+}
+template <typename T> void sum_parts(const VarlenParams<T>& p, T* first, T* second, int parts, long elements, hipStream_t s) {
+    varlen_sum_kernel<T><<<dim3((unsigned)cdiv(elements, 1024), second ? 2 : 1), 256, 0, s>>>(p.part, first, second, parts, elements);
 }
 
 inline int row_slots(long tokens, int g, int n, int per) { return (int)(tokens * g / per + n + 1); }

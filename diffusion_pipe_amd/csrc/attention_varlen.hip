@@ -158,6 +158,12 @@ __device__ __forceinline__ void store_row(bf16_t* dst, bf16_t* lo, const f32x16&
     }
 }
 
+// the same 32 channels in fp32, to a part
+__device__ __forceinline__ void store_part(float* dst, const f32x16& a, float scale, int h) {
+#pragma unroll
+    for (int eg = 0; eg < 4; ++eg) *reinterpret_cast<float4*>(dst + 8 * eg + 4 * h) = make_float4(a[4 * eg] * scale, a[4 * eg + 1] * scale, a[4 * eg + 2] * scale, a[4 * eg + 3] * scale);
+}
+
 // ================================================================================================ forward
 // 128 rows per workgroup of 4 waves, two workgroups per CU: one's softmax runs under the other's products without a barrier between them (8 waves of one workgroup: 3137 us where two
 // of 4 take 2991; 64 rows a wave, one wave a SIMD: 3733; the next tile's S issued before this one's softmax within a wave: 3977).  16 + 16 products of 32 cycles a tile against
@@ -271,11 +277,8 @@ __global__ void __launch_bounds__(NT, KR == KT ? 2 : 3) varlen_fwd_kernel(const 
     if (SPLIT && sum == 0.f) return;                           // the join does not read this row
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
-        if (!SPLIT) { store_row(p.o + row * D + 32 * db, p.o_lo ? p.o_lo + row * D + 32 * db : nullptr, oacc[db], inv, h); continue; }
-#pragma unroll
-        for (int eg = 0; eg < 4; ++eg)
-            *reinterpret_cast<float4*>(p.part + (part + row) * D + 32 * db + 8 * eg + 4 * h) =
-                make_float4(oacc[db][4 * eg] * inv, oacc[db][4 * eg + 1] * inv, oacc[db][4 * eg + 2] * inv, oacc[db][4 * eg + 3] * inv);
+        if (SPLIT) store_part(p.part + (part + row) * D + 32 * db, oacc[db], inv, h);
+        else store_row(p.o + row * D + 32 * db, p.o_lo ? p.o_lo + row * D + 32 * db : nullptr, oacc[db], inv, h);
     }
 }
 
@@ -284,11 +287,11 @@ __global__ void __launch_bounds__(NT, KR == KT ? 2 : 3) varlen_fwd_kernel(const 
 // nearly cancel in dS): the forward keeps what the rounding of O left in bf16 too, 17 bits in 4 bytes a channel and half the traffic of an fp32 copy beside O (9216 queries on 512
 // keys: forward 207 -> 169 us).
 // Per 64-key tile: K, read by rows (S^T = K . Q^T) and transposed (dQ^T += K^T . dS^T), and V by rows (dP^T = V . dO^T).
-template <int D>
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
     constexpr int NKS = D / 16, NDB = D / 32, IMG = KT * D * 2, STAGE = 2 * IMG;
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-    const Work w = find_work(blockIdx.x, p.hk, 1);
+    const Work w = find_work(blockIdx.x, p.hk, SPLIT ? p.dq_split : 1);
     const Tile t = find_tile<ROWS>(p, w.slot, false, p.causal);
     if (!t.live) return;
 
@@ -302,7 +305,11 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
     const long row = r.token * p.hq + r.head, at = r.head * p.tq + r.token;
     const float sl2 = p.scale * LOG2E;
 
-    const int nkt = (seen.group + KT - 1) / KT;
+    int kt0 = 0, nkt = (seen.group + KT - 1) / KT;
+    if (SPLIT) {                                               // every part of the sequence's key tiles, cut by its full length
+        const int all = (t.lk + KT - 1) / KT, per = (all + p.dq_split - 1) / p.dq_split;
+        kt0 = min(nkt, w.part * per); nkt = min(nkt, kt0 + per);
+    }
     Offsets<D, 4> oK, oV;
     oK.init(wid, lane, p.k_ss); oV.init(wid, lane, p.v_ss);
     auto issue = [&](int kt) {
@@ -310,7 +317,7 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
         oK.issue(rows_rsrc<D>(K, p.k_ss, kt * KT, t.lk), base, wid);
         oV.issue(rows_rsrc<D>(V, p.v_ss, kt * KT, t.lk), base + IMG, wid);
     };
-    if (nkt > 0) issue(0);
+    if (kt0 < nkt) issue(kt0);
     // One tensor after the other: a load takes 32 bytes of 32 rows, the next three the rest of the same lines, which the L1 holds for four lines of a tensor a row but not for four
     // tensors' at once (with the four interleaved: 304 MB in 147 us instead of 66; the kernel at 9277 tokens, 32 heads 350 -> 335 us, at 9216 queries on 512 keys 270 -> 240).
     // A lane behind the last row reads the sequence's first: its P is 0 (lse), and nothing of its column is stored.
@@ -328,12 +335,12 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
         for (int e = 0; e < 8; ++e) dl += (bf16_to_f32((bf16_t)oh[ks][e]) + bf16_to_f32((bf16_t)ol[ks][e])) * bf16_to_f32((bf16_t)dof[ks][e]);
     dl = sum_halves(dl);
     const float lse = r.live ? p.lse[at] : INFINITY;
-    if (r.live && h == 0) p.delta[at] = dl;
+    if (r.live && h == 0 && (!SPLIT || w.part == 0)) p.delta[at] = dl;
     f32x16 dq[NDB];
 #pragma unroll
     for (int db = 0; db < NDB; ++db) dq[db] = zero16();
 
-    for (int kt = 0; kt < nkt; ++kt) {
+    for (int kt = kt0; kt < nkt; ++kt) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         if (kt + 1 < nkt) issue(kt + 1);
@@ -373,7 +380,9 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
     }
     if (!r.live) return;
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) store_row(p.dq + row * D + 32 * db, nullptr, dq[db], p.scale, h);
+    for (int db = 0; db < NDB; ++db) {
+        if (SPLIT) store_part(p.part + (w.part * p.tq * p.hq + row) * D + 32 * db, dq[db], p.scale, h); else store_row(p.dq + row * D + 32 * db, nullptr, dq[db], p.scale, h);
+    }
 }
 
 // ================================================================================================ backward: dK, dV
@@ -540,6 +549,12 @@ int fwd_splits(long tq, long tk, int n, int hq, int hk, int D) {
 }
 // keys of a dK / dV workgroup: 8 waves at D = 128, whose K image and registers leave room for one workgroup per CU, 4 at 64
 constexpr int key_tile(int D) { return D == 128 ? 256 : 128; }
+// parts of the key range for dQ, D = 128 / 64: 1.55 / 1.2 us a tile.  With the sum, us, whole / as chosen: 4096 tokens, 4 heads
+// of 128: 106 / 76; 500 queries on 4000 + 3000 keys, 8 heads: 98 / 43; 3000 causal tokens, 3 / 1 heads of 64: 54 / 28; 2048 tokens, 10 heads of 128: 58 / 58
+int dq_splits(long tq, long tk, int n, int hq, int hk, int D) {
+    const long rows = tq * (hq / hk);
+    return best_parts(cdiv(rows, ROWS), rows, hk, tk / n / KT, n, {D == 128 ? 1.55f : 1.2f, D == 128 ? 0.94f : 0.75f, 8.f, 6.f, 1.6f * (tq * hq * (float)D * 1e-6f), D == 128 ? 2 : 3});
+}
 // parts of the query tiles (of all g heads) for dK / dV, D = 128 / 64: 3.0 / 1.6 us a tile.  With grouped heads up to g parts also where the key tiles alone are fewer than 3 a CU and the
 // sequences long enough that the parts' fp32 sums do not cost more than the balance gives (4 x 2048 causal tokens, 32 / 8 heads, backward: 648 -> 604 us; 16 x 512: 310 unsplit, 332 split)
 int dkv_splits(long tq, long tk, int n, int hq, int hk, int D) {
@@ -562,7 +577,8 @@ int fill(VarlenParams<T>& p, const char* what, const void* q, const void* k, con
     if (D != 64 && D != 128) return bad("head dim must be 64 or 128", DPIPE_ERR_UNSUPPORTED);
     if (!(scale > 0.f) || scale > 1e30f) return bad("scale must be positive and finite");
     p.nsplit = backward ? dkv_splits(tq, tk, n, hq, hk, D) : fwd_splits(tq, tk, n, hq, hk, D);
-    if (tq * (hq / hk) >= (1l << 31) - 256 || tk >= (1l << 31) - 256 || work_groups(tq * (hq / hk) / ROWS + n + 1, hk, backward ? 1 : p.nsplit) >= (1l << 23) ||
+    p.dq_split = backward ? dq_splits(tq, tk, n, hq, hk, D) : 1;
+    if (tq * (hq / hk) >= (1l << 31) - 256 || tk >= (1l << 31) - 256 || work_groups(tq * (hq / hk) / ROWS + n + 1, hk, backward ? p.dq_split : p.nsplit) >= (1l << 23) ||
         (backward && work_groups(tk / ROWS + n + 1, hk, p.nsplit) >= (1l << 23)))
         return bad("too many rows or sequences", DPIPE_ERR_UNSUPPORTED);
     if (!rows_ok(q, q_ss, q_sh, D) || !rows_ok(k, k_ss, k_sh, D) || !rows_ok(v, v_ss, v_sh, D)) return bad("tensors must be 16-byte aligned with strides multiple of 8 elements");
@@ -579,11 +595,18 @@ template <int D> void forward(const Params& p, hipStream_t s) {
     join<bf16_t, D>(p, s);
 }
 template <int D> void backward(const Params& p, hipStream_t s) {
-    varlen_dq_kernel<D><<<(unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, 1), NT, 0, s>>>(p);
+    const unsigned rows = (unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, p.dq_split);
+    if (p.dq_split == 1) varlen_dq_kernel<D, false><<<rows, NT, 0, s>>>(p);
+    else { varlen_dq_kernel<D, true><<<rows, NT, 0, s>>>(p); sum_parts(p, p.dq, (bf16_t*)nullptr, p.dq_split, p.tq * p.hq * D, s); }
     constexpr int NW = key_tile(D) / 32;
-    const unsigned grid = (unsigned)work_groups(row_slots(p.tk, 1, p.n, 32 * NW), p.hk, p.nsplit);
-    if (p.tk / p.n <= KT) varlen_dkv_kernel<D, NW, true><<<grid, 64 * NW, 0, s>>>(p); else varlen_dkv_kernel<D, NW, false><<<grid, 64 * NW, 0, s>>>(p);
-    if (p.nsplit > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<bf16_t><<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
+    const unsigned keys = (unsigned)work_groups(row_slots(p.tk, 1, p.n, 32 * NW), p.hk, p.nsplit);
+    if (p.tk / p.n <= KT) varlen_dkv_kernel<D, NW, true><<<keys, 64 * NW, 0, s>>>(p); else varlen_dkv_kernel<D, NW, false><<<keys, 64 * NW, 0, s>>>(p);
+    if (p.nsplit > 1) sum_parts(p, p.dk, p.dv, p.nsplit, p.tk * p.hk * D, s);
+}
+// fp32 values of the parts: dQ's are summed before dK's and dV's are written
+long bwd_floats(long tq, long tk, int hq, int hk, int D, int dq_parts, int dkv_parts) {
+    const long a = dq_parts > 1 ? dq_parts * tq * hq * D : 0, b = dkv_parts > 1 ? 2l * dkv_parts * tk * hk * D : 0;
+    return a > b ? a : b;
 }
 
 }  // namespace
@@ -597,8 +620,7 @@ long dpipe_attn_varlen_fwd_workspace_floats(long tq, long tk, int n, int hq, int
 }
 long dpipe_attn_varlen_bwd_workspace_floats(long tq, long tk, int n, int hq, int hk, int D) {
     if (tq <= 0 || tk <= 0 || n <= 0 || hq <= 0 || hk <= 0 || hq % hk || (D != 64 && D != 128)) return 0;
-    const int s = dkv_splits(tq, tk, n, hq, hk, D);
-    return s > 1 ? 2l * s * tk * hk * D : 0;
+    return bwd_floats(tq, tk, hq, hk, D, dq_splits(tq, tk, n, hq, hk, D), dkv_splits(tq, tk, n, hq, hk, D));
 }
 
 int dpipe_attn_varlen_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, void* o_lo, float* lse, float* ws, long ws_floats, long tq,
@@ -632,7 +654,7 @@ int dpipe_attn_varlen_bwd(const void* q, const void* k, const void* v, const int
         VarlenParams<T> p = {};
         const int rc = fill(p, "dpipe_attn_varlen_bwd", q, k, v, cu_q, cu_k, tq, tk, n, hq, hk, D, q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, scale, causal, true);
         if (rc) return rc;
-        const long need = p.nsplit > 1 ? 2l * p.nsplit * tk * hk * D : 0;
+        const long need = bwd_floats(tq, tk, hq, hk, D, p.dq_split, p.nsplit);
         if (!o || (sizeof(T) == 2 && !o_lo) || !dout || !lse || !delta || !dq || !dk || !dv || !aligned16(o) || !aligned16(o_lo) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
             !rows_ok(dout, do_ss, do_sh, D) || (need > 0 && (!ws || ws_floats < need || !aligned16(ws)))) {
             set_last_error("dpipe_attn_varlen_bwd: bad gradient or workspace"); return DPIPE_ERR_ARG; }

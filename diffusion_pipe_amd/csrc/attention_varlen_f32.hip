@@ -134,11 +134,11 @@ __global__ void __launch_bounds__(NT, 2) varlen_f32_fwd_kernel(const Params p) {
     for (int db = 0; db < NDB; ++db) store_row((SPLIT ? p.part + part * D : p.o) + row * D + 32 * db, o[db], inv, h);
 }
 
-template <int D>
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(NT, 2) varlen_f32_dq_kernel(const Params p) {
     constexpr int NDB = D / 32;
     __shared__ __attribute__((aligned(16))) float Kl[KT * (D + 2)], Vl[KT * (D + 2)];
-    const Work w = find_work(blockIdx.x, p.hk, 1);
+    const Work w = find_work(blockIdx.x, p.hk, SPLIT ? p.dq_split : 1);
     const Tile t = find_tile<ROWS>(p, w.slot, false, p.causal);
     if (!t.live) return;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
@@ -157,20 +157,25 @@ __global__ void __launch_bounds__(NT, 2) varlen_f32_dq_kernel(const Params p) {
     q.load(p.q + r.token * p.q_ss + r.head * p.q_sh, h, r.live);
     dl = sum_halves(dl);
     const float lse = r.live ? p.lse[at] : INFINITY;
-    if (r.live && h == 0) p.delta[at] = dl;
+    if (r.live && h == 0 && (!SPLIT || w.part == 0)) p.delta[at] = dl;
     f32x16 dq[NDB];
 #pragma unroll
     for (int db = 0; db < NDB; ++db) dq[db] = zero16();
+    int k0 = 0, k1 = seen.group;
+    if (SPLIT) {
+        const int per = ((t.lk + KT - 1) / KT + p.dq_split - 1) / p.dq_split * KT;
+        k0 = min((long)k1, (long)w.part * per); k1 = min(k1, k0 + per);
+    }
     const float *kp = p.k + t.k0 * p.k_ss + w.head * p.k_sh, *vp = p.v + t.k0 * p.v_ss + w.head * p.v_sh;
     Staged<D> ks, vs;
     constexpr bool AHEAD = D == 64;                            // (D = 128: the other workgroup of the CU computes meanwhile)
-    if (AHEAD) { ks.load(kp, p.k_ss, 0, seen.group); vs.load(vp, p.v_ss, 0, seen.group); }
-    for (int key0 = 0; key0 < seen.group; key0 += KT) {
-        if (!AHEAD) { ks.load(kp, p.k_ss, key0, seen.group); vs.load(vp, p.v_ss, key0, seen.group); }
+    if (AHEAD) { ks.load(kp, p.k_ss, k0, k1); vs.load(vp, p.v_ss, k0, k1); }
+    for (int key0 = k0; key0 < k1; key0 += KT) {
+        if (!AHEAD) { ks.load(kp, p.k_ss, key0, k1); vs.load(vp, p.v_ss, key0, k1); }
         __syncthreads();
         ks.store(Kl); vs.store(Vl);
         __syncthreads();
-        if (AHEAD) { ks.load(kp, p.k_ss, key0 + KT, seen.group); vs.load(vp, p.v_ss, key0 + KT, seen.group); }
+        if (AHEAD) { ks.load(kp, p.k_ss, key0 + KT, k1); vs.load(vp, p.v_ss, key0 + KT, k1); }
         if (key0 >= seen.wave) continue;
         f32x16 s = over_channels<D>(Kl, q, lane);
         const f32x16 dp = over_channels<D>(Vl, d, lane);
@@ -180,7 +185,7 @@ __global__ void __launch_bounds__(NT, 2) varlen_f32_dq_kernel(const Params p) {
     }
     if (!r.live) return;
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) store_row(p.dq + row * D + 32 * db, dq[db], p.scale, h);
+    for (int db = 0; db < NDB; ++db) store_row((SPLIT ? p.part + w.part * p.tq * p.hq * D : p.dq) + row * D + 32 * db, dq[db], p.scale, h);
 }
 
 template <int D>
@@ -255,9 +260,11 @@ template <int D> void forward(const Params& p, hipStream_t s) {
     join<float, D>(p, s);
 }
 template <int D> void backward(const Params& p, hipStream_t s) {
-    varlen_f32_dq_kernel<D><<<(unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, 1), NT, 0, s>>>(p);
+    const unsigned rows = (unsigned)work_groups(row_slots(p.tq, p.g, p.n, ROWS), p.hk, p.dq_split);
+    if (p.dq_split == 1) varlen_f32_dq_kernel<D, false><<<rows, NT, 0, s>>>(p);
+    else { varlen_f32_dq_kernel<D, true><<<rows, NT, 0, s>>>(p); sum_parts(p, p.dq, (float*)nullptr, p.dq_split, p.tq * p.hq * D, s); }
     varlen_f32_dkv_kernel<D><<<(unsigned)work_groups(row_slots(p.tk, 1, p.n, ROWS), p.hk, p.nsplit), NT, 0, s>>>(p);
-    if (p.nsplit > 1) { const long e = p.tk * p.hk * D; varlen_dkv_sum_kernel<float><<<(unsigned)cdiv(e, 1024), 256, 0, s>>>(p, e); }
+    if (p.nsplit > 1) sum_parts(p, p.dk, p.dv, p.nsplit, p.tk * p.hk * D, s);
 }
 
 }  // namespace
