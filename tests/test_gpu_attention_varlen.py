@@ -123,11 +123,12 @@ def test_fp32_forward_and_gradients(gpu, case, D):
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
 @pytest.mark.parametrize('D', [64, 128])
 def test_few_rows_against_long_keys(gpu, D, dtype):
-    """the key range is split over workgroups and joined; some sequences are shorter than the parts"""
+    """the key range is split over workgroups and joined, in the forward and in dQ; some sequences are shorter than the parts"""
     lens_q, lens_k = [1, 3, 1, 1], [9001, 4096, 63, 1]
     data = _inputs(gpu, lens_q, lens_k, 16, 4, D, dtype=dtype)
     from diffusion_pipe_amd import hip
     assert hip.lib().dpipe_attn_varlen_fwd_workspace_floats(data[0].shape[0], data[1].shape[0], 4, 16, 4, D) > 0
+    assert hip.lib().dpipe_attn_varlen_bwd_workspace_floats(data[0].shape[0], data[1].shape[0], 4, 16, 4, D) > 0
     for causal in (True, False):
         _check(_run(*data, causal), _exact(*data[:4], lens_q, lens_k, causal, 1.0 / math.sqrt(D)), f'few rows D={D} causal={causal}', dtype)
 

@@ -132,5 +132,7 @@ def test_workspace_is_asked_for_where_few_tiles_meet_a_long_axis():
     from diffusion_pipe_amd import hip
     fwd, bwd = hip.lib().dpipe_attn_varlen_fwd_workspace_floats, hip.lib().dpipe_attn_varlen_bwd_workspace_floats
     assert fwd(4, 20000, 2, 8, 2, 128) > 0 and bwd(20000, 77, 1, 8, 8, 128) > 0
+    assert bwd(500, 7000, 2, 8, 8, 128) > 0 and bwd(500, 7000, 2, 8, 8, 128) % (500 * 8 * 128) == 0      # (dQ's parts)
+    assert fwd(8000, 512, 1, 4, 4, 128) == 0 and fwd(77, 77, 1, 12, 12, 64) == 0 == bwd(77, 77, 1, 12, 12, 64)
     assert fwd(20000, 20000, 2, 24, 24, 128) == 0 and bwd(20000, 20000, 2, 24, 24, 128) == 0
     assert fwd(4, 100, 2, 8, 2, 128) == 0 and fwd(0, 5, 1, 1, 1, 64) == 0 and bwd(5, 5, 1, 3, 2, 64) == 0
