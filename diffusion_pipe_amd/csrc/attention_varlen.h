@@ -81,6 +81,7 @@ __device__ __forceinline__ Tile find_tile(const VarlenShape& p, int slot, bool k
     t.row0 = (long)(reversed ? nt - 1 - at : at) * PER;
     t.q0 = keys ? o0 : s0; t.k0 = keys ? s0 : o0;
     t.lq = keys ? o1 - o0 : s1 - s0; t.lk = keys ? s1 - s0 : o1 - o0;
+    if (keys && p.causal && t.lq > t.lk) { t.q0 += t.lq - t.lk; t.lq = t.lk; }      // (dK / dV) the queries in front see no key: not read, what they hold is 0 * NaN to nobody
     return t;
 }
 

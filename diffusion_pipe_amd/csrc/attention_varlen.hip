@@ -275,6 +275,10 @@ __global__ void __launch_bounds__(NT, KR == KT ? 2 : 3) varlen_fwd_kernel(const 
     const long row = r.token * p.hq + r.head, at = r.head * p.tq + r.token, part = SPLIT ? w.part * p.tq * p.hq : 0;
     if (h == 0 && (SPLIT || p.lse)) (SPLIT ? p.part_lse + part : p.lse)[at] = lse;
     if (SPLIT && sum == 0.f) return;                           // the join does not read this row
+    if (r.last < 0) {                                          // sees no key: 0, also where its neighbours' keys are not finite
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) oacc[db] = zero16();
+    }
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
         if (SPLIT) store_part(p.part + (part + row) * D + 32 * db, oacc[db], inv, h);
@@ -379,6 +383,10 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
         }
     }
     if (!r.live) return;
+    if (r.last < 0) {                                          // sees no key: 0, whatever it and its gradient hold
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) dq[db] = zero16();
+    }
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
         if (SPLIT) store_part(p.part + (w.part * p.tq * p.hq + row) * D + 32 * db, dq[db], p.scale, h); else store_row(p.dq + row * D + 32 * db, nullptr, dq[db], p.scale, h);

@@ -130,6 +130,10 @@ __global__ void __launch_bounds__(NT, 2) varlen_f32_fwd_kernel(const Params p) {
     const float lse = sum == 0.f ? (SPLIT ? -INFINITY : INFINITY) : m + __builtin_amdgcn_logf(sum);
     if (h == 0 && (SPLIT || p.lse)) (SPLIT ? p.part_lse + part : p.lse)[at] = lse;
     if (SPLIT && sum == 0.f) return;
+    if (r.last < 0) {                                          // sees no key: 0, also where its neighbours' keys are not finite
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[db] = zero16();
+    }
 #pragma unroll
     for (int db = 0; db < NDB; ++db) store_row((SPLIT ? p.part + part * D : p.o) + row * D + 32 * db, o[db], inv, h);
 }
@@ -184,6 +188,10 @@ __global__ void __launch_bounds__(NT, 2) varlen_f32_dq_kernel(const Params p) {
         over_rows<D>(dq, Kl, s, lane);
     }
     if (!r.live) return;
+    if (r.last < 0) {
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) dq[db] = zero16();
+    }
 #pragma unroll
     for (int db = 0; db < NDB; ++db) store_row((SPLIT ? p.part + w.part * p.tq * p.hq * D : p.dq) + row * D + 32 * db, dq[db], p.scale, h);
 }

@@ -1838,8 +1838,8 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=False):
     of which may be empty.  cu_k None: the queries' offsets (Tk = Tq).  The lengths are never read on the host: the call can be captured and replayed with other offsets.
     (As with any operator: while its backward pass is captured, no eager graph of the same leaf tensors may be alive -- their accumulation nodes would run on that graph's stream.)
     causal: query i sees key j of its sequence when j - len_k <= i - len_q (the last query sees every key; with equal lengths j <= i).
-    A query that sees no key, and the rows behind the last sequence, give zeros and take and give no gradient, whatever those rows hold (values INSIDE a sequence are expected to be
-    finite: a masked infinity or NaN reaches its sequence's other rows).  The same inputs give the same bits (no atomics).  (models/wan/attention.py:91-122)
+    A query that sees no key, and the rows behind the last sequence, give zeros and take and give no gradient, whatever those rows hold (the other values of a sequence are expected
+    to be finite: an infinity or NaN reaches its sequence's other rows, also where it is masked).  The same inputs give the same bits (no atomics).  (models/wan/attention.py:91-122)
     -> [Tq, H, D]"""
     cu_k = cu_q if cu_k is None else cu_k
     qs, ks, dtype = q.shape, k.shape, q.dtype
