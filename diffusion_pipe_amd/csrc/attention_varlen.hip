@@ -44,9 +44,11 @@ constexpr int KT = 64;                   // keys (dK / dV: queries) per LDS tile
 constexpr int AQ = 4, AK = 1;            // steps of LDS operands read ahead of their products in the dQ and the dK / dV kernels
 // CORNER: in a row of few keys (a column of few queries) nothing averages the rounding of P and dS away, and the forward's reaches the row's dS through delta.  The forward and dQ
 // therefore multiply what the rounding of a sequence's first tile of keys left as well: one tile in lk / 64 (long sequences: within 1 %), and the rows that only see that tile, which
-// in causal sequences carry the largest gradients, are rounded once.  dK / dV do it for the first tile of keys against the first of queries where the sequences average at most one
-// tile (a variant: its registers cost the long ones 8 %, at D = 64 30 %).  Error against 64 bits, dQ / dK / dV, 24 causal sequences of 1 - 2 tokens: 2.53e-3 / 2.32e-3 / 1.82e-3 ->
-// 1.7e-3 each (one rounding); 457 + 16 + 32 + 172 + 208 causal tokens: dQ 2.40e-3 -> 1.8e-3.
+// in causal sequences carry the largest gradients, are rounded once.  dK / dV do it for sequences of one tile of keys and one of queries (those that see keys), whatever else is in
+// the batch: they walk their tiles twice, the second time with what the rounding left (64 sequences of 64 tokens, 24 heads of 128, forward and backward: 127 -> 133 us against a kernel
+// for batches of short sequences only; longer sequences as without it.  The second products behind the first in the same pass cost the long ones 8 % in registers, at D = 64 30 %; a
+// second body for short sequences in the kernel 2 %; the second walk inside a tile's iteration 4 %).  Error against 64 bits, dQ / dK / dV, 24 causal sequences of 1 - 2 tokens:
+// 2.53e-3 / 2.32e-3 / 1.82e-3 -> 1.7e-3 each (one rounding); 457 + 16 + 32 + 172 + 208 causal tokens: dQ 2.40e-3 -> 1.8e-3.
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, long bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
@@ -135,6 +137,15 @@ __device__ __forceinline__ bf16x8_t pack_rest(const f32x16& s, int e0) {
         r[i] = pack_bf16x2(x - __uint_as_float(w << 16), y - __uint_as_float(w & 0xffff0000u));
     }
     return __builtin_bit_cast(bf16x8_t, make_uint4(r[0], r[1], r[2], r[3]));
+}
+
+// the same in place, for a whole tile
+__device__ __forceinline__ void rounding_left(f32x16& s) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+        const uint32_t w = pack_bf16x2(s[e], s[e + 1]);
+        s[e] -= __uint_as_float(w << 16); s[e + 1] -= __uint_as_float(w & 0xffff0000u);
+    }
 }
 
 // 32 channels of a lane's row from a transposed accumulator (the lane holds channels 8 e + 4 h + 0 .. 3): halves exchanged with lane ^ 32, two 16-byte stores a lane.
@@ -398,8 +409,8 @@ __global__ void __launch_bounds__(NT, 2) varlen_dq_kernel(const Params p) {
 // and dO, both read by rows and transposed, and the tile's lse / delta.  Query rows past the sequence arrive as zeros (Q, dO, lse, delta): P = 1 there, but dO = 0 and dS = 0.
 // One kernel for dK and dV shares S and P between them (two kernels made 5 products instead of 4: 7764 -> 6134 us on the longest case above); K in LDS instead of registers gives the
 // operands room one step ahead of their products (5992 -> 5640).  At D = 128 its 8 waves are two a SIMD and the LDS of a CU; 4 waves at D = 64, three a SIMD.
-template <int D, int NW, bool CORNER>
-__global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dkv_kernel(const Params p) {
+template <int D, int NW>
+__global__ void __launch_bounds__(NW * 64, D == 64 ? 3 : 2) varlen_dkv_kernel(const Params p) {
     constexpr int QT = KT, NKS = D / 16, NDB = D / 32, IMG = QT * D * 2, O_STAT = 2 * IMG, STAGE = O_STAT + 1024;
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE + NW / 2 * IMG];
     const Work w = find_work(blockIdx.x, p.hk, p.nsplit);
@@ -415,7 +426,8 @@ __global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dk
     const int first = p.causal ? max(0, (int)t.row0 - ahead) / QT * QT : 0;
     const int per_head = max(0, (t.lq - first + QT - 1) / QT);
     const long all = (long)per_head * p.g, per = (all + p.nsplit - 1) / p.nsplit;
-    const int it0 = (int)min(all, w.part * per), count = (int)min(all, it0 + per) - it0;
+    const int twice = t.lq <= KT && t.lk <= KT ? 1 : 0;       // (CORNER) every tile once more, with what the rounding left
+    const int it0 = (int)min(all, w.part * per), count = ((int)min(all, it0 + per) - it0) << twice;
     int hd = per_head > 0 ? it0 / per_head : 0, q = first + (it0 - hd * per_head) * QT;      // of the tile to fetch next
     const bf16_t* Q = p.q + t.q0 * p.q_ss + w.head * p.g * p.q_sh;
     const bf16_t* DO = p.dout + t.q0 * p.do_ss + w.head * p.g * p.do_sh;
@@ -450,8 +462,11 @@ __global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dk
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         const int qt = q;                                      // the tile at hand
-        q += QT;
-        if (q >= t.lq) { q = first; ++hd; }
+        const bool rest = twice & it;
+        if (!twice || rest) {
+            q += QT;
+            if (q >= t.lq) { q = first; ++hd; }
+        }
         if (it + 1 < count) issue((it + 1) & 1);
         const char* Ql = lds + (it & 1) * STAGE;
         const char* DOl = Ql + IMG;
@@ -491,16 +506,7 @@ __global__ void __launch_bounds__(NW * 64, D == 64 && !CORNER ? 3 : 2) varlen_dk
                     s[e] = pr[e] * (dp[e] - dd[j]);
                 }
             }
-            if (CORNER && qt == 0 && k0w < KT) {
-                const bf16x8_t pl[2] = {pack_rest(pr, 0), pack_rest(pr, 8)}, sl[2] = {pack_rest(s, 0), pack_rest(s, 8)};
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int db = 0; db < NDB; ++db) {
-                        dv[db] = mfma16(by_cols(DOl, 32 * db, 32 * qb + 16 * u, lane), pl[u], dv[db]);
-                        dk[db] = mfma16(by_cols(Ql, 32 * db, 32 * qb + 16 * u, lane), sl[u], dk[db]);
-                    }
-            }
+            if (rest) { rounding_left(pr); rounding_left(s); }
             const bf16x8_t pf[2] = {pack_frag(pr, 0), pack_frag(pr, 8)}, ds[2] = {pack_frag(s, 0), pack_frag(s, 8)};
             products_first<D>(true);
             __builtin_amdgcn_sched_barrier(0);
@@ -608,7 +614,7 @@ template <int D> void backward(const Params& p, hipStream_t s) {
     else { varlen_dq_kernel<D, true><<<rows, NT, 0, s>>>(p); sum_parts(p, p.dq, (bf16_t*)nullptr, p.dq_split, p.tq * p.hq * D, s); }
     constexpr int NW = key_tile(D) / 32;
     const unsigned keys = (unsigned)work_groups(row_slots(p.tk, 1, p.n, 32 * NW), p.hk, p.nsplit);
-    if (p.tk / p.n <= KT) varlen_dkv_kernel<D, NW, true><<<keys, 64 * NW, 0, s>>>(p); else varlen_dkv_kernel<D, NW, false><<<keys, 64 * NW, 0, s>>>(p);
+    varlen_dkv_kernel<D, NW><<<keys, 64 * NW, 0, s>>>(p);
     if (p.nsplit > 1) sum_parts(p, p.dk, p.dv, p.nsplit, p.tk * p.hk * D, s);
 }
 // fp32 values of the parts: dQ's are summed before dK's and dV's are written
