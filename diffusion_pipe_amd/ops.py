@@ -10,7 +10,7 @@ import math
 import os as _os_mod
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import hip
 from .hip import ACT, DpipeHipError, check, dtype_code, lib, ptr, require_cuda, stream
@@ -1447,6 +1447,13 @@ def _one_device(*tensors):
     return device
 
 
+def _no_tangents(what, *tensors):
+    """Forward-mode derivatives are refused, not dropped: a dual tensor does not ask for a gradient, so it would take the path without autograd.  (The level is read first: no dual
+    level, no tangents, and nothing to unpack.)"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise DpipeHipError(f'{what}: forward-mode derivatives are not supported')
+
+
 @contextlib.contextmanager
 def _launching_on(device):
     """kernels are launched on the current device: make it the operands'"""
@@ -1549,7 +1556,7 @@ class _RopeAxesFn(Function):
 
 
 def rope_axes(q, k, positions, axes_dim, theta=10000.0, q_weight=None, k_weight=None, eps=1e-6, interleaved=True, shared=False):
-    """Rotary positions with several axes on query and key heads, optionally behind their per-head RMS norms, in one launch; differentiable in q, k and the weights.
+    """Rotary positions with several axes on query and key heads, optionally behind their per-head RMS norms, in one launch; differentiable in q, k and the weights (reverse mode).
 
     q [..., H, D], k [..., Hk, D] or None (bf16 or fp32, the same leading sizes; D a multiple of 8 up to 256; column blocks of a fused projection are read in place).
     positions [..., axes] (fp32, int32 or int64): one row per token, or one row per token of the innermost leading sizes, repeated over the outer ones ([S, axes] for q [B, S, H, D]).
@@ -1577,6 +1584,7 @@ def rope_axes(q, k, positions, axes_dim, theta=10000.0, q_weight=None, k_weight=
             raise DpipeHipError(f'rope_axes: norm weights have shape [{D}]; got {tuple(w.shape)}')
     if k is None and k_weight is not None:
         raise DpipeHipError('rope_axes: a key weight needs k')
+    _no_tangents('rope_axes', q, k, positions, q_weight, k_weight)
     q_weight, k_weight = (w if w is None or w.is_contiguous() else w.contiguous() for w in (q_weight, k_weight))
     args = (q, k, _contig(positions), q_weight, k_weight, tables, float(eps), 0 if interleaved else 1)
     with _on(_one_device(q, k, positions, q_weight, k_weight)):
@@ -1831,7 +1839,7 @@ class _AttnVarlenFn(Function):
 
 
 def attention_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=False):
-    """softmax(scale q k^T) v over sequences of different lengths packed back to back; bf16, or fp32 throughout, head dim 64 or 128, differentiable in q, k, v.
+    """softmax(scale q k^T) v over sequences of different lengths packed back to back; bf16, or fp32 throughout, head dim 64 or 128, differentiable in q, k, v (reverse mode).
 
     q [Tq, H, D], k / v [Tk, Hk, D] with H a multiple of Hk: query head h reads key head h // (H // Hk).  Column blocks of a fused projection are read in place.
     cu_q, cu_k: int32 offsets [N + 1] on the device, ascending from 0; sequence b holds query tokens cu_q[b] .. cu_q[b + 1] - 1 and key tokens cu_k[b] .. cu_k[b + 1] - 1, either
@@ -1855,6 +1863,7 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=False):
     scale = 1.0 / math.sqrt(qs[2]) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise DpipeHipError(f'attention_varlen: scale must be positive and finite, got {scale}')
+    _no_tangents('attention_varlen', q, k, v)
     device = _one_device(q, k, v, cu_q, cu_k)
     cu_q, cu_k = (cu if cu.dtype == torch.int32 and cu.is_contiguous() else cu.to(torch.int32).contiguous() for cu in (cu_q, cu_k))
     with _on(device):

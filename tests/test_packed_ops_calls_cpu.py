@@ -1,0 +1,34 @@
+"""CPU: calls of rope_axes and attention_varlen that are refused, or not, before anything touches a device."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+ROPE = {'q': (6, 4, 64), 'k': (6, 2, 64), 'positions': (6, 3), 'q_weight': (64,), 'k_weight': (64,)}
+ATTENTION = {'q': (6, 4, 64), 'k': (6, 2, 64), 'v': (6, 2, 64)}
+
+
+def _rope(t):
+    from diffusion_pipe_amd import ops
+    return ops.rope_axes(t['q'], t['k'], t['positions'], (8, 28, 28), q_weight=t['q_weight'], k_weight=t['k_weight'])
+
+
+def _attention(t):
+    from diffusion_pipe_amd import ops
+    return ops.attention_varlen(t['q'], t['k'], t['v'], torch.tensor([0, 2, 6], dtype=torch.int32))
+
+
+@pytest.mark.parametrize('call,shapes,name', [(c, s, n) for c, s in ((_rope, ROPE), (_attention, ATTENTION)) for n in s], ids=lambda x: x.strip('_') if isinstance(x, str) else '')
+def test_forward_mode_tangents_are_refused(call, shapes, name):
+    """a dual tensor does not require a gradient: its tangent must not vanish on the path without autograd"""
+    from diffusion_pipe_amd.hip import DpipeHipError
+    t = {n: torch.zeros(*s) for n, s in shapes.items()}
+    with fw.dual_level():
+        with pytest.raises(DpipeHipError, match='device tensors'):           # no tangent: as outside
+            call(t)
+        whole = fw.make_dual(torch.zeros(2, *shapes[name]), torch.ones(2, *shapes[name]))
+        for dual in (fw.make_dual(t[name], torch.ones_like(t[name])), whole[1]):       # (a view of a dual tensor is one)
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(DpipeHipError, match='forward-mode'):
+                    call({**t, name: dual})
+    with pytest.raises(DpipeHipError, match='device tensors'):
+        call(t)
