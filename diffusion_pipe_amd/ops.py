@@ -1849,17 +1849,18 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=False):
     A query that sees no key, and the rows behind the last sequence, give zeros and take and give no gradient, whatever those rows hold (the other values of a sequence are expected
     to be finite: an infinity or NaN reaches its sequence's other rows, also where it is masked).  The same inputs give the same bits (no atomics).  (models/wan/attention.py:91-122)
     -> [Tq, H, D]"""
-    cu_k = cu_q if cu_k is None else cu_k
     qs, ks, dtype = q.shape, k.shape, q.dtype
     if len(qs) != 3 or len(ks) != 3 or ks != v.shape or ks[2] != qs[2] or ks[1] == 0 or qs[1] == 0 or qs[1] % ks[1]:
         raise DpipeHipError(f'attention_varlen: q [Tq, H, D], k and v [Tk, Hk, D] with H a multiple of Hk; got {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}')
     if dtype not in (torch.bfloat16, torch.float32) or qs[2] not in (64, 128) or k.dtype != dtype or v.dtype != dtype:
         raise DpipeHipError(f'attention_varlen computes in bf16 or fp32 at head dim 64 or 128; got {dtype}, {k.dtype}, {v.dtype}, head dim {qs[2]}')
+    if cu_k is None:
+        if ks[0] != qs[0]:
+            raise DpipeHipError(f'attention_varlen: shared offsets need as many keys as queries; got {qs[0]} and {ks[0]}')
+        cu_k = cu_q
     for cu in (cu_q, cu_k):
         if cu.dtype not in (torch.int32, torch.int64) or cu.dim() != 1 or cu.shape[0] < 2 or cu.shape[0] != cu_q.shape[0]:
             raise DpipeHipError(f'attention_varlen: offsets are int32 [N + 1], N >= 1, for queries and keys alike; got {cu.dtype} {tuple(cu.shape)}, {tuple(cu_q.shape)}')
-    if cu_k is cu_q and ks[0] != qs[0]:
-        raise DpipeHipError(f'attention_varlen: shared offsets need as many keys as queries; got {qs[0]} and {ks[0]}')
     scale = 1.0 / math.sqrt(qs[2]) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise DpipeHipError(f'attention_varlen: scale must be positive and finite, got {scale}')

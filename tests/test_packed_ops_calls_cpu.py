@@ -32,3 +32,15 @@ def test_forward_mode_tangents_are_refused(call, shapes, name):
                     call({**t, name: dual})
     with pytest.raises(DpipeHipError, match='device tensors'):
         call(t)
+
+
+def test_the_same_offsets_given_for_both_sides_allow_buffers_of_two_sizes():
+    """what is allowed goes by the offsets' values, not by which object holds them: rows behind the last sequence may differ in number"""
+    from diffusion_pipe_amd import ops
+    from diffusion_pipe_amd.hip import DpipeHipError
+    cu, (q, k) = torch.tensor([0, 2, 6], dtype=torch.int32), (torch.zeros(n, 2, 64) for n in (6, 9))
+    for cu_k in (cu, cu.clone()):
+        with pytest.raises(DpipeHipError, match='device tensors'):
+            ops.attention_varlen(q, k, k, cu, cu_k)
+    with pytest.raises(DpipeHipError, match='as many keys'):
+        ops.attention_varlen(q, k, k, cu)
