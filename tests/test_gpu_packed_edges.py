@@ -1,4 +1,5 @@
-"""ops.attention_varlen at its edges: rows that see no key and hold NaN, short sequences beside long ones.  Bounds: those of test_gpu_attention_varlen, element by element."""
+"""ops.attention_varlen and ops.rope_axes at their edges: rows that see no key and hold NaN, short sequences beside long ones, axes that are cut where a sequence has several row tiles,
+rows behind the last sequence where an axis is cut, and every buffer between guards.  Bounds: those of test_gpu_attention_varlen, element by element."""
 import math
 
 import pytest
@@ -68,3 +69,150 @@ def test_short_sequences_are_rounded_once_in_any_company(gpu, company, H, Hk, D,
         worst = ((t[:n].detach().double() - value).abs() / (bound + h * (value.abs() + bound))).max().item()
         print(f'{company} {x}: worst error / bound {worst:.3f}')
         assert worst <= 1.0, x
+
+
+# ------------------------------------------------------------------------------------------------ cut axes
+@BOTH
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('case', [([300, 200], [4000, 3000], 8, 8), ([129, 70, 1], [2500, 70, 3000], 8, 2), ([4096], [4096], 4, 4)], ids=['two_sequences', 'grouped', 'one_sequence'])
+def test_cut_axes_with_several_row_tiles(gpu, case, D, dtype):
+    """several tiles of rows and several parts of the keys at once, forward and dQ; causal: parts that begin behind everything a tile sees"""
+    from diffusion_pipe_amd import hip
+    lens_q, lens_k, H, Hk = case
+    data = av._inputs(gpu, lens_q, lens_k, H, Hk, D, dtype=dtype)
+    sizes = (sum(lens_q), sum(lens_k), len(lens_q), H, Hk, D)
+    assert hip.lib().dpipe_attn_varlen_fwd_workspace_floats(*sizes) > 0 and hip.lib().dpipe_attn_varlen_bwd_workspace_floats(*sizes) >= 2 * sum(lens_q) * H * D
+    for causal in (False, True):
+        first = av._run(*data, causal)
+        av._check(first, av._exact(*data[:4], lens_q, lens_k, causal, 1.0 / math.sqrt(D)), f'{case} D={D} causal={causal}', dtype)
+        again = av._run(*data, causal)
+        assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+@BOTH
+@pytest.mark.parametrize('case', [([1, 3, 2], [9001, 4096, 63], 16, 4, 128), ([3000, 1500], [77, 20], 4, 4, 64), ([300, 200], [4000, 3000], 8, 8, 128)],
+                         ids=['few_rows', 'few_keys', 'several_row_tiles'])
+def test_rows_behind_the_last_sequence_where_axes_are_cut(gpu, case, dtype):
+    lens_q, lens_k, H, Hk, D = case
+    q, k, v, do, cu_q, cu_k = av._inputs(gpu, lens_q, lens_k, H, Hk, D, tail_q=150, tail_k=300, dtype=dtype)
+    nq, nk = sum(lens_q), sum(lens_k)
+    for t, n in ((q, nq), (do, nq), (k, nk), (v, nk)):
+        t[n:] = NAN
+    for causal in (False, True):
+        got = av._run(q, k, v, do, cu_q, cu_k, causal)
+        for name, t in got.items():
+            assert (t[(nq if name in ('o', 'dq') else nk):] == 0).all(), name
+        want = av._exact(q[:nq], k[:nk], v[:nk], do[:nq], lens_q, lens_k, causal, 1.0 / math.sqrt(D))
+        av._check({n: t[:(nq if n in ('o', 'dq') else nk)] for n, t in got.items()}, want, f'{case} causal={causal}', dtype)
+
+
+# ------------------------------------------------------------------------------------------------ guards
+GUARD, MARK = 40, 2.0 ** 100            # rows (floats: 64 of them) on either side; a value that no result takes
+
+
+class _Guarded:
+    """an operand inside a larger buffer: NaN around what is read, a mark around (and in) what is written"""
+
+    def __init__(self, shape, dtype, device, data=None):
+        rows, rest = shape[0], tuple(shape[1:])
+        self.guard = GUARD if rest else 64
+        self.read = data is not None
+        self.whole = torch.full((rows + 2 * self.guard, *rest), NAN if self.read else MARK, dtype=dtype, device=device)
+        self.t = self.whole[self.guard:self.guard + rows]
+        if self.read:
+            self.t.copy_(data)
+        assert self.t.data_ptr() % 16 == 0
+
+    def ptr(self):
+        return self.t.data_ptr()
+
+    def check(self, name):
+        outside = torch.cat([self.whole[:self.guard].flatten(), self.whole[self.guard + self.t.shape[0]:].flatten()])
+        assert (outside.isnan() if self.read else outside == MARK).all(), f'{name}: written outside'
+        assert self.t.isfinite().all(), f'{name}: what lies outside an operand was read'
+
+
+PLANS = [  # (query rows, key rows, query offsets, key offsets, H, Hk)
+    (200, 200, [0, 100, 200], None, 2, 2),
+    (290, 290, [0, 70, 200], None, 4, 2),
+    (200, 200, [0, 150, 100], None, 2, 1),                 # (from here on offsets that do not ascend from 0 to the end)
+    (200, 200, [0, -5, 900], None, 2, 2),
+    (200, 200, [0, 2000000000, -2000000000], None, 2, 2),
+    (200, 200, [50, 20, 200], None, 4, 1),
+    (200, 330, [0, 150, 100], [0, 400, 90], 2, 2),
+    (300, 300, [0] + [250, 3, -7, 300, 310, 120] * 8, None, 2, 1),
+    (7, 9100, [0, 1, 4], [0, 9001, 9050], 16, 4),          # cut keys
+    (7, 9100, [0, 9, 4], [0, 9001, 50], 16, 4),
+    (500, 7000, [0, 300, 500], [0, 4000, 7000], 8, 8),
+    (500, 7000, [0, 300, 200], [0, 8000, -1], 8, 8),
+    (4600, 97, [0, 3000, 4500], [0, 77, 97], 4, 4),        # cut queries
+    (4600, 97, [0, 3000, 100], [0, 100, -3], 4, 4),
+]
+
+
+@BOTH
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('plan', PLANS, ids=lambda p: f'{p[0]}x{p[1]}_{"_".join(map(str, p[2][:4]))}')
+def test_attention_stays_inside_its_buffers(gpu, plan, D, dtype):
+    """the C entries on operands, outputs and workspaces with guards on both sides, also where the offsets are wrong (their rows' values are then unspecified, their places are not)"""
+    from diffusion_pipe_amd import hip
+    tq, tk, cu_q, cu_k, H, Hk = plan
+    g = torch.Generator().manual_seed(tq + tk)
+    f32, lib = torch.float32, hip.lib()
+    make = lambda *s: _Guarded(s, dtype, gpu, torch.randn(*s, generator=g))
+    out = lambda *s, dt=dtype: _Guarded(s, dt, gpu)
+    cu_q, cu_k = (torch.tensor([0] * 8 + cu + [0] * 8, dtype=torch.int32, device=gpu)[8:8 + len(cu)] for cu in (cu_q, cu_k or cu_q))
+    sizes = (tq, tk, cu_q.shape[0] - 1, H, Hk, D)
+    b = {'q': make(tq, H, D), 'k': make(tk, Hk, D), 'v': make(tk, Hk, D), 'do': make(tq, H, D), 'o': out(tq, H, D), 'o_lo': out(tq, H, D), 'lse': out(H * tq, dt=f32),
+         'delta': out(H * tq, dt=f32), 'dq': out(tq, H, D), 'dk': out(tk, Hk, D), 'dv': out(tk, Hk, D)}
+    need = lib.dpipe_attn_varlen_fwd_workspace_floats(*sizes), lib.dpipe_attn_varlen_bwd_workspace_floats(*sizes)
+    ws = [out(max(x, 4), dt=f32) for x in need]
+    p = {x: t.ptr() for x, t in b.items()}
+    strides = (H * D, D, Hk * D, D, Hk * D, D)
+    for causal in (0, 1):
+        for x in b.values():
+            if not x.read:
+                x.t.fill_(MARK)
+        code = hip.BF16 if dtype == torch.bfloat16 else hip.F32
+        hip.check(lib.dpipe_attn_varlen_fwd(p['q'], p['k'], p['v'], cu_q.data_ptr(), cu_k.data_ptr(), p['o'], p['o_lo'], p['lse'], ws[0].ptr(), need[0], *sizes, *strides,
+                                            1.0 / math.sqrt(D), causal, code, hip.stream()), 'fwd')
+        hip.check(lib.dpipe_attn_varlen_bwd(p['q'], p['k'], p['v'], cu_q.data_ptr(), cu_k.data_ptr(), p['o'], p['o_lo'], p['do'], p['lse'], p['delta'], p['dq'], p['dk'], p['dv'],
+                                            ws[1].ptr(), need[1], *sizes, *strides, H * D, D, 1.0 / math.sqrt(D), causal, code, hip.stream()), 'bwd')
+        torch.cuda.synchronize()
+        for name, x in b.items():
+            if name != 'lse':
+                x.check(name)
+        assert not b['lse'].t.isnan().any()
+        b['lse'].t.fill_(0.0)                              # (+inf for a row that sees nothing)
+        b['lse'].check('lse')
+        for i, x in enumerate(ws):
+            x.t.fill_(0.0)
+            x.check(f'workspace {i}')
+
+
+@BOTH
+@pytest.mark.parametrize('tokens,H,Hk,D,axes', [(1, 1, 1, 64, (8, 28, 28)), (133, 5, 2, 128, (16, 56, 56)), (37, 3, 0, 80, (16, 24, 24)), (2100, 4, 1, 256, (64,))])
+def test_rotary_positions_stay_inside_their_buffers(gpu, tokens, H, Hk, D, axes, dtype):
+    from diffusion_pipe_amd import hip, ops
+    g = torch.Generator().manual_seed(tokens)
+    f32, lib = torch.float32, hip.lib()
+    make = lambda *s, dt=dtype: _Guarded(s, dt, gpu, torch.randn(*s, generator=g))
+    hk = max(Hk, 1)
+    b = {'q': make(tokens, H, D), 'k': make(tokens, hk, D), 'gq': make(tokens, H, D), 'gk': make(tokens, hk, D), 'pos': make(tokens, len(axes), dt=f32), 'wq': make(D), 'wk': make(D),
+         'yq': _Guarded((tokens, H, D), dtype, gpu), 'yk': _Guarded((tokens, hk, D), dtype, gpu), 'dq': _Guarded((tokens, H, D), dtype, gpu), 'dk': _Guarded((tokens, hk, D), dtype, gpu),
+         'dwq': _Guarded((D,), dtype, gpu), 'dwk': _Guarded((D,), dtype, gpu), 'ws': _Guarded((lib.dpipe_rope_axes_workspace_floats(D),), f32, gpu)}
+    p = {n: x.ptr() for n, x in b.items()}
+    if not Hk:
+        p.update(k=None, gk=None, yk=None, dk=None, dwk=None, wk=None)
+    code = hip.BF16 if dtype == torch.bfloat16 else hip.F32
+    for half in (0, 1):
+        freq, axis, pairs = ops._rope_axes_tables(axes, 10000.0, False, D, half == 0)
+        for normed in (True, False):
+            wq, wk = (p['wq'], p['wk']) if normed else (None, None)
+            meta, strides = (tokens, tokens, len(axes), pairs, H, Hk, D), (H * D, D, Hk * D, D)
+            hip.check(lib.dpipe_rope_axes_fwd(p['q'], p['k'], p['pos'], 0, freq, axis, wq, wk, p['yq'], p['yk'], *meta, *strides, 1e-6, half, code, code, code, hip.stream()), 'fwd')
+            hip.check(lib.dpipe_rope_axes_bwd(p['q'], p['k'], p['gq'], p['gk'], p['pos'], 0, freq, axis, wq, wk, p['dq'], p['dk'], p['dwq'] if normed else None,
+                                              p['dwk'] if normed else None, p['ws'], *meta, *strides, *strides, 1e-6, half, code, code, code, 0, 0, hip.stream()), 'bwd')
+            torch.cuda.synchronize()
+            for name, x in b.items():
+                x.check(name)
