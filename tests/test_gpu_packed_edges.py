@@ -90,6 +90,21 @@ def test_cut_axes_with_several_row_tiles(gpu, case, D, dtype):
 
 
 @BOTH
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('case', [([1, 3] + [0] * 30, [9001, 500] + [0] * 30, 16, 4), ([2] + [1] * 39, [16001] + [50, 0, 130] * 13, 8, 2), ([5000] + [10, 0, 1] * 13, [200] + [0, 70, 3] * 13, 4, 4)],
+                         ids=['empty', 'short', 'long_queries'])
+def test_a_long_sequence_among_empty_and_short_ones(gpu, case, D, dtype):
+    """the axis is cut for the long one; the parts that the others do not need leave nothing behind"""
+    from diffusion_pipe_amd import hip
+    lens_q, lens_k, H, Hk = case
+    data = av._inputs(gpu, lens_q, lens_k, H, Hk, D, dtype=dtype)
+    sizes = (sum(lens_q), sum(lens_k), len(lens_q), H, Hk, D)
+    assert hip.lib().dpipe_attn_varlen_bwd_workspace_floats(*sizes) > 0 and (lens_q[0] > 100 or hip.lib().dpipe_attn_varlen_fwd_workspace_floats(*sizes) > 0)
+    for causal in (False, True):
+        av._check(av._run(*data, causal), av._exact(*data[:4], lens_q, lens_k, causal, 1.0 / math.sqrt(D)), f'{case} D={D} causal={causal}', dtype)
+
+
+@BOTH
 @pytest.mark.parametrize('case', [([1, 3, 2], [9001, 4096, 63], 16, 4, 128), ([3000, 1500], [77, 20], 4, 4, 64), ([300, 200], [4000, 3000], 8, 8, 128)],
                          ids=['few_rows', 'few_keys', 'several_row_tiles'])
 def test_rows_behind_the_last_sequence_where_axes_are_cut(gpu, case, dtype):

@@ -44,3 +44,18 @@ def test_the_same_offsets_given_for_both_sides_allow_buffers_of_two_sizes():
             ops.attention_varlen(q, k, k, cu, cu_k)
     with pytest.raises(DpipeHipError, match='as many keys'):
         ops.attention_varlen(q, k, k, cu)
+
+
+@pytest.mark.parametrize('n', [2, 4, 8, 16, 32, 64])
+def test_an_axis_is_cut_however_many_sequences_stand_beside_the_long_one(n):
+    """few rows against a long axis leave most of the card idle unless the axis is cut: neither empty sequences (offsets of a fixed capacity) nor short neighbours may talk the rule out
+    of it, and equal short sequences are left whole"""
+    from diffusion_pipe_amd import hip
+    fwd, bwd = hip.lib().dpipe_attn_varlen_fwd_workspace_floats, hip.lib().dpipe_attn_varlen_bwd_workspace_floats
+    for rows, keys, hq, hk, D in ((1, 8191, 32, 8, 128), (64, 30063, 32, 8, 128), (n, 16384 + 100 * n, 32, 8, 128), (8, 16384, 12, 12, 64)):
+        assert fwd(rows, keys, n, hq, hk, D) // (rows * hq * (D + 1)) >= 4, (rows, keys)
+        assert bwd(rows, keys, n, hq, hk, D) >= 4 * rows * hq * D, (rows, keys)
+    for rows, keys, heads, D in ((8000, 512, 4, 128), (4096, 512, 10, 64)):
+        assert bwd(rows, keys, n, heads, heads, D) >= 2 * 2 * keys * heads * D, (rows, keys)
+    assert fwd(77 * n, 77 * n, n, 12, 12, 64) == 0 == bwd(77 * n, 77 * n, n, 12, 12, 64)
+    assert fwd(1000 * n, 1000 * n, n, 24, 24, 128) == 0 == bwd(1000 * n, 1000 * n, n, 24, 24, 128)
