@@ -541,14 +541,14 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? 3 : 2) varlen_dkv_kernel(co
 // 89 / 89 (four parts 102); 2048 tokens, 12 heads of 64: 33 / 33 (three parts 45); 8000 queries on 512 keys, 4 heads: 21 / 21 (three parts 49).  dK / dV: 1000 tokens, 10 heads: 52 / 41;
 // 4096 tokens, 4 heads 190 / 94, 7 heads 198 / 147; 8000 queries on 512 keys 346 / 44; six causal sequences of 1000, 8 heads: 60 / 60 (three parts 94).
 // The average says nothing about one sequence among many: offsets of a fixed capacity end in empty sequences, and a long one may have short neighbours.  The other extreme is one
-// sequence that holds all rows and the whole axis, beside workgroups that find nothing to do (1 ns a sequence, head and part).  The parts are the fewest, from the average's choice on,
-// that are estimated at no more than twice the least time there.  32 / 8 heads of 128, by the average alone / as chosen, us a replayed call: 1 row on 8191 keys in offsets for 64 sequences 146 / 41
-// (for one 22), 64 rows on 30 063 keys in offsets for 64 527 / 141 (61), 64 single tokens, one on 16 384 keys and 63 on 100: 284 / 92; 8000 queries on 512 keys, 4 heads, in offsets
-// for 16, forward and backward 403 / 132 (91); 4096 + 15 x 64 causal tokens, 4 heads, 370 / 296.  What equal lengths pay for it: 64 single tokens on 512 keys each 29 / 39, on 2048 113 / 124,
-// 16 on 512 18 / 20; longer rows nothing (12 x 1000 tokens, 8 heads, 242 / 242).
+// sequence that holds all rows and the whole axis, beside workgroups that find nothing to do (1 ns a sequence, head and part; a quarter where there are more sequences than rows).  The
+// parts are the fewest, from the average's choice on, that are estimated at no more than twice the least time there.  By the average alone / as chosen, us a replayed call, 32 / 8 heads
+// of 128: 1 row on 8191 keys in offsets for 64 sequences 146 / 53 (for one 22), 64 rows on 30 063 keys in offsets for 64 527 / 141 (61), 64 single tokens, one on 16 384 keys and 63 on
+// 100, 284 / 92; 4 heads, forward and backward: 8000 queries on 512 keys in offsets for 16 403 / 132 (91), 4096 + 15 x 64 causal tokens 370 / 296.  What equal lengths pay for it: 64
+// single tokens on 512 keys each 29 / 39, on 2048 113 / 124, 16 on 512 18 / 20; longer rows nothing (12 x 1000 tokens, 8 heads, 242 / 242).
 struct SplitCost { float tile, share, once, sum, part; int per_cu; };
 int best_parts(long row_tiles, long rows, int heads, long tiles, long all_tiles, int n, const SplitCost& k) {      // tiles: a sequence's on average; all_tiles: the whole axis
-    const float cu = heads / 256.f, groups = row_tiles > n ? row_tiles : n < rows ? n : rows, idle = 1e-3f * heads * (n < rows ? n : rows);
+    const float cu = heads / 256.f, groups = row_tiles > n ? row_tiles : n < rows ? n : rows, idle = 1e-3f * heads * (n < rows ? n : 0.25f * n + 0.75f * rows);
     auto us = [&](int s) {
         const float x = n > 1 ? row_tiles * s * cu : ceilf(row_tiles * s * cu);
         return k.tile * tiles / s * fmaxf(n > 1 ? 1.5f : 1.f, k.share * x) + k.once * ceilf(groups * s * cu / k.per_cu) + (s > 1 ? k.sum + k.part * s : 0.f);
@@ -570,11 +570,15 @@ int best_parts(long row_tiles, long rows, int heads, long tiles, long all_tiles,
     while (best < most(all_tiles) && us_one(best) > 2.f * least) ++best;
     return best;
 }
+// no more parts than leave the grid below 2^23 workgroups
+constexpr long MAX_GROUPS = (1l << 23) - 1;
+int fitting(long parts, long slots, int heads) { const long most = MAX_GROUPS / work_groups(slots, heads, 1); return (int)(parts > most && parts > 1 ? (most > 1 ? most : 1) : parts); }
 // parts of the key range, D = 128 / 64: 1.2 / 0.85 us a tile (a workgroup's run over 64 tiles alone on its CU: 84 us, two to a CU 1.9 us a tile each)
 int fwd_splits(long tq, long tk, int n, int hq, int hk, int D) {
     const float m = tq * hq * (float)D * 1e-6f;               // (millions of partial results a part)
     const long rows = tq * (hq / hk);
-    return best_parts(cdiv(rows, ROWS), rows, hk, tk / n / KT, tk / KT, n, {D == 128 ? 1.2f : 0.85f, D == 128 ? 0.78f : 0.55f, 7.f, 5.5f + 2.5f * m, 1.5f * m, D == 128 ? 2 : 3});
+    const int s = best_parts(cdiv(rows, ROWS), rows, hk, tk / n / KT, tk / KT, n, {D == 128 ? 1.2f : 0.85f, D == 128 ? 0.78f : 0.55f, 7.f, 5.5f + 2.5f * m, 1.5f * m, D == 128 ? 2 : 3});
+    return fitting(s, rows / ROWS + n + 1, hk);
 }
 // keys of a dK / dV workgroup: 8 waves at D = 128, whose K image and registers leave room for one workgroup per CU, 4 at 64
 constexpr int key_tile(int D) { return D == 128 ? 256 : 128; }
@@ -582,7 +586,8 @@ constexpr int key_tile(int D) { return D == 128 ? 256 : 128; }
 // of 128: 106 / 76; 500 queries on 4000 + 3000 keys, 8 heads: 98 / 43; 3000 causal tokens, 3 / 1 heads of 64: 54 / 28; 2048 tokens, 10 heads of 128: 58 / 58
 int dq_splits(long tq, long tk, int n, int hq, int hk, int D) {
     const long rows = tq * (hq / hk);
-    return best_parts(cdiv(rows, ROWS), rows, hk, tk / n / KT, tk / KT, n, {D == 128 ? 1.55f : 1.2f, D == 128 ? 0.94f : 0.75f, 8.f, 6.f, 1.6f * (tq * hq * (float)D * 1e-6f), D == 128 ? 2 : 3});
+    const int s = best_parts(cdiv(rows, ROWS), rows, hk, tk / n / KT, tk / KT, n, {D == 128 ? 1.55f : 1.2f, D == 128 ? 0.94f : 0.75f, 8.f, 6.f, 1.6f * (tq * hq * (float)D * 1e-6f), D == 128 ? 2 : 3});
+    return fitting(s, rows / ROWS + n + 1, hk);
 }
 // parts of the query tiles (of all g heads) for dK / dV, D = 128 / 64: 3.0 / 1.6 us a tile.  With grouped heads up to g parts also where the key tiles alone are fewer than 3 a CU and the
 // sequences long enough that the parts' fp32 sums do not cost more than the balance gives (4 x 2048 causal tokens, 32 / 8 heads, backward: 648 -> 604 us; 16 x 512: 310 unsplit, 332 split)
@@ -591,7 +596,7 @@ int dkv_splits(long tq, long tk, int n, int hq, int hk, int D) {
     const float part = 3.1f * (tk * hk * (float)D * 1e-6f);
     long s = D == 128 ? best_parts(key_tiles, tk, hk, tiles, tq / KT * g, n, {3.0f, 1.0f, 6.f, 6.f, part, 1}) : best_parts(key_tiles, tk, hk, tiles, tq / KT * g, n, {1.6f, 0.55f, 6.f, 6.f, part, 3});
     if (wgs < 768 && g > 1 && tiles >= 16 * g) { long m = cdiv(768, wgs); if (m > g) m = g; if (m > s) s = m; }
-    return (int)(s > 64 ? 64 : s);
+    return fitting(s > 64 ? 64 : s, tk / ROWS + n + 1, hk);
 }
 
 bool rows_ok(const void* p, long ss, long sh, int D) {
@@ -607,8 +612,8 @@ int fill(VarlenParams<T>& p, const char* what, const void* q, const void* k, con
     if (!(scale > 0.f) || scale > 1e30f) return bad("scale must be positive and finite");
     p.nsplit = backward ? dkv_splits(tq, tk, n, hq, hk, D) : fwd_splits(tq, tk, n, hq, hk, D);
     p.dq_split = backward ? dq_splits(tq, tk, n, hq, hk, D) : 1;
-    if (tq * (hq / hk) >= (1l << 31) - 256 || tk >= (1l << 31) - 256 || work_groups(tq * (hq / hk) / ROWS + n + 1, hk, backward ? p.dq_split : p.nsplit) >= (1l << 23) ||
-        (backward && work_groups(tk / ROWS + n + 1, hk, p.nsplit) >= (1l << 23)))
+    if (tq * (hq / hk) >= (1l << 31) - 256 || tk >= (1l << 31) - 256 || work_groups(tq * (hq / hk) / ROWS + n + 1, hk, backward ? p.dq_split : p.nsplit) > MAX_GROUPS ||
+        (backward && work_groups(tk / ROWS + n + 1, hk, p.nsplit) > MAX_GROUPS))
         return bad("too many rows or sequences", DPIPE_ERR_UNSUPPORTED);
     if (!rows_ok(q, q_ss, q_sh, D) || !rows_ok(k, k_ss, k_sh, D) || !rows_ok(v, v_ss, v_sh, D)) return bad("tensors must be 16-byte aligned with strides multiple of 8 elements");
     p.q = (const T*)q; p.k = (const T*)k; p.v = (const T*)v; p.cu_q = cu_q; p.cu_k = cu_k; p.tq = tq; p.tk = tk; p.n = n; p.hq = hq; p.hk = hk; p.g = hq / hk;

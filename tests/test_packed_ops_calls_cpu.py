@@ -59,3 +59,16 @@ def test_an_axis_is_cut_however_many_sequences_stand_beside_the_long_one(n):
         assert bwd(rows, keys, n, heads, heads, D) >= 2 * 2 * keys * heads * D, (rows, keys)
     assert fwd(77 * n, 77 * n, n, 12, 12, 64) == 0 == bwd(77 * n, 77 * n, n, 12, 12, 64)
     assert fwd(1000 * n, 1000 * n, n, 24, 24, 128) == 0 == bwd(1000 * n, 1000 * n, n, 24, 24, 128)
+
+
+@pytest.mark.parametrize('sizes', [(1, 2584, 245673, 24, 24, 128), (1, 39237, 104819, 4, 4, 128), (100, 2 ** 21, 20000, 40, 40, 128), (2 ** 21, 100, 20000, 40, 40, 128), (64, 2 ** 22, 200000, 8, 8, 64)])
+def test_cutting_refuses_no_call_that_fits_whole(sizes):
+    """offsets for very many sequences: the parts are as many as the grid allows, one if need be.  (o is missing, so nothing is launched)"""
+    from diffusion_pipe_amd import hip
+    tq, tk, n, hq, hk, D = sizes
+    strides = (hq * D, D, hk * D, D, hk * D, D)
+    lib = hip.lib()
+    assert lib.dpipe_attn_varlen_fwd(256, 256, 256, 256, 256, None, None, None, None, 0, *sizes, *strides, 0.125, 0, hip.BF16, None) < 0
+    assert 'bad output or workspace' in lib.dpipe_last_error().decode()
+    assert lib.dpipe_attn_varlen_bwd(256, 256, 256, 256, 256, None, None, 256, 256, 256, 256, 256, 256, None, 0, *sizes, *strides, hq * D, D, 0.125, 0, hip.BF16, None) < 0
+    assert 'bad gradient or workspace' in lib.dpipe_last_error().decode()
