@@ -1454,6 +1454,12 @@ def _no_tangents(what, *tensors):
         raise DpipeHipError(f'{what}: forward-mode derivatives are not supported')
 
 
+def _no_second_graph(what):
+    """Called in a backward: the gradient has no gradient of its own here.  Asked to record one (create_graph), it refuses: a term of a second derivative would vanish from its sum."""
+    if torch.is_grad_enabled():
+        raise DpipeHipError(f'{what} is differentiable once: no graph of its gradient (create_graph)')
+
+
 @contextlib.contextmanager
 def _launching_on(device):
     """kernels are launched on the current device: make it the operands'"""
@@ -1522,6 +1528,7 @@ class _RopeAxesFn(Function):
 
     @staticmethod
     def backward(ctx, gq, gk):
+        _no_second_graph('rope_axes')
         q, k, positions, q_weight, k_weight = ctx.saved_tensors
         meta, strides, tail, (freq, axis, _) = ctx.call
         tokens, has_k, D, device = meta[0], meta[5] > 0, meta[6], gq.device
@@ -1556,7 +1563,7 @@ class _RopeAxesFn(Function):
 
 
 def rope_axes(q, k, positions, axes_dim, theta=10000.0, q_weight=None, k_weight=None, eps=1e-6, interleaved=True, shared=False):
-    """Rotary positions with several axes on query and key heads, optionally behind their per-head RMS norms, in one launch; differentiable in q, k and the weights (reverse mode).
+    """Rotary positions with several axes on query and key heads, optionally behind their per-head RMS norms, in one launch; differentiable once in q, k and the weights (reverse mode).
 
     q [..., H, D], k [..., Hk, D] or None (bf16 or fp32, the same leading sizes; D a multiple of 8 up to 256; column blocks of a fused projection are read in place).
     positions [..., axes] (fp32, int32 or int64): one row per token, or one row per token of the innermost leading sizes, repeated over the outer ones ([S, axes] for q [B, S, H, D]).
@@ -1820,6 +1827,7 @@ class _AttnVarlenFn(Function):
 
     @staticmethod
     def backward(ctx, do):
+        _no_second_graph('attention_varlen')
         device = do.device
         if ctx.call is None:
             *shapes, dtype = ctx.shapes
@@ -1839,7 +1847,7 @@ class _AttnVarlenFn(Function):
 
 
 def attention_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=False):
-    """softmax(scale q k^T) v over sequences of different lengths packed back to back; bf16, or fp32 throughout, head dim 64 or 128, differentiable in q, k, v (reverse mode).
+    """softmax(scale q k^T) v over sequences of different lengths packed back to back; bf16, or fp32 throughout, head dim 64 or 128, differentiable once in q, k, v (reverse mode).
 
     q [Tq, H, D], k / v [Tk, Hk, D] with H a multiple of Hk: query head h reads key head h // (H // Hk).  Column blocks of a fused projection are read in place.
     cu_q, cu_k: int32 offsets [N + 1] on the device, ascending from 0; sequence b holds query tokens cu_q[b] .. cu_q[b + 1] - 1 and key tokens cu_k[b] .. cu_k[b + 1] - 1, either

@@ -231,3 +231,19 @@ def test_rotary_positions_stay_inside_their_buffers(gpu, tokens, H, Hk, D, axes,
             torch.cuda.synchronize()
             for name, x in b.items():
                 x.check(name)
+
+
+# ------------------------------------------------------------------------------------------------ derivatives of derivatives
+def test_a_graph_of_the_gradient_is_refused(gpu):
+    """a gradient of a gradient has no formula here: the term must not vanish from a sum whose other terms have one"""
+    from diffusion_pipe_amd import ops
+    from diffusion_pipe_amd.hip import DpipeHipError
+    q, k, v, do, cu, _ = av._inputs(gpu, [40, 30], [40, 30], 2, 1, 64)
+    q.requires_grad_(True)
+    pos = torch.arange(70, device=gpu).unsqueeze(-1)
+    for y in (ops.attention_varlen(q, k, v, cu), ops.attention_varlen(q, k[:0], v[:0], cu, torch.zeros_like(cu)), ops.rope_axes(q, None, pos, (64,))[0],
+              ops.rope_axes(q, k, pos, (64,), q_weight=torch.ones(64, device=gpu))[0]):
+        with pytest.raises(DpipeHipError, match='differentiable once'):
+            dq, = torch.autograd.grad(y, q, do, create_graph=True)
+            torch.autograd.grad(q.sum() + dq.square().sum(), q)
+        assert torch.autograd.grad(y, q, do, retain_graph=True)[0].isfinite().all()
