@@ -17,12 +17,12 @@
 // lane-local), tiles stream global -> LDS by buffer_load ... lds into a two-deep ring; rows past a sequence's end come back as zeros from the
 // buffer bounds check, whatever the neighbouring sequence holds.  Each tile has a buffer descriptor of its own, so a sequence may span more than 4 GiB.
 //
-// Bound: the matrix pipe, and with it the clock -- on long sequences the pipe is 55 - 66 % busy at 1.7 - 1.9 GHz (2.2 where it is less busy), as in a library product of 8192^3
+// Bound: the matrix pipe, and with it the clock -- on long sequences the pipe is 57 - 68 % busy at 1.7 - 1.9 GHz (2.2 where it is less busy), as in a library product of 8192^3
 // (70 % at 1.9 GHz, 1238 TFLOP/s).  TFLOP/s of the products each kernel makes (forward 2, dQ 3, dK / dV 4):
-//   15000 + 6001 tokens, 24 heads of 128         forward 2.91 ms = 1102    dQ 3.90 ms = 1232    dK / dV 5.48 ms = 1171
-//   4608 + 2560 + 1311 tokens, 24 heads of 128            357 us = 1015           490 us = 1111             665 us = 1091
-//   7 causal sequences, 9277 tokens, 32 / 8 heads of 128  246 us =  817           315 us =  957             446 us =  901
-//   4096 + 2501 + 1024 tokens, 10 heads of 64              89 us =  694           110 us =  843             151 us =  819
+//   15000 + 6001 tokens, 24 heads of 128         forward 2.93 ms = 1093    dQ 3.95 ms = 1218    dK / dV 5.53 ms = 1159
+//   4608 + 2560 + 1311 tokens, 24 heads of 128            363 us =  999           475 us = 1145             662 us = 1095
+//   7 causal sequences, 9277 tokens, 32 / 8 heads of 128  242 us =  831           308 us =  979             446 us =  901
+//   4096 + 2501 + 1024 tokens, 10 heads of 64              89 us =  694           107 us =  865             148 us =  832
 // The formulas have seven products, these kernels nine: both backward kernels make S and dP, so that dQ needs neither atomics nor a sum over fp32 parts (at 256 keys a part, len_k / 256
 // times the bytes of an fp32 dQ, written and read).
 #include <cstdio>
@@ -178,10 +178,10 @@ __device__ __forceinline__ void store_part(float* dst, const f32x16& a, float sc
 // ================================================================================================ forward
 // 128 rows per workgroup of 4 waves, two workgroups per CU: one's softmax runs under the other's products without a barrier between them (8 waves of one workgroup: 3137 us where two
 // of 4 take 2991; 64 rows a wave, one wave a SIMD: 3733; the next tile's S issued before this one's softmax within a wave: 3977).  16 + 16 products of 32 cycles a tile against
-// ~300 vector instructions: the vector pipe is 47 % busy at D = 128 and, with half the products, the first limit at D = 64.
+// ~300 vector instructions: the vector pipe is 40 - 49 % busy beside 40 - 57 % of the matrix pipe; at D = 64, with half the products, 47 beside 28.
 // A sequence of 8 key tiles or fewer is bound by what a workgroup does once -- its sequence, its rows' loads, the stores: 6 of 22 us at 9216 queries on 512 keys.
-// SPLIT, a few rows on long keys: HBM; 8 tokens on 60 354 keys, 32 / 8 heads of 128: 51 us = 4.8 TB/s from HBM, 40 us from the last-level cache.  Tiles of KR = 32 keys there, whose
-// registers and LDS leave room for three workgroups a CU (tiles of 64, two: 54 us), unless the parts are too few to fill them (2 tokens on 3000 keys: 16.3 us, with tiles of 64 15.8).
+// SPLIT, a few rows on long keys: HBM; 8 tokens on 60 354 keys, 32 / 8 heads of 128: 57 us = 4.3 TB/s from HBM, 42 us from the last-level cache.  Tiles of KR = 32 keys there, whose
+// registers and LDS leave room for three workgroups a CU (tiles of 64, two: 6 % more), unless the parts are too few to fill them (2 tokens on 3000 keys: 16.3 us, with tiles of 64 15.8).
 template <int D, bool SPLIT, int KR>
 __global__ void __launch_bounds__(NT, KR == KT ? 2 : 3) varlen_fwd_kernel(const Params p) {
     constexpr int NKB = KR / 32, NKS = D / 16, NDB = D / 32, IMG = KR * D * 2, STAGE = 2 * IMG;

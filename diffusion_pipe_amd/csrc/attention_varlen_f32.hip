@@ -4,8 +4,8 @@
 // h is that row -- P and dS go back into the matrix pipe straight from their accumulators, one entry a product.  Tiles of 32 rows, staged through registers into LDS (a bound check
 // fills the rows past a sequence with zeros); the row pitch of D + 2 floats makes the row reads (8 bytes a lane) conflict-free, and a product of 64 cycles hides them.
 //
-// Bound: the fp32 matrix pipe, 1 / 16 of the bf16 rate (an 8192^3 library product: 153 TFLOP/s).  1311 + 2560 + 4608 tokens, 24 heads of 128: forward 2.95 ms = 123 TFLOP/s, dQ 4.59 ms
-// = 118, dK / dV 6.79 ms = 107; 8 x 1024 tokens, 24 heads of 64: 0.44 / 0.62 / 0.85 ms.  What hides the staging is measured per kernel: the next tile's loads in flight over this one's
+// Bound: the fp32 matrix pipe, 1 / 16 of the bf16 rate (an 8192^3 library product: 153 TFLOP/s).  1311 + 2560 + 4608 tokens, 24 heads of 128: forward 2.92 ms = 124 TFLOP/s, dQ 4.38 ms
+// = 124, dK / dV 6.73 ms = 108; 8 x 1024 tokens, 24 heads of 64: 0.43 / 0.61 / 0.85 ms.  (The axes are cut by the estimate of the bf16 kernels.)  What hides the staging is measured per kernel: the next tile's loads in flight over this one's
 // products (forward 4.70 -> 3.23 ms, backward 14.6 -> 11.5), then two workgroups to a CU where 256 registers a lane are enough (forward 3.23 -> 2.95); dQ at D = 128 has them with no
 // loads ahead (4.59 ms, 22 registers spilled before the loop; one workgroup with loads ahead 4.68), dK / dV at D = 128 keeps K, V, dK and dV of 32 keys in registers and has one.
 #include "dpipe_common.h"
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(NT, 2) varlen_f32_dq_kernel(const Params p) {
     float dl = 0.f;                                            // delta = rowsum(dO . O)
 #pragma unroll
     for (int j = 0; j < D / 4; ++j) {
-        const float2 o = *reinterpret_cast<const float2*>(p.o + row * D + 4 * j + 2 * h);       // (a lane without a row reads the workgroup's first: its dO is 0 -- delta may be NaN, unused)
+        const float2 o = *reinterpret_cast<const float2*>(p.o + row * D + 4 * j + 2 * h);       // (a lane without a row reads its sequence's first: its dO is 0 -- delta may be NaN, unused)
         dl += d.v[j].x * o.x + d.v[j].y * o.y;
     }
     q.load(p.q + r.token * p.q_ss + r.head * p.q_sh, h, r.live);

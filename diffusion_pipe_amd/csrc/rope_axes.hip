@@ -10,7 +10,7 @@
 // rotated channels; channels behind R pass through (normalised, not rotated).
 //
 // Bound: HBM (forward reads x and writes y once, the backward of a normed row reads x and gy and writes dx).  61 456 tokens x (24 + 24) heads of 128 in bf16 with norms: forward
-// 1.51 GB in 258 us = 5.9 TB/s, backward 2.27 GB in 424 us = 5.3 TB/s (a copy of 2 GiB: 4.9); 4608 tokens of the same heads, cached: 21 us.
+// 1.51 GB in 256 us = 5.9 TB/s, backward 2.27 GB in 400 us = 5.7 TB/s (a copy of 2 GiB: 4.8); 4608 tokens of the same heads, cached: 22 us.
 // One workgroup takes up to 8 tokens: its threads make the tokens' (cos, sin) pairs in LDS once, then every head row of q and of k uses them -- the trigonometry (fp64 turns) is
 // paid once per token, not per head, and no table is read.  A head row is LPR lanes of 8 channels; the norm's sums stay inside the lane group, by operand modifiers of the add
 // instead of LDS exchanges, and 4 rows a lane group are in flight (forward 286 -> 272 us, then 258 with streaming accesses).
