@@ -392,7 +392,7 @@ int fill(RopeAxesParams& p, const char* what, const void* q, const void* k, cons
     const int groups = NB / lanes_per_row(D);
     for (int w = 0; w < 2; ++w) { const int h = p.heads[w] > 0 ? p.heads[w] : 1; p.step_t[w] = groups / h; p.step_h[w] = groups % h; }
     for (int i = 0; i < pairs; ++i) {
-        if (axis[i] < 0 || axis[i] >= axes) return bad("axis index out of range");
+        if (axis[i] < 0 || axis[i] >= axes || axis[i] > 255) return bad("axis index out of range (below axes and 256)");
         p.freq[i] = freq[i]; p.axis[i] = (unsigned char)axis[i];
     }
     p.tb = tile_tokens(tokens, pairs);

@@ -397,7 +397,7 @@ int dpipe_attn_varlen_bwd(const void* q, const void* k, const void* v, const int
  * width); diffusers FluxPosEmbed + apply_rotary_emb behind models/flux.py; hyvideo get_nd_rotary_pos_embed behind models/hunyuan_video.py:35-81)
  * q [tokens, heads_q, D], k [tokens, heads_k, D] (heads_k = 0: none), token / head strides in elements, head dim contiguous; yq, yk contiguous.  dtype bf16 or fp32, D % 8 == 0, <= 256.
  * positions [period, axes], pos_type 0 fp32, 1 int32, 2 int64; token t uses row t % period.  freq, axis: HOST arrays of `pairs` entries, copied into the launch: channel pair p turns
- * by positions[.][axis[p]] * freq[p] TURNS (one turn = 2 pi).  half = 0: pair p = channels (2 p, 2 p + 1); 1: (p, p + pairs), pairs % 4 == 0.  Channels from 2 * pairs on are not rotated.
+ * by positions[.][axis[p]] * freq[p] TURNS (one turn = 2 pi), axis[p] < axes and < 256.  half = 0: pair p = channels (2 p, 2 p + 1); 1: (p, p + pairs), pairs % 4 == 0.  Channels from 2 * pairs on are not rotated.
  * wq, wk (NULL: no norm): weight [D] of x * rsqrt(mean(x^2) + eps) * w, applied before the rotation. */
 int dpipe_rope_axes_fwd(const void* q, const void* k, const void* positions, int pos_type, const double* freq, const int* axis, const void* wq, const void* wk, void* yq,
                         void* yk, long tokens, long period, int axes, int pairs, int heads_q, int heads_k, int D, long q_ss, long q_sh, long k_ss, long k_sh, float eps,

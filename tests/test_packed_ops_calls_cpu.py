@@ -72,3 +72,14 @@ def test_cutting_refuses_no_call_that_fits_whole(sizes):
     assert 'bad output or workspace' in lib.dpipe_last_error().decode()
     assert lib.dpipe_attn_varlen_bwd(256, 256, 256, 256, 256, None, None, 256, 256, 256, 256, 256, 256, None, 0, *sizes, *strides, hq * D, D, 0.125, 0, hip.BF16, None) < 0
     assert 'bad gradient or workspace' in lib.dpipe_last_error().decode()
+
+
+def test_rope_axes_c_entry_refuses_an_axis_that_it_cannot_hold():
+    """the launch keeps an axis in 8 bits: a position column from the 257th on is refused, not taken for another"""
+    import ctypes
+    from diffusion_pipe_amd import hip
+    a = dict(q=256, k=None, pos=256, pos_type=0, freq=(ctypes.c_double * 32)(), axis=(ctypes.c_int * 32)(*[256] * 32), wq=None, wk=None, yq=None, yk=None, tokens=6, period=6, axes=400, pairs=32,
+             hq=2, hk=0, D=64, q_ss=128, q_sh=64, k_ss=0, k_sh=0, eps=1e-6, half=0, dtype=1, wq_dt=1, wk_dt=1)
+    for column, message in ((256, 'axis index'), (255, 'bad output')):        # (no output is given, so nothing is launched)
+        a['axis'] = (ctypes.c_int * 32)(*[column] * 32)
+        assert hip.lib().dpipe_rope_axes_fwd(*a.values(), None) < 0 and message in hip.lib().dpipe_last_error().decode(), column
