@@ -247,3 +247,35 @@ def test_a_graph_of_the_gradient_is_refused(gpu):
             dq, = torch.autograd.grad(y, q, do, create_graph=True)
             torch.autograd.grad(q.sum() + dq.square().sum(), q)
         assert torch.autograd.grad(y, q, do, retain_graph=True)[0].isfinite().all()
+
+
+# ------------------------------------------------------------------------------------------------ layouts
+@BOTH
+def test_any_layout_gives_the_bits_of_the_contiguous_one(gpu, dtype):
+    """heads before tokens, heads interleaved with other tensors, one head, one token, a gradient in either order, rows that overlap a wider buffer"""
+    from diffusion_pipe_amd import ops
+    lens, H, Hk, D = [70, 1, 59], 4, 2, 64
+    q, k, v, do, cu, _ = av._inputs(gpu, lens, lens, H, Hk, D, dtype=dtype)
+    base = av._run(q, k, v, do, cu, None, True)
+    heads_first = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+    interleaved = lambda t: torch.stack([t, t + 1, t - 1], dim=2)[:, :, 0]
+    wide = lambda t: torch.cat([t.flatten(1), t.flatten(1)[:, :8]], dim=1)[:, :t.shape[1] * D].unflatten(1, (t.shape[1], D))
+    for layout in (heads_first, interleaved, wide):
+        got = av._run(*(layout(t) for t in (q, k, v, do)), cu, None, True)
+        assert all(torch.equal(got[n], base[n]) for n in base)
+        pos = torch.arange(130, device=gpu).unsqueeze(-1) % 70
+        w = torch.linspace(0.5, 1.5, D, device=gpu)
+        for weight in (w, None):
+            want = ops.rope_axes(q, k, pos, (48,), q_weight=weight, k_weight=weight)
+            got = ops.rope_axes(layout(q), layout(k), pos, (48,), q_weight=weight, k_weight=weight)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            batch = lambda t: torch.stack([t[:65], t[65:]])                  # [2, 65, H, D], heads first inside a sample
+            got = ops.rope_axes(batch(q).transpose(1, 2).contiguous().transpose(1, 2), batch(k), pos.view(2, 65, 1), (48,), q_weight=weight, k_weight=weight)
+            assert all(torch.equal(a.flatten(0, 1), b) for a, b in zip(got, want))
+    one = av._run(q[:, :1], k[:, :1], v[:, :1], do[:, :1], cu, None, True)
+    same = av._run(*(t[:, :1].contiguous() for t in (q, k, v, do)), cu, None, True)
+    assert all(torch.equal(one[n], same[n]) for n in one)
+    cu1 = torch.tensor([0, 1], dtype=torch.int32, device=gpu)
+    one = av._run(*(heads_first(t)[5:6] for t in (q, k, v, do)), cu1, None, False)
+    same = av._run(*(t[5:6].contiguous() for t in (q, k, v, do)), cu1, None, False)
+    assert all(torch.equal(one[n], same[n]) for n in one)
