@@ -7,7 +7,7 @@
 // Bound: the fp32 matrix pipe, 1 / 16 of the bf16 rate (an 8192^3 library product: 153 TFLOP/s).  1311 + 2560 + 4608 tokens, 24 heads of 128: forward 2.92 ms = 124 TFLOP/s, dQ 4.38 ms
 // = 124, dK / dV 6.73 ms = 108; 8 x 1024 tokens, 24 heads of 64: 0.43 / 0.61 / 0.85 ms.  (The axes are cut by the estimate of the bf16 kernels.)  What hides the staging is measured per kernel: the next tile's loads in flight over this one's
 // products (forward 4.70 -> 3.23 ms, backward 14.6 -> 11.5), then two workgroups to a CU where 256 registers a lane are enough (forward 3.23 -> 2.95); dQ at D = 128 has them with no
-// loads ahead (4.59 ms, 22 registers spilled before the loop; one workgroup with loads ahead 4.68), dK / dV at D = 128 keeps K, V, dK and dV of 32 keys in registers and has one.
+// loads ahead (4.38 - 4.59 ms, 22 registers spilled, 10 scratch accesses beside a tile's 192 products; one workgroup with loads ahead 4.68), dK / dV at D = 128 keeps K, V, dK and dV of 32 keys in registers and has one.
 #include "dpipe_common.h"
 #include "attention_tiles.h"
 #include "attention_varlen.h"
